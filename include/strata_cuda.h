@@ -58,7 +58,8 @@ enum {
   SC_ERR_UNSUPPORTED = -8, /* a combination this build does not take (caller falls back)     */
   SC_ERR_TIMEOUT = -9,     /* recorded by a kernel: a bounded wait gave up                    */
   SC_ERR_INDEX = -10,      /* recorded by a kernel: an expert id >= the number of experts    */
-  SC_ERR_SCRATCH = -11     /* the call needs more scratch than SC_NOALLOC_SCRATCH_BYTES       */
+  SC_ERR_SCRATCH = -11,    /* the call needs more scratch than SC_NOALLOC_SCRATCH_BYTES       */
+  SC_ERR_PAGE = -12        /* recorded by a kernel: a page id or a length outside the cache   */
 };
 
 /* library version (SC_ABI_VERSION) */
@@ -294,6 +295,80 @@ SC_API int sc_add_rmsnorm(void* x, const void* delta, const void* w, int rows, i
 SC_API int sc_rope_cache(void* q, const void* k, const void* v, int tokens, int q_heads, int kv_heads, int head_dim,
                          const float* cos, const float* sin, const int32_t* pos, const int32_t* block_table, int page,
                          void* k_cache, void* v_cache, int dtype, void* stream);
+
+/* What a decoder keeps of its context (no counterpart in strata-mlx's MoE path). A paged key/value cache of a batch of
+ * sequences: sequence b's slot s is token s % page of page table[b * table_row + s / page] of the pools k and v, and its
+ * first lengths[b] slots hold tokens. Strides count elements; a head's head_dim values are adjacent. `lengths` is
+ * read on the device, so that a step replays from a CUDA graph. weight and position (batch rows of max_pages x page
+ * slots) are optional to sc_decode_attention, position is not used by it; sc_evict needs both. */
+typedef struct sc_kv_pages {
+  void *k, *v;                   /* pools of pool_pages pages, bfloat16 or float16, 16-byte aligned               */
+  int64_t k_page, k_token, k_head; /* strides, multiples of 8                                                     */
+  int64_t v_page, v_token, v_head;
+  const int32_t* table;          /* (batch, max_pages) page ids, rows table_row apart                              */
+  int64_t table_row;
+  const int32_t* lengths;        /* (batch) slots in use                                                           */
+  float* weight;                 /* (batch, max_pages * page) attention weight each slot gathered, or NULL          */
+  int64_t weight_row;
+  int32_t* position;             /* (batch, max_pages * page) the position of each slot's token, or NULL            */
+  int64_t position_row;
+  int batch, kv_heads, head_dim, page, pool_pages, max_pages, dtype; /* page a power of two                         */
+} sc_kv_pages;
+
+/* Attention of one new token a sequence over its cache: out[b, h] = sum_s p[s] v[s, h / (q_heads / kv_heads)] with
+ * p = softmax over s < lengths[b] of scale q[b, h] . k[s]; zeros where lengths[b] is 0. q (batch, q_heads, head_dim)
+ * with strides q_row, q_head (multiples of 8, 16-byte aligned); out the same shape, contiguous, of q's type. Where
+ * kv->weight is not NULL, weight[b, s] += sum over the query heads of p[s]. Softmax statistics and sums in float32,
+ * the same bits on every run. head_dim a multiple of 8, at most 256; q_heads a multiple of kv_heads. Slots past a
+ * length are never read. A page id outside the pool or a length outside the table records SC_ERR_PAGE in err; such
+ * slots are left out. workspace: sc_decode_attention_workspace bytes, 16-byte aligned, not shared by calls that may
+ * overlap. */
+SC_API int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t q_row, int64_t q_head, int q_heads,
+                               float scale, void* out, void* workspace, size_t workspace_bytes, int* err, void* stream);
+SC_API size_t sc_decode_attention_workspace(const sc_kv_pages* kv, int q_heads);
+
+/* Eviction by accumulated attention weight: each sequence with more than `keep` tokens keeps `keep` of them -- first
+ * those at position < sinks or >= seen[b] - recent, then the others, each class by weight, the largest first (a NaN
+ * counts as the largest), equal weights by the lower slot -- and its kept tokens move to slots 0 .. keep - 1: the kept
+ * tokens at slots >= keep, in slot order, into the evicted slots < keep, in slot order; all other kept tokens stay
+ * where they are, since attention does not go by slot order. k and v move in place. weight_out and position_out
+ * (rows of at least min(keep, slots) values) get the first min(keep, length) slots' values, lengths_out the new
+ * lengths; each may be the cache's own array. Sequences within the budget keep all. workspace: sc_evict_workspace
+ * bytes, 16-byte aligned. Errors as sc_decode_attention. */
+SC_API int sc_evict(const sc_kv_pages* kv, const int32_t* seen, int keep, int sinks, int recent, float* weight_out,
+                    int64_t weight_out_row, int32_t* position_out, int64_t position_out_row, int32_t* lengths_out,
+                    void* workspace, size_t workspace_bytes, int* err, void* stream);
+SC_API size_t sc_evict_workspace(const sc_kv_pages* kv, int keep);
+
+/* Linear attention with a decay a head and token. With S a head's state (k_dim, v_dim),
+ *   S_t = exp(decay_t) S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t.
+ * q, k (batch, tokens, k_heads, k_dim), v (batch, tokens, v_heads, v_dim), bfloat16 or float16, the last axis
+ * adjacent; value head h reads key head h / (v_heads / k_heads). decay (batch, tokens, v_heads) float32 logarithms
+ * (0 keeps, -inf forgets), any strides, 0 among them. state_in (batch, v_heads, k_dim, v_dim) float32 contiguous, or
+ * NULL for zeros; state_out the same shape (may be state_in). lengths (batch) on the device, or NULL: tokens past a
+ * sequence's length are not read and their outputs are zeros. out (batch, tokens, v_heads, v_dim) contiguous, of q's
+ * type. k_dim and v_dim multiples of 8, at most 128. Strides of q, k, v multiples of 8, pointers 16-byte aligned. */
+typedef struct sc_linear {
+  const void *q, *k, *v;
+  const float* decay;
+  const float* state_in;
+  float* state_out;
+  const int32_t* lengths;
+  void* out;
+  int64_t q_row, q_token, q_head; /* strides in elements: batch, token, head */
+  int64_t k_row, k_token, k_head;
+  int64_t v_row, v_token, v_head;
+  int64_t decay_row, decay_token, decay_head;
+  int batch, tokens, k_heads, v_heads, k_dim, v_dim, dtype;
+  float scale;
+} sc_linear;
+
+/* Prompts: any number of tokens, the state carried in float32. workspace: sc_linear_attention_workspace bytes. */
+SC_API int sc_linear_attention(const sc_linear* a, void* workspace, size_t workspace_bytes, int* err, void* stream);
+SC_API size_t sc_linear_attention_workspace(const sc_linear* a);
+
+/* One token a sequence (tokens = 1, lengths NULL): the recurrence itself. */
+SC_API int sc_linear_attention_step(const sc_linear* a, void* stream);
 
 /* No counterpart in strata-mlx: an addition for callers that cannot allocate device memory.
  *

@@ -25,7 +25,7 @@ ABI_VERSION = 1
 
 ERRORS = {-1: "SC_ERR_KIND", -2: "SC_ERR_SHAPE", -3: "SC_ERR_DTYPE", -4: "SC_ERR_ALIGN", -5: "SC_ERR_ARG",
           -6: "SC_ERR_CUDA", -7: "SC_ERR_WORKSPACE", -8: "SC_ERR_UNSUPPORTED", -9: "SC_ERR_TIMEOUT",
-          -10: "SC_ERR_INDEX", -11: "SC_ERR_SCRATCH"}
+          -10: "SC_ERR_INDEX", -11: "SC_ERR_SCRATCH", -12: "SC_ERR_PAGE"}
 
 # every symbol include/strata_cuda.h declares, with its ctypes signature
 _P, _I, _I64, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
@@ -72,6 +72,13 @@ SIGNATURES = {
     "sc_paged_attention_workspace": (_SZ, [_I, _I]),
     "sc_add_rmsnorm": (_I, [_P, _P, _P, _I, _I, ctypes.c_float, _I, _P, _P]),
     "sc_rope_cache": (_I, [_P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _I, _P]),
+    "sc_decode_attention": (_I, [_P, _P, _I64, _I64, _I, ctypes.c_float, _P, _P, _SZ, _P, _P]),
+    "sc_decode_attention_workspace": (_SZ, [_P, _I]),
+    "sc_evict": (_I, [_P, _P, _I, _I, _I, _P, _I64, _P, _I64, _P, _P, _SZ, _P, _P]),
+    "sc_evict_workspace": (_SZ, [_P, _I]),
+    "sc_linear_attention": (_I, [_P, _P, _SZ, _P, _P]),
+    "sc_linear_attention_workspace": (_SZ, [_P]),
+    "sc_linear_attention_step": (_I, [_P, _P]),
     "sc_moe_decode_layer_noalloc": (_I, [_P, _P, _I, _P, _P]),
     "sc_moe_decode_noalloc_error": (_I, [ctypes.POINTER(_I), _P]),
 }
@@ -91,6 +98,23 @@ class SCLayer(ctypes.Structure):
                 ("gate", _P), ("up", _P), ("down", _P), ("router", _P),
                 ("shared_inter", _I), ("kind_sgate", _I), ("kind_sup", _I), ("kind_sdown", _I),
                 ("sgate", _P), ("sup", _P), ("sdown", _P), ("shared_gate", _P), ("dtype", _I)]
+
+
+class SCPages(ctypes.Structure):
+    """sc_kv_pages (include/strata_cuda.h): a batch's paged key/value cache."""
+    _fields_ = [("k", _P), ("v", _P), ("k_page", _I64), ("k_token", _I64), ("k_head", _I64), ("v_page", _I64),
+                ("v_token", _I64), ("v_head", _I64), ("table", _P), ("table_row", _I64), ("lengths", _P),
+                ("weight", _P), ("weight_row", _I64), ("position", _P), ("position_row", _I64), ("batch", _I),
+                ("kv_heads", _I), ("head_dim", _I), ("page", _I), ("pool_pages", _I), ("max_pages", _I), ("dtype", _I)]
+
+
+class SCLinear(ctypes.Structure):
+    """sc_linear (include/strata_cuda.h): a linear attention call."""
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("decay", _P), ("state_in", _P), ("state_out", _P), ("lengths", _P),
+                ("out", _P), ("q_row", _I64), ("q_token", _I64), ("q_head", _I64), ("k_row", _I64), ("k_token", _I64),
+                ("k_head", _I64), ("v_row", _I64), ("v_token", _I64), ("v_head", _I64), ("decay_row", _I64),
+                ("decay_token", _I64), ("decay_head", _I64), ("batch", _I), ("tokens", _I), ("k_heads", _I),
+                ("v_heads", _I), ("k_dim", _I), ("v_dim", _I), ("dtype", _I), ("scale", ctypes.c_float)]
 
 
 _lib = None

@@ -1,0 +1,236 @@
+"""What a decoder keeps of its context, for a batch of sequences: a paged key/value cache that can be held to a budget,
+and linear attention, whose state has one size at any length. The reference's engine keeps both kinds
+(strata_mlx/engine.py:276-279 runs a trunk of linear and of full attention layers around the MoE blocks); these are
+the operators for such a trunk on the B200.
+
+    KVPages                 a batch's cache: pools of pages, a table and a length a sequence
+      .attend(q)            attention of one new token a sequence; the weights each slot gathers, on request
+      .evict(seen, keep)    keeps the tokens with the most weight and moves them to the front of the cache, in place
+    decode_attention        KVPages(...).attend(q) for a single call
+    linear_attention        S_t = exp(g_t) S_{t-1} + k_t v_t^T, out_t = scale q_t S_t over a prompt
+    linear_attention_step   the same for one token a sequence, the state in place
+
+Every call enqueues on the current CUDA stream and returns; nothing is read back. Activations are bfloat16 or
+float16; softmax statistics, accumulated weights and states are float32.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import check, ptr, require_cuda, stream
+
+_TYPES = {torch.float16: 1, torch.bfloat16: 2}  # SC_F16, SC_BF16
+
+
+def _here(*ts) -> torch.device:
+    """The device all the tensors are on, which has to be the current one: calls go to its current stream."""
+    require_cuda(*ts)
+    device = ts[0].device
+    for t in ts:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}")
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+    return device
+
+
+def _ints(name: str, t: torch.Tensor, shape: tuple) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous int32 {shape} expected, got {t.dtype} {tuple(t.shape)}")
+
+
+class KVPages:
+    """A batch's paged key/value cache (one layer's). k, v (pages, page, kv_heads, head_dim) bfloat16 or float16, of
+    any strides with the last axis adjacent; table (batch, max_pages) int32, sequence b's slot s in page
+    table[b, s // page] (rows may be views, and the same row may serve several sequences that only read); lengths
+    (batch,) int32, the slots in use. weight (batch, >= max_pages * page) float32 gathers each slot's attention
+    weight; position, the same shape int32, holds the position of each slot's token (evict needs both). The tensors
+    stay the caller's: the object keeps references and reads lengths and table on the device at every call, so that
+    steps replay from a CUDA graph. Calls on one stream may follow each other freely; each stream has a workspace of
+    its own."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+                 weight: torch.Tensor | None = None, position: torch.Tensor | None = None):
+        self.device = _here(k, v, table, lengths, weight, position)
+        if k.dtype not in _TYPES or v.dtype != k.dtype:
+            raise ValueError(f"k and v both bfloat16 or both float16 expected, got {k.dtype} and {v.dtype}")
+        if k.dim() != 4 or k.shape != v.shape or k.stride(-1) != 1 or v.stride(-1) != 1:
+            raise ValueError(f"k and v (pages, page, kv_heads, head_dim) with the last axis adjacent expected, got "
+                             f"{tuple(k.shape)} and {tuple(v.shape)}")
+        if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
+            raise ValueError("table: int32 (batch, max_pages) with adjacent rows expected")
+        self.batch, self.max_pages = table.shape
+        _ints("lengths", lengths, (self.batch,))
+        self.slots = self.max_pages * k.shape[1]
+        for name, t, dtype in (("weight", weight, torch.float32), ("position", position, torch.int32)):
+            if t is not None and (t.dtype != dtype or t.dim() != 2 or t.shape[0] != self.batch or t.stride(1) != 1
+                                  or t.shape[1] < self.slots):
+                raise ValueError(f"{name}: {dtype} ({self.batch}, at least {self.slots}) expected")
+        self.k, self.v, self.table, self.lengths, self.weight, self.position = k, v, table, lengths, weight, position
+        self.dtype, self.kv_heads, self.head_dim = k.dtype, k.shape[2], k.shape[3]
+        P = _lib.SCPages()
+        P.k, P.v, P.table, P.lengths = ptr(k), ptr(v), ptr(table), ptr(lengths)
+        P.k_page, P.k_token, P.k_head = k.stride()[:3]
+        P.v_page, P.v_token, P.v_head = v.stride()[:3]
+        P.table_row = table.stride(0)
+        P.weight, P.position = ptr(weight), ptr(position)
+        P.weight_row = 0 if weight is None else weight.stride(0)
+        P.position_row = 0 if position is None else position.stride(0)
+        P.batch, P.kv_heads, P.head_dim, P.page = self.batch, self.kv_heads, self.head_dim, k.shape[1]
+        P.pool_pages, P.max_pages, P.dtype = k.shape[0], self.max_pages, _TYPES[k.dtype]
+        self._pages, self._ref = P, ctypes.addressof(P)
+        self._lib, self._err = _lib.lib(), ptr(_lib.error_word(self.device))
+        self._ws: dict = {}
+
+    def _workspace(self, what: tuple, s: int, size) -> tuple:
+        """The workspace of a kind of call on stream s: its address and bytes (fresh in a capture, whose memory is
+        the graph's)."""
+        ws = self._ws.get((s, *what))
+        if ws is None or torch.cuda.is_current_stream_capturing():
+            n = size()
+            if n == 0:
+                raise ValueError(f"{what[0]}: this cache or these arguments are not taken (head_dim a multiple of 8 up "
+                                 "to 256, a power-of-two page, query heads a multiple of the cache's)")
+            t = torch.empty(n, dtype=torch.uint8, device=self.device)
+            ws = (t.data_ptr(), n, t)
+            if not torch.cuda.is_current_stream_capturing():
+                self._ws[(s, *what)] = ws
+        return ws
+
+    def attend(self, q: torch.Tensor, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """softmax(scale q k^T) v of one new token a sequence: q (batch, q_heads, head_dim), out the same. The token's
+        own key and value are in the cache already. scale defaults to head_dim ** -0.5. A sequence of length 0 gives
+        zeros. With `weight`, every slot's probability, summed over the query heads, is added to it."""
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != self.batch or shape[2] != self.head_dim or q.dtype != self.dtype:
+            raise ValueError(f"q ({self.batch}, q_heads, {self.head_dim}) {self.dtype} expected, got {tuple(shape)} "
+                             f"{q.dtype}")
+        if q.device != self.device or torch.cuda.current_device() != self.device.index:
+            raise ValueError(f"q on {q.device}; the cache is on {self.device}, which has to be current")
+        if q.stride(2) != 1:
+            q = q.contiguous()
+        if out is None:
+            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+        elif out.shape != shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous():
+            raise ValueError(f"out: contiguous {tuple(shape)} {q.dtype} expected")
+        s, heads = stream(), shape[1]
+        ws = self._workspace(("attend", heads), s,
+                             lambda: self._lib.sc_decode_attention_workspace(self._ref, heads))
+        check(self._lib.sc_decode_attention(self._ref, q.data_ptr(), q.stride(0), q.stride(1), heads,
+                                            self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), ws[0],
+                                            ws[1], self._err, s), "decode_attention")
+        return out
+
+    def evict(self, seen: torch.Tensor, keep: int, sinks: int = 4, recent: int = 0, out: tuple | None = None) -> None:
+        """Keeps `keep` tokens of every longer sequence: those at positions below `sinks` or within the last `recent`
+        of the seen[b] positions the sequence has had, then those with the most weight (equal ones: the lower slot).
+        The kept tokens beyond the budget move into the slots of evicted ones, keys, values, weight and position;
+        lengths becomes min(length, keep). out: (weight, position, lengths) tensors that get the first min(keep,
+        length) slots' values and the lengths in place of the cache's own (layers that share one `lengths` each need
+        theirs until all are done). Slots past the new length keep what they held."""
+        if self.weight is None or self.position is None:
+            raise ValueError("evict needs the cache's weight and position")
+        _here(self.k, seen)
+        _ints("seen", seen, (self.batch,))
+        weight, position, lengths = (self.weight, self.position, self.lengths) if out is None else out
+        _here(self.k, weight, position, lengths)
+        for name, t, dtype in (("weight", weight, torch.float32), ("position", position, torch.int32)):
+            if (t.dtype != dtype or t.dim() != 2 or t.shape[0] != self.batch or t.stride(1) != 1
+                    or t.shape[1] < min(keep, self.slots)):
+                raise ValueError(f"out {name}: {dtype} ({self.batch}, at least {min(keep, self.slots)}) expected")
+        _ints("out lengths", lengths, (self.batch,))
+        s = stream()
+        if keep < 0 or sinks < 0 or recent < 0 or sinks + recent > keep:
+            raise ValueError(f"sinks {sinks} and recent {recent} have to fit in keep {keep}")
+        ws = self._workspace(("evict", keep), s, lambda: self._lib.sc_evict_workspace(self._ref, keep))
+        check(self._lib.sc_evict(self._ref, seen.data_ptr(), keep, sinks, recent, weight.data_ptr(), weight.stride(0),
+                                 position.data_ptr(), position.stride(0), lengths.data_ptr(), ws[0], ws[1], self._err,
+                                 s), "evict")
+
+
+def decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+                     scale: float | None = None, weight: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """KVPages(k, v, table, lengths, weight).attend(q, scale, out): attention of one new token a sequence."""
+    return KVPages(k, v, table, lengths, weight).attend(q, scale, out)
+
+
+def _linear(q, k, v, decay, state, scale) -> tuple:
+    """The checked call as an SCLinear without its outputs, and what has to stay alive until it is enqueued."""
+    device = _here(q, k, v, decay, state)
+    if q.dtype not in _TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k and v all bfloat16 or all float16 expected, got {q.dtype}, {k.dtype}, {v.dtype}")
+    lead = tuple(q.shape[:-2])
+    if k.shape != q.shape or tuple(v.shape[:-2]) != lead or q.shape[-2] == 0 or v.shape[-2] % q.shape[-2]:
+        raise ValueError(f"q and k alike, v of the same tokens with a multiple of their heads expected, got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    hv, dk, dv = v.shape[-2], q.shape[-1], v.shape[-1]
+    if decay.dtype != torch.float32 or tuple(decay.shape) != (*lead, hv):
+        raise ValueError(f"decay: float32 {(*lead, hv)} expected, got {decay.dtype} {tuple(decay.shape)}")
+    if state is not None and (state.dtype != torch.float32 or tuple(state.shape) != (lead[0], hv, dk, dv)
+                              or not state.is_contiguous()):
+        raise ValueError(f"state: contiguous float32 {(lead[0], hv, dk, dv)} expected")
+    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+    A = _lib.SCLinear()
+    A.q, A.k, A.v, A.decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr()
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        st = t.stride()
+        setattr(A, name + "_row", st[0])
+        setattr(A, name + "_head", st[-2])
+        if len(lead) == 2:
+            setattr(A, name + "_token", st[1])
+    st = decay.stride()
+    A.decay_row, A.decay_head = st[0], st[-1]
+    if len(lead) == 2:
+        A.decay_token = st[1]
+    A.batch, A.tokens = lead[0], lead[1] if len(lead) == 2 else 1
+    A.k_heads, A.v_heads, A.k_dim, A.v_dim, A.dtype = q.shape[-2], hv, dk, dv, _TYPES[q.dtype]
+    A.scale = dk ** -0.5 if scale is None else scale
+    return A, (q, k, v), device
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
+                     state: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                     scale: float | None = None) -> tuple:
+    """A prompt (or a chunk of one) through linear attention: S_t = exp(decay_t) S_{t-1} + k_t v_t^T, out_t = scale
+    q_t S_t. q, k (batch, tokens, k_heads, k_dim), v (batch, tokens, v_heads, v_dim): value head h reads key head
+    h // (v_heads / k_heads); k_dim and v_dim multiples of 8 up to 128. decay (batch, tokens, v_heads) float32
+    logarithms, of any strides (a fixed decay a head is an expanded view). state (batch, v_heads, k_dim, v_dim)
+    float32, zeros when None, is left as it was. lengths (batch,) int32: tokens past a sequence's length are not read,
+    their outputs zeros. scale defaults to k_dim ** -0.5. Returns (out of v's shape, the state after the last token)."""
+    if q.dim() != 4 or v.dim() != 4:
+        raise ValueError("q, k, v (batch, tokens, heads, dim) expected")
+    A, keep, device = _linear(q, k, v, decay, state, scale)
+    if lengths is not None:
+        _here(q, lengths)
+        _ints("lengths", lengths, (A.batch,))
+        A.lengths = lengths.data_ptr()
+    out = torch.empty(v.shape, dtype=v.dtype, device=device)
+    new = torch.empty((A.batch, A.v_heads, A.k_dim, A.v_dim), dtype=torch.float32, device=device)
+    A.state_in, A.state_out, A.out = ptr(state), new.data_ptr(), out.data_ptr()
+    lib, ref = _lib.lib(), ctypes.addressof(A)
+    n = lib.sc_linear_attention_workspace(ref)
+    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+    check(lib.sc_linear_attention(ref, ws.data_ptr(), n, ptr(_lib.error_word(device)), stream()), "linear_attention")
+    return out, new
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
+                          scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """linear_attention for one token a sequence: q, k (batch, k_heads, k_dim), v (batch, v_heads, v_dim), decay (batch,
+    v_heads); state (batch, v_heads, k_dim, v_dim) float32 is updated in place. Returns out (batch, v_heads, v_dim)."""
+    if q.dim() != 3 or v.dim() != 3 or state is None:
+        raise ValueError("q, k, v (batch, heads, dim) and a state expected")
+    A, keep, device = _linear(q, k, v, decay, state, scale)
+    if out is None:
+        out = torch.empty(v.shape, dtype=v.dtype, device=device)
+    elif out.shape != v.shape or out.dtype != v.dtype or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out: contiguous {tuple(v.shape)} {v.dtype} expected")
+    A.state_in = A.state_out = state.data_ptr()
+    A.out = out.data_ptr()
+    check(_lib.lib().sc_linear_attention_step(ctypes.addressof(A), stream()), "linear_attention_step")
+    return out

@@ -1,0 +1,109 @@
+// Linear attention with a decay a head and token (sc_linear_attention, sc_linear_attention_step): the recurrence
+//   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t
+// as it stands. A block per (sequence, value head, 32 value dimensions) holds its columns of S in registers, a thread
+// 1/8 of a column, and walks the tokens; the eight parts of o_t meet in shared memory.
+#include "common.cuh"
+
+namespace sc {
+namespace la {
+
+constexpr int COLS = 32, PARTS = 8, MAXK = 128, PER = MAXK / PARTS;
+
+template <typename T>
+__global__ void __launch_bounds__(COLS * PARTS) recurrent_kernel(const sc_linear A) {
+  __shared__ float s_q[MAXK], s_k[MAXK], s_o[PARTS][COLS];
+  const int h = blockIdx.x, b = blockIdx.y, hk = h / (A.v_heads / A.k_heads);
+  const int col = blockIdx.z * COLS + threadIdx.x % COLS, part = threadIdx.x / COLS;
+  const bool live = col < A.v_dim;
+  int n = A.tokens;
+  if (A.lengths) n = min(max(A.lengths[b], 0), n);
+  const int64_t at = (int64_t(b) * A.v_heads + h) * A.k_dim * A.v_dim + col;
+  float S[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = part + PARTS * i;
+    S[i] = live && r < A.k_dim && A.state_in ? A.state_in[at + int64_t(r) * A.v_dim] : 0.f;
+  }
+  T* out = static_cast<T*>(A.out) + (int64_t(b) * A.tokens * A.v_heads + h) * A.v_dim + col;
+  for (int t = 0; t < n; ++t) {
+    if (threadIdx.x < MAXK) {
+      const int d = threadIdx.x;
+      const bool in = d < A.k_dim;
+      s_q[d] = in ? to_f32(static_cast<const T*>(A.q)[b * A.q_row + t * A.q_token + hk * A.q_head + d]) * A.scale : 0.f;
+      s_k[d] = in ? to_f32(static_cast<const T*>(A.k)[b * A.k_row + t * A.k_token + hk * A.k_head + d]) : 0.f;
+    }
+    const float v = live ? to_f32(static_cast<const T*>(A.v)[b * A.v_row + t * A.v_token + h * A.v_head + col]) : 0.f;
+    // exp(g) - 1: near 1 the decay itself would carry a rounding that every later token repeats
+    const float a1 = expm1f(A.decay[b * A.decay_row + t * A.decay_token + h * A.decay_head]);
+    __syncthreads();
+    float o = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = part + PARTS * i;
+      S[i] = fmaf(s_k[r], v, fmaf(a1, S[i], S[i]));
+      o = fmaf(s_q[r], S[i], o);
+    }
+    s_o[part][threadIdx.x % COLS] = o;
+    __syncthreads();
+    if (part == 0 && live) {
+      float r = 0.f;
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) r += s_o[i][threadIdx.x];
+      out[int64_t(t) * A.v_heads * A.v_dim] = from_f32<T>(r);
+    }
+  }
+  if (live && part == 0)
+    for (int t = n; t < A.tokens; ++t) out[int64_t(t) * A.v_heads * A.v_dim] = from_f32<T>(0.f);
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = part + PARTS * i;
+    if (live && r < A.k_dim) A.state_out[at + int64_t(r) * A.v_dim] = S[i];
+  }
+}
+
+inline int check(const sc_linear* a) {
+  if (!a || a->batch < 0 || a->tokens < 0 || (a->batch && !a->state_out) ||
+      (a->batch && a->tokens && (!a->q || !a->k || !a->v || !a->decay || !a->out)))
+    return SC_ERR_ARG;
+  if (a->dtype != SC_F16 && a->dtype != SC_BF16) return SC_ERR_DTYPE;
+  if (a->k_heads < 1 || a->v_heads < 1 || a->v_heads % a->k_heads || a->k_dim < 8 || a->k_dim % 8 || a->k_dim > MAXK ||
+      a->v_dim < 8 || a->v_dim % 8 || a->v_dim > 128 || a->batch > 65535)
+    return SC_ERR_SHAPE;
+  const int64_t strides = a->q_row | a->q_token | a->q_head | a->k_row | a->k_token | a->k_head | a->v_row | a->v_token |
+                          a->v_head;
+  const uintptr_t p = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) |
+                      reinterpret_cast<uintptr_t>(a->v) | reinterpret_cast<uintptr_t>(a->out) |
+                      reinterpret_cast<uintptr_t>(a->state_in) | reinterpret_cast<uintptr_t>(a->state_out);
+  if ((strides & 7) || (p & 15)) return SC_ERR_ALIGN;
+  return SC_OK;
+}
+
+int launch(const sc_linear& a, void* stream) {
+  if (a.batch == 0) return SC_OK;
+  const dim3 grid(unsigned(a.v_heads), unsigned(a.batch), unsigned((a.v_dim + COLS - 1) / COLS));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a.dtype == SC_BF16) recurrent_kernel<__nv_bfloat16><<<grid, COLS * PARTS, 0, s>>>(a);
+  else recurrent_kernel<__half><<<grid, COLS * PARTS, 0, s>>>(a);
+  if (cudaError_t e = cudaGetLastError()) return cuda_failed(e, "linear attention launch");
+  return SC_OK;
+}
+
+}  // namespace la
+}  // namespace sc
+
+using namespace sc;
+
+extern "C" size_t sc_linear_attention_workspace(const sc_linear* a) { return la::check(a) ? 0 : 16; }
+
+extern "C" int sc_linear_attention(const sc_linear* a, void* workspace, size_t workspace_bytes, int* err, void* stream) {
+  if (int rc = la::check(a)) return rc;
+  if (!workspace) return SC_ERR_ARG;
+  if (workspace_bytes < sc_linear_attention_workspace(a)) return SC_ERR_WORKSPACE;
+  return la::launch(*a, stream);
+}
+
+extern "C" int sc_linear_attention_step(const sc_linear* a, void* stream) {
+  if (int rc = la::check(a)) return rc;
+  if (a->tokens != 1 || a->lengths) return SC_ERR_SHAPE;
+  return la::launch(*a, stream);
+}
