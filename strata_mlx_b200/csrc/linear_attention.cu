@@ -33,14 +33,17 @@ __global__ void __launch_bounds__(COLS * PARTS) recurrent_kernel(const sc_linear
       s_k[d] = in ? to_f32(static_cast<const T*>(A.k)[b * A.k_row + t * A.k_token + hk * A.k_head + d]) : 0.f;
     }
     const float v = live ? to_f32(static_cast<const T*>(A.v)[b * A.v_row + t * A.v_token + h * A.v_head + col]) : 0.f;
-    // exp(g) - 1: near 1 the decay itself would carry a rounding that every later token repeats
-    const float a1 = expm1f(A.decay[b * A.decay_row + t * A.decay_token + h * A.decay_head]);
+    // S + (exp(g) - 1) S: near 1 the decay itself would carry a rounding that every later token repeats. A decay
+    // below 1/2 multiplies S alone, or the difference would cancel.
+    const float g = A.decay[b * A.decay_row + t * A.decay_token + h * A.decay_head];
+    const bool near = g > -0.69314718f;
+    const float a = near ? expm1f(g) : expf(g), one = near ? 1.f : 0.f;
     __syncthreads();
     float o = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int r = part + PARTS * i;
-      S[i] = fmaf(s_k[r], v, fmaf(a1, S[i], S[i]));
+      S[i] = fmaf(s_k[r], v, fmaf(a, S[i], one * S[i]));
       o = fmaf(s_q[r], S[i], o);
     }
     s_o[part][threadIdx.x % COLS] = o;
