@@ -1,103 +1,540 @@
 // Attention of one new token a sequence over a batch's paged cache, the weights accumulated on request
-// (sc_decode_attention). A block per (sequence, query head): its warps take the slots in turn, each with an online
-// softmax of its own (running maximum m, sum l and output o, rescaled by 2^(m - m') when the maximum moves), joined in
-// shared memory. With weights, a second kernel takes 2^(s - m) / l of every head at each slot.
+// (sc_decode_attention): o = sum_s p_s v_s, p = softmax_s(scale q . k_s). Every key and value is read once, so the
+// cache's bytes bound it; what the kernel has to do is keep enough of them in flight.
+//
+//   attend_kernel  The batch's caches are cut into units of 64 slots or more (a tile a warp), counted over sequence,
+//                  key/value head and slot, and every block takes an equal run of units: ragged lengths balance, and
+//                  a long cache spreads over all SMs. A block joins its warps' results in shared memory; a run that
+//                  covers a head's whole length writes the output, the others partial results (at most two a block).
+//   join_kernel    joins the partial results in block order (the same bits on every run), and adds the weights.
+//
+// A warp's tile goes from memory straight into tensor-core fragments (mma.sync m16n8k16; up to eight query heads share
+// the key/value head, so a product of 16 slots by 8 heads has little padding, and 128-row tcgen05 products would
+// have nothing to fill them). The order of a sum's terms is free, so each lane takes 16-byte pieces of rows:
+//   scores   S^T = K Q^T, 16 slots by 8 heads: lane (g, t) holds dims 8 (4 j + t) .. + 7 of slots g and g + 8, four
+//            dims to a product; Q is laid out the same way;
+//   values   O^T = V^T P^T, 16 dims by 8 heads: the lane holds dims 64 i + 8 g .. + 7 of slots 2t, 2t + 1, 2t + 8 and
+//            2t + 9, paired by byte permutes; the scores' accumulators become P^T's fragments by movmatrix.
+// The softmax is online: scores are taken relative to a running maximum a head, moved only when a score passes it by
+// 2^8 (a vote a tile instead of a reduction; float32 holds the larger probabilities as exactly). A probability enters
+// the value product as two terms of the activations' type (its rounding and the rest), so that only the output is
+// rounded to 16 bits. The next tile's keys load while this tile's softmax and value product run, its values after.
+#include <algorithm>
 #include <type_traits>
 
+#include "mma_decode.cuh"
 #include "pages.cuh"
 
 namespace sc {
 namespace da {
 
-constexpr int WARPS = 8;
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int HEADS = 8;       // query heads of a block: the products' N
+constexpr int BLOCKS_PER_SM = 2;
+constexpr int SMS = 148;
+constexpr float SLACK = 8.f;   // log2 by which a score may pass the running maximum
+constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_SLOTS = 1024;  // slots of a weight block
 
 struct Args {
   Pages pages;
   const void* q;
   int64_t q_row, q_head;
-  int q_heads, group, dim;
+  int batch, q_heads, kv_heads, group, head_tiles, dim, columns;  // columns: blocks that share the units
   float scale_log2;
   void* out;
   float* weight;
   int64_t weight_row;
-  float2* stats;  // (batch, q_heads): maximum (log2 domain) and sum
+  float* scores;      // (batch, kv_heads, head_tiles, slots, pack) with weights, log2 domain
+  int64_t slots;
+  int pack;           // heads a slot's scores are stored for: min(group, 8) rounded up to a power of two
+  float* part_o;      // (head_tiles, columns, 2, 8, DP) unnormalized outputs of runs that cover part of a head
+  float2* part_ml;    // (head_tiles, columns, 2, 8) their maxima and sums
+  float2* whole_ml;   // (batch, q_heads) those of heads that one block covered
   int* err;
 };
 
-// the score of one slot: a warp, lane l takes values l, l + 32, ...
-template <typename T>
-__device__ __forceinline__ float score(const float (&q)[8], const T* k, int dim, int lane) {
-  float s = 0.f;
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+__device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
+
+template <int N>
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* sh) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (lane + 32 * i < dim) s = fmaf(q[i], to_f32(k[lane + 32 * i]), s);
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int64_t t = 0;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  for (int i = 0; i < N / 32; ++i) t += sh[i];
+  __syncthreads();
+  return t;
+}
+
+template <int N>
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& total) {  // inclusive
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  if (lane == 31) sh[warp] = v;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < N / 32; ++w) {
+    if (w < warp) v += sh[w];
+    total += sh[w];
+  }
+  __syncthreads();
+  return v;
+}
+
+// The units' numbering: sequence after sequence, in each head after head. Block x of X takes units [x U / X,
+// (x + 1) U / X), so unit u is block ((u + 1) X - 1) / U's; X is at most U, so that every block up to X has a unit.
+template <int N>
+__device__ __forceinline__ int64_t units_before(const Args& A, int unit, int b, int64_t* sh, int* err) {
+  int64_t n = 0;
+  for (int i = threadIdx.x; i < b; i += N) n += (length_of(A.pages, i, err) + unit - 1) / unit;
+  return block_sum<N>(n, sh) * A.kv_heads;
+}
+
+template <typename T, int DP, int SUB>
+__global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Args A) {
+  constexpr int KC = DP / 32, VC = DP / 64, TILE = 16 * SUB, UNIT = WARPS * TILE;
+  constexpr int IDS = (TILE + 31) / 32;
+  __shared__ uint4 s_q[KC][32];
+  __shared__ __align__(16) float s_o[WARPS][HEADS][DP];
+  __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS];
+  __shared__ int64_t s_sum[WARPS], s_before;
+  __shared__ int s_b;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int ht = blockIdx.y;
+  const int64_t x = blockIdx.x;
+  pdl_launch_dependents();
+  const int64_t U = units_before<THREADS>(A, UNIT, A.batch, s_sum, A.err), X = min(int64_t(A.columns), U);
+  if (x >= X) return;
+  int64_t u = x * U / X;
+  const int64_t u1 = (x + 1) * U / X;
+  // the sequence that holds unit u
+  {
+    int64_t before = 0;
+    if (tid == 0) s_b = -1;
+    for (int b0 = 0; b0 < A.batch; b0 += THREADS) {
+      const int mine = b0 + tid < A.batch ? (length_of(A.pages, b0 + tid, nullptr) + UNIT - 1) / UNIT : 0;
+      int64_t total;
+      const int64_t to = before + block_scan<THREADS>(mine, s_sum, total);
+      if (u >= (to - mine) * A.kv_heads && u < to * A.kv_heads) s_b = b0 + tid, s_before = to - mine;
+      __syncthreads();
+      if (s_b >= 0) break;
+      before += total;
+    }
+  }
+  int b = s_b;
+  if (b < 0) return;  // the lengths changed under the kernel
+  int hk, ul;
+  {
+    const int n = (length_of(A.pages, b, nullptr) + UNIT - 1) / UNIT;
+    const int64_t in = u - s_before * A.kv_heads;
+    hk = int(in / n), ul = int(in % n);
+  }
+  const Pages& P = A.pages;
+  const int mask = (1 << P.shift) - 1, chunks = A.dim / 8;
+  const int heads = min(HEADS, A.group - ht * HEADS);  // of this block
+  while (u < u1 && b < A.batch) {
+    const int len = length_of(P, b, nullptr), n_units = (len + UNIT - 1) / UNIT;
+    if (n_units == 0 || hk == A.kv_heads) {
+      ++b, hk = 0, ul = 0;
+      continue;
+    }
+    const int ue = int(min(int64_t(n_units), ul + (u1 - u)));
+    // ---- the heads' queries, in the products' order
+    for (int i = tid; i < KC * 32; i += THREADS) {
+      const int c = (i / 32) * 4 + (i & 3), h = (i & 31) >> 2;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (h < heads && c < chunks)
+        v = *reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + b * A.q_row +
+                                            int64_t(hk * A.group + ht * HEADS + h) * A.q_head + 8 * c);
+      s_q[i / 32][i & 31] = v;
+    }
+    __syncthreads();
+    // ---- this warp's tiles
+    const int end = min(len, ue * UNIT);
+    int base = (ul * WARPS + warp) * TILE;
+    const char* kb = P.k + hk * P.k_head + 16 * t;
+    const char* vb = P.v + hk * P.v_head + 16 * g;
+    const int32_t* table = P.table + b * P.table_row;
+    // page ids of a tile's slots, lane l that of slots l and l + 32; -1 past the end or outside the pool
+    auto load_ids = [&](int at, int (&id)[IDS]) {
+#pragma unroll
+      for (int i = 0; i < IDS; ++i) {
+        const int s = at + lane + 32 * i;
+        id[i] = -1;
+        if (s < end && lane + 32 * i < TILE) {
+          id[i] = __ldg(table + (s >> P.shift));
+          if (unsigned(id[i]) >= unsigned(P.pool_pages)) {
+            record_error(A.err, SC_ERR_PAGE);
+            id[i] = -1;
+          }
+        }
+      }
+    };
+    uint4 kf[SUB][2][KC], vf[SUB][4][VC];
+    auto load_k = [&](int at, const int (&id)[IDS]) -> uint32_t {  // returns which of the lane's slots hold a token
+      uint32_t valid = 0;
+#pragma unroll
+      for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int o = 16 * s + 8 * r + g, page = __shfl_sync(0xffffffffu, id[s / 2], o & 31);
+          const char* p = kb + page * P.k_page + ((at + o) & mask) * P.k_token;
+          if (page >= 0) valid |= 1u << (2 * s + r);
+#pragma unroll
+          for (int j = 0; j < KC; ++j) {
+            kf[s][r][j] = make_uint4(0, 0, 0, 0);
+            if (page >= 0 && 4 * j + t < chunks) kf[s][r][j] = load16(p + 64 * j);
+          }
+        }
+      return valid;
+    };
+    auto load_v = [&](int at, const int (&id)[IDS]) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int o = 16 * s + 8 * (r >> 1) + 2 * t + (r & 1), page = __shfl_sync(0xffffffffu, id[s / 2], o & 31);
+          const char* p = vb + page * P.v_page + ((at + o) & mask) * P.v_token;
+#pragma unroll
+          for (int i = 0; i < VC; ++i) {
+            vf[s][r][i] = make_uint4(0, 0, 0, 0);
+            if (page >= 0 && 8 * i + g < chunks) vf[s][r][i] = load16(p + 128 * i);
+          }
+        }
+    };
+    float o[VC][4][4];
+#pragma unroll
+    for (int i = 0; i < VC; ++i)
+#pragma unroll
+      for (int m = 0; m < 4; ++m) o[i][m][0] = o[i][m][1] = o[i][m][2] = o[i][m][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, b0 = 0.f, b1 = 0.f, l0 = 0.f, l1 = 0.f;  // of heads 2t and 2t + 1
+    int id[IDS], next[IDS];
+    load_ids(base, id);
+    uint32_t valid = load_k(base, id);
+    load_v(base, id);
+    load_ids(base + UNIT, next);
+    for (; base < end; base += UNIT) {
+      float s[SUB][4];
+#pragma unroll
+      for (int i = 0; i < SUB; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        const uint4 q = s_q[j][lane];
+#pragma unroll
+        for (int i = 0; i < SUB; ++i) {
+          const uint4 &ka = kf[i][0][j], &kc = kf[i][1][j];
+          const uint32_t a0[4] = {ka.x, kc.x, ka.y, kc.y}, a1[4] = {ka.z, kc.z, ka.w, kc.w};
+          mma16816<T>(s[i], a0, q.x, q.y);
+          mma16816<T>(s[i], a1, q.z, q.w);
+        }
+      }
+      const uint32_t in = valid;
+      valid = load_k(base + UNIT, next);
+      float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < SUB; ++i) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const bool ok = (in >> (2 * i + r)) & 1;
+          s[i][2 * r] = ok ? s[i][2 * r] * A.scale_log2 : -INFINITY;
+          s[i][2 * r + 1] = ok ? s[i][2 * r + 1] * A.scale_log2 : -INFINITY;
+          x0 = fmaxf(x0, s[i][2 * r]);
+          x1 = fmaxf(x1, s[i][2 * r + 1]);
+        }
+      }
+      if (A.scores) {
+#pragma unroll
+        for (int i = 0; i < SUB; ++i)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int slot = base + 16 * i + 8 * r + g;
+            if (slot < end && 2 * t < A.pack) {
+              float* to = A.scores + (((int64_t(b) * A.kv_heads + hk) * A.head_tiles + ht) * A.slots + slot) * A.pack + 2 * t;
+              if (A.pack > 1) *reinterpret_cast<float2*>(to) = make_float2(s[i][2 * r], s[i][2 * r + 1]);
+              else *to = s[i][2 * r];
+            }
+          }
+      }
+      if (__any_sync(0xffffffffu, x0 > m0 + SLACK || x1 > m1 + SLACK)) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) {
+          x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, w));
+          x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, w));
+        }
+        x0 = fmaxf(x0, m0), x1 = fmaxf(x1, m1);
+        b0 = finite_or_0(x0), b1 = finite_or_0(x1);
+        const float c0 = exp2f(m0 - b0), c1 = exp2f(m1 - b1);
+        m0 = x0, m1 = x1;
+        l0 *= c0, l1 *= c1;
+#pragma unroll
+        for (int i = 0; i < VC; ++i)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) o[i][m][0] *= c0, o[i][m][1] *= c1, o[i][m][2] *= c0, o[i][m][3] *= c1;
+      }
+#pragma unroll
+      for (int i = 0; i < SUB; ++i) {
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float p0 = exp2f(s[i][2 * r] - b0), p1 = exp2f(s[i][2 * r + 1] - b1);
+          l0 += p0, l1 += p1;
+          const uint32_t h = pack2<T>(p0, p1);
+          const float2 back = unpack2<T>(h);
+          hi[r] = transpose8x8(h);
+          lo[r] = transpose8x8(pack2<T>(p0 - back.x, p1 - back.y));
+        }
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+          const uint32_t* r0 = reinterpret_cast<const uint32_t*>(&vf[i][0][c]);
+          const uint32_t* r1 = reinterpret_cast<const uint32_t*>(&vf[i][1][c]);
+          const uint32_t* r2 = reinterpret_cast<const uint32_t*>(&vf[i][2][c]);
+          const uint32_t* r3 = reinterpret_cast<const uint32_t*>(&vf[i][3][c]);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const uint32_t a[4] = {__byte_perm(r0[m], r1[m], 0x5410), __byte_perm(r0[m], r1[m], 0x7632),
+                                   __byte_perm(r2[m], r3[m], 0x5410), __byte_perm(r2[m], r3[m], 0x7632)};
+            mma16816<T>(o[c][m], a, hi[0], hi[1]);
+            mma16816<T>(o[c][m], a, lo[0], lo[1]);
+          }
+        }
+      }
+      load_v(base + UNIT, next);
+      load_ids(base + 2 * UNIT, next);
+    }
+    // ---- the warps' results joined
+#pragma unroll
+    for (int w = 4; w < 32; w <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, w);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, w);
+    }
+    if (g == 0) s_m[warp][2 * t] = m0, s_m[warp][2 * t + 1] = m1, s_l[warp][2 * t] = l0, s_l[warp][2 * t + 1] = l1;
+    __syncthreads();
+    float M0 = -INFINITY, M1 = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) M0 = fmaxf(M0, s_m[w][2 * t]), M1 = fmaxf(M1, s_m[w][2 * t + 1]);
+    const float c0 = exp2f(m0 - finite_or_0(M0)), c1 = exp2f(m1 - finite_or_0(M1));
+#pragma unroll
+    for (int i = 0; i < VC; ++i) {
+      float4* to = reinterpret_cast<float4*>(&s_o[warp][2 * t][64 * i + 8 * g]);
+      to[0] = make_float4(o[i][0][0] * c0, o[i][0][2] * c0, o[i][1][0] * c0, o[i][1][2] * c0);
+      to[1] = make_float4(o[i][2][0] * c0, o[i][2][2] * c0, o[i][3][0] * c0, o[i][3][2] * c0);
+      to = reinterpret_cast<float4*>(&s_o[warp][2 * t + 1][64 * i + 8 * g]);
+      to[0] = make_float4(o[i][0][1] * c1, o[i][0][3] * c1, o[i][1][1] * c1, o[i][1][3] * c1);
+      to[1] = make_float4(o[i][2][1] * c1, o[i][2][3] * c1, o[i][3][1] * c1, o[i][3][3] * c1);
+    }
+    __syncthreads();
+    const bool whole = ul == 0 && ue == n_units;
+    const int64_t part = ((int64_t(ht) * A.columns + x) * 2 + (ul == 0)) * HEADS;  // 0: a head's later run, 1: its first
+    for (int e = tid; e < heads * (DP / 4); e += THREADS) {
+      const int h = e / (DP / 4), d = 4 * (e % (DP / 4));
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][h]);
+      const float mb = finite_or_0(M);
+      float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        L += s_l[w][h] * exp2f(s_m[w][h] - mb);
+        const float4 v = *reinterpret_cast<const float4*>(&s_o[w][h][d]);
+        r.x += v.x, r.y += v.y, r.z += v.z, r.w += v.w;
+      }
+      const int64_t row = int64_t(b) * A.q_heads + hk * A.group + ht * HEADS + h;
+      if (whole) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        if (d < A.dim)
+          *reinterpret_cast<uint2*>(static_cast<T*>(A.out) + row * A.dim + d) =
+              make_uint2(pack2<T>(r.x * inv, r.y * inv), pack2<T>(r.z * inv, r.w * inv));
+        if (d == 0 && A.scores) A.whole_ml[row] = make_float2(mb, L);
+      } else {
+        *reinterpret_cast<float4*>(A.part_o + (part + h) * DP + d) = r;
+        if (d == 0) A.part_ml[part + h] = make_float2(M, L);
+      }
+    }
+    __syncthreads();  // s_q, s_m and s_o are the next run's
+    u += ue - ul;
+    ul = 0;
+    ++hk;
+  }
+}
+
+// The blocks that share the units of a sequence's heads: head hk's are first(hk) .. last(hk), none when n is 0.
+struct Share {
+  int64_t U, X, before, n;
+  __device__ int first(int hk) const { return int(((before + hk * n + 1) * X - 1) / U); }
+  __device__ int last(int hk) const { return int(((before + hk * n + n) * X - 1) / U); }
+};
+template <int N>
+__device__ __forceinline__ Share share_of(const Args& A, int unit, int b, int64_t* sh) {
+  int64_t all = 0, before = 0;
+  for (int i = threadIdx.x; i < A.batch; i += N) {
+    const int64_t n = (length_of(A.pages, i, nullptr) + unit - 1) / unit;
+    all += n;
+    if (i < b) before += n;
+  }
+  Share s;
+  s.U = block_sum<N>(all, sh) * A.kv_heads;
+  s.X = min(int64_t(A.columns), s.U);
+  s.before = block_sum<N>(before, sh) * A.kv_heads;
+  s.n = (length_of(A.pages, b, nullptr) + unit - 1) / unit;
   return s;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) attend_kernel(const Args A) {
-  __shared__ float s_m[WARPS], s_l[WARPS], s_o[WARPS][256];
-  const int b = blockIdx.x, h = blockIdx.y, hk = h / A.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = length_of(A.pages, b, A.err);
-  const T* q = static_cast<const T*>(A.q) + b * A.q_row + h * A.q_head;
-  float qv[8], o[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    qv[i] = lane + 32 * i < A.dim ? to_f32(q[lane + 32 * i]) * A.scale_log2 : 0.f;
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  const int mask = (1 << A.pages.shift) - 1;
-  for (int s = warp; s < n; s += WARPS) {
-    const int page = page_of(A.pages, b, s, A.err);
-    if (page < 0) continue;
-    const T* k = reinterpret_cast<const T*>(A.pages.k + page * A.pages.k_page + (s & mask) * A.pages.k_token + hk * A.pages.k_head);
-    const T* v = reinterpret_cast<const T*>(A.pages.v + page * A.pages.v_page + (s & mask) * A.pages.v_token + hk * A.pages.v_head);
-    const float x = score(qv, k, A.dim, lane), top = fmaxf(m, x);
-    const float c = m == top ? 1.f : exp2f(m - top), p = exp2f(x - (top == -INFINITY ? 0.f : top));
-    m = top;
-    l = l * c + p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < A.dim) o[i] = fmaf(p, to_f32(v[lane + 32 * i]), o[i] * c);
-  }
-  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s_o[warp][lane + 32 * i] = o[i];
-  __syncthreads();
+// a warp: the joint maximum (finite) and sum of query head h, from its partial results or the one whole one
+__device__ __forceinline__ float2 joint(const Args& A, const Share& s, int b, int h, float* terms) {
+  const int lane = threadIdx.x & 31, hk = h / A.group, ht = (h % A.group) / HEADS, hr = (h % A.group) % HEADS;
+  const int first = s.first(hk), last = s.last(hk);
+  if (first == last) return A.whole_ml[int64_t(b) * A.q_heads + h];
+  auto at = [&](int x) { return ((int64_t(ht) * A.columns + x) * 2 + (x == first)) * HEADS + hr; };
   float M = -INFINITY, L = 0.f;
-  for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w]);
-  const float base = M == -INFINITY ? 0.f : M;
-  for (int w = 0; w < WARPS; ++w) L += s_l[w] * exp2f(s_m[w] - base);
-  for (int d = threadIdx.x; d < A.dim; d += WARPS * 32) {
-    float r = 0.f;
-    for (int w = 0; w < WARPS; ++w) r += s_o[w][d] * exp2f(s_m[w] - base);
-    static_cast<T*>(A.out)[(int64_t(b) * A.q_heads + h) * A.dim + d] = from_f32<T>(L == 0.f ? 0.f : r / L);
+#pragma unroll 4
+  for (int x = first + lane; x <= last; x += 32) M = fmaxf(M, A.part_ml[at(x)].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  M = finite_or_0(M);
+#pragma unroll 4
+  for (int x = first + lane; x <= last; x += 32) {
+    const float2 ml = A.part_ml[at(x)];
+    const float c = exp2f(ml.x - M);
+    if (terms) terms[x - first] = c;
+    L += ml.y * c;
   }
-  if (threadIdx.x == 0) A.stats[int64_t(b) * A.q_heads + h] = make_float2(base, L);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  return make_float2(M, L);
 }
 
-// a warp a slot: every query head's probability there
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) weight_kernel(const Args A) {
-  const int b = blockIdx.y, s = blockIdx.x * WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (s >= length_of(A.pages, b, nullptr)) return;
-  const int page = page_of(A.pages, b, s, nullptr);
-  if (page < 0) return;
-  const int mask = (1 << A.pages.shift) - 1;
-  float sum = 0.f;
-  for (int h = 0; h < A.q_heads; ++h) {
-    const T* q = static_cast<const T*>(A.q) + b * A.q_row + h * A.q_head;
-    const T* k = reinterpret_cast<const T*>(A.pages.k + page * A.pages.k_page + (s & mask) * A.pages.k_token + h / A.group * A.pages.k_head);
-    float qv[8];
+// Blocks 0 .. batch x q_heads - 1: a query head's output from its partial results (zeros for an empty sequence). The
+// rest, with weights: JOIN_SLOTS slots of a sequence.
+template <typename T, int DP>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int unit, int slot_blocks) {
+  constexpr int LANES = DP / 4, GROUPS = JOIN_THREADS / LANES;  // threads of a row, and rows read side by side
+  __shared__ int64_t sh[JOIN_THREADS / 32];
+  __shared__ __align__(16) float s_o[GROUPS][DP];
+  __shared__ float s_c[BLOCKS_PER_SM * SMS], s_l;
+  extern __shared__ float2 s_ml[];  // of every query head (weights)
+  const int tid = threadIdx.x;
+  const int outs = A.batch * A.q_heads;
+  if (int(blockIdx.x) < outs) {
+    const int b = blockIdx.x / A.q_heads, h = blockIdx.x % A.q_heads, hk = h / A.group, hh = h % A.group;
+    const int ht = hh / HEADS, hr = hh % HEADS;
+    T* out = static_cast<T*>(A.out) + int64_t(blockIdx.x) * A.dim;
+    const Share s = share_of<JOIN_THREADS>(A, unit, b, sh);
+    const int first = s.n ? s.first(hk) : 0, last = s.n ? s.last(hk) : 0;
+    pdl_wait();
+    if (s.n == 0) {
+      for (int d = tid; d < A.dim; d += JOIN_THREADS) out[d] = from_f32<T>(0.f);
+      return;
+    }
+    if (first == last) return;  // one block covered it
+    if (tid < 32) {
+      const float2 ml = joint(A, s, b, h, s_c);
+      if (tid == 0) s_l = ml.y;
+    }
+    __syncthreads();
+    const int row = tid / LANES, d = 4 * (tid % LANES);
+    const float* from = A.part_o + (int64_t(ht) * A.columns * 2 * HEADS + hr) * DP + d;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int x = first + row; x <= last; x += GROUPS) {
+      const float4 v = *reinterpret_cast<const float4*>(from + (int64_t(x) * 2 + (x == first)) * HEADS * DP);
+      const float c = s_c[x - first];
+      o.x += v.x * c, o.y += v.y * c, o.z += v.z * c, o.w += v.w * c;
+    }
+    *reinterpret_cast<float4*>(&s_o[row][d]) = o;
+    __syncthreads();
+    if (row == 0 && d < A.dim) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) qv[i] = lane + 32 * i < A.dim ? to_f32(q[lane + 32 * i]) * A.scale_log2 : 0.f;
-    const float2 st = A.stats[int64_t(b) * A.q_heads + h];
-    sum += exp2f(score(qv, k, A.dim, lane) - st.x) / st.y;
+      for (int i = 1; i < GROUPS; ++i) {
+        const float4 v = *reinterpret_cast<const float4*>(&s_o[i][d]);
+        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+      }
+      const float inv = s_l == 0.f ? 0.f : 1.f / s_l;
+      *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+    }
+    return;
   }
-  if (lane == 0) A.weight[b * A.weight_row + s] += sum;
+  const int e = blockIdx.x - outs, b = e / slot_blocks, s0 = (e % slot_blocks) * JOIN_SLOTS;
+  const int len = length_of(A.pages, b, nullptr);
+  if (s0 >= len) return;
+  const Share share = share_of<JOIN_THREADS>(A, unit, b, sh);
+  pdl_wait();
+  for (int h = tid / 32; h < A.q_heads; h += JOIN_THREADS / 32) {
+    const float2 ml = joint(A, share, b, h, nullptr);
+    if (tid % 32 == 0) s_ml[h] = make_float2(ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y);
+  }
+  __syncthreads();
+  for (int s = s0 + tid; s < min(len, s0 + JOIN_SLOTS); s += JOIN_THREADS) {
+    float sum = 0.f;
+    for (int hk = 0; hk < A.kv_heads; ++hk)
+      for (int ht = 0; ht < A.head_tiles; ++ht) {
+        const float* x = A.scores + (((int64_t(b) * A.kv_heads + hk) * A.head_tiles + ht) * A.slots + s) * A.pack;
+        const float2* ml = s_ml + hk * A.group + ht * HEADS;
+        for (int h = 0; h < min(HEADS, A.group - ht * HEADS); ++h) sum += exp2f(x[h] - ml[h].x) * ml[h].y;
+      }
+    A.weight[b * A.weight_row + s] += sum;
+  }
+}
+
+// ---- host
+
+// dimensions as the kernels are built for them, and the slots of a warp's tile: 16 KB of keys and values at each
+inline int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+inline int tile_of(int dp) { return dp == 64 ? 64 : dp == 128 ? 32 : 16; }
+
+struct Layout {
+  int dp, unit, head_tiles, columns, pack;
+  size_t part_o, part_ml, whole_ml, scores, bytes;
+};
+
+inline Layout layout(const sc_kv_pages& c, int q_heads) {
+  Layout l{};
+  const int group = q_heads / c.kv_heads;
+  l.dp = padded(c.head_dim);
+  l.unit = WARPS * tile_of(l.dp);
+  l.head_tiles = (group + HEADS - 1) / HEADS;
+  for (l.pack = 1; l.pack < std::min(group, HEADS); l.pack *= 2) {}
+  const int64_t slots = int64_t(c.max_pages) * c.page, units = int64_t(c.batch) * c.kv_heads * ceil_div(slots, l.unit);
+  l.columns = int(std::max<int64_t>(1, std::min<int64_t>(units, BLOCKS_PER_SM * SMS / l.head_tiles)));
+  const size_t parts = size_t(l.head_tiles) * l.columns * 2 * HEADS;
+  auto take = [&](size_t n) {
+    const size_t at = l.bytes;
+    l.bytes += (n + 15) / 16 * 16;
+    return at;
+  };
+  l.part_o = take(parts * l.dp * 4);
+  l.part_ml = take(parts * 8);
+  if (c.weight) {
+    l.whole_ml = take(size_t(c.batch) * q_heads * 8);
+    l.scores = take(size_t(c.batch) * c.kv_heads * l.head_tiles * slots * l.pack * 4);
+  }
+  return l;
 }
 
 }  // namespace da
@@ -106,8 +543,8 @@ __global__ void __launch_bounds__(WARPS * 32) weight_kernel(const Args A) {
 using namespace sc;
 
 extern "C" size_t sc_decode_attention_workspace(const sc_kv_pages* kv, int q_heads) {
-  if (check_pages(kv) || q_heads < 1 || q_heads % kv->kv_heads) return 0;
-  return size_t(kv->batch > 0 ? kv->batch : 1) * q_heads * sizeof(float2);
+  if (check_pages(kv) || q_heads < 1 || q_heads % kv->kv_heads || q_heads > 4096) return 0;
+  return da::layout(*kv, q_heads).bytes;
 }
 
 extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t q_row, int64_t q_head, int q_heads,
@@ -115,29 +552,59 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
                                    void* stream) {
   if (int rc = check_pages(kv)) return rc;
   if (kv->batch && (!q || !out || !workspace)) return SC_ERR_ARG;
-  if (q_heads < 1 || q_heads % kv->kv_heads || q_heads > 65535) return SC_ERR_SHAPE;
+  if (q_heads < 1 || q_heads % kv->kv_heads || q_heads > 4096) return SC_ERR_SHAPE;
   if (((q_row | q_head) & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & 15))
     return SC_ERR_ALIGN;
-  if (workspace_bytes < sc_decode_attention_workspace(kv, q_heads)) return SC_ERR_WORKSPACE;
+  const da::Layout l = da::layout(*kv, q_heads);
+  if (workspace_bytes < l.bytes) return SC_ERR_WORKSPACE;
   if (kv->batch == 0) return SC_OK;
   da::Args A{};
   A.pages = pages_of(*kv);
   A.q = q, A.q_row = q_row, A.q_head = q_head;
-  A.q_heads = q_heads, A.group = q_heads / kv->kv_heads, A.dim = kv->head_dim;
+  A.batch = kv->batch, A.q_heads = q_heads, A.kv_heads = kv->kv_heads, A.group = q_heads / kv->kv_heads;
+  A.head_tiles = l.head_tiles, A.dim = kv->head_dim, A.columns = l.columns;
   A.scale_log2 = scale * 1.4426950408889634f;
   A.out = out, A.weight = kv->weight, A.weight_row = kv->weight_row;
-  A.stats = static_cast<float2*>(workspace);
+  char* ws = static_cast<char*>(workspace);
+  A.part_o = reinterpret_cast<float*>(ws + l.part_o);
+  A.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
+  A.slots = int64_t(kv->max_pages) * kv->page;
+  A.pack = l.pack;
+  if (kv->weight) {
+    A.whole_ml = reinterpret_cast<float2*>(ws + l.whole_ml);
+    A.scores = reinterpret_cast<float*>(ws + l.scores);
+  }
   A.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  auto run = [&](auto t) {
+  const int slot_blocks = kv->weight ? int(ceil_div(A.slots, da::JOIN_SLOTS)) : 0;
+  const int64_t join_blocks = int64_t(kv->batch) * (q_heads + slot_blocks);
+  if (join_blocks > INT32_MAX) return SC_ERR_SHAPE;
+  auto run = [&](auto t, auto dp, auto sub) -> int {
     using T = decltype(t);
-    da::attend_kernel<T><<<dim3(kv->batch, q_heads), da::WARPS * 32, 0, s>>>(A);
-    if (A.weight)
-      da::weight_kernel<T><<<dim3(unsigned(ceil_div(int64_t(kv->max_pages) * kv->page, da::WARPS)), kv->batch), da::WARPS * 32, 0, s>>>(A);
+    constexpr int DP = decltype(dp)::value, SUB = decltype(sub)::value;
+    da::attend_kernel<T, DP, SUB><<<dim3(unsigned(l.columns), unsigned(l.head_tiles)), da::THREADS, 0, s>>>(A);
+    // programmatic dependent launch: the joining blocks are placed as the attention's leave
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(join_blocks));
+    cfg.blockDim = dim3(da::JOIN_THREADS);
+    cfg.dynamicSmemBytes = kv->weight ? size_t(q_heads) * 8 : 0;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, da::join_kernel<T, DP>, A, l.unit, slot_blocks))
+      return cuda_failed(e, "decode attention join launch");
+    if (cudaError_t e = cudaGetLastError()) return cuda_failed(e, "decode attention launch");
+    return SC_OK;
   };
-  if (kv->dtype == SC_BF16) run(__nv_bfloat16{});
-  else run(__half{});
-  if (cudaError_t e = cudaGetLastError()) return cuda_failed(e, "decode attention launch");
-  return SC_OK;
+  auto typed = [&](auto t) -> int {
+    using std::integral_constant;
+    if (l.dp == 64) return run(t, integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    if (l.dp == 128) return run(t, integral_constant<int, 128>{}, integral_constant<int, 2>{});
+    return run(t, integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  };
+  return kv->dtype == SC_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
 }
