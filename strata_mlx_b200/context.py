@@ -17,12 +17,15 @@ float16; softmax statistics, accumulated weights and states are float32.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
 from . import _lib
-from ._lib import check, ptr, require_cuda, stream
+from ._lib import check, ptr, require_cuda
 
+_stream = torch._C._cuda_getCurrentRawStream  # a call's stream without building a Stream object
+_capturing = torch.cuda.is_current_stream_capturing
 _TYPES = {torch.float16: 1, torch.bfloat16: 2}  # SC_F16, SC_BF16
 
 
@@ -85,20 +88,21 @@ class KVPages:
         self._pages, self._ref = P, ctypes.addressof(P)
         self._lib, self._err = _lib.lib(), ptr(_lib.error_word(self.device))
         self._ws: dict = {}
+        self._sizes: dict = {}  # of attend's workspace, by the query heads
+        self._index, self._scale = self.device.index, self.head_dim ** -0.5
 
-    def _workspace(self, what: tuple, s: int, size) -> tuple:
+    def _workspace(self, what: str, size: int, s: int) -> tuple:
         """The workspace of a kind of call on stream s: its address and bytes (fresh in a capture, whose memory is
-        the graph's)."""
-        ws = self._ws.get((s, *what))
-        if ws is None or torch.cuda.is_current_stream_capturing():
-            n = size()
-            if n == 0:
-                raise ValueError(f"{what[0]}: this cache or these arguments are not taken (head_dim a multiple of 8 up "
-                                 "to 256, a power-of-two page, query heads a multiple of the cache's)")
-            t = torch.empty(n, dtype=torch.uint8, device=self.device)
-            ws = (t.data_ptr(), n, t)
-            if not torch.cuda.is_current_stream_capturing():
-                self._ws[(s, *what)] = ws
+        the graph's). Zeroed: kernels count in it, and leave the counts at zero."""
+        if size == 0:
+            raise ValueError(f"{what}: this cache or these arguments are not taken (head_dim a multiple of 8 up to 256, "
+                             "a power-of-two page, 16-byte rows, query heads a multiple of the cache's)")
+        ws = self._ws.get((what, s))
+        if ws is None or ws[1] < size or _capturing():
+            t = torch.zeros(size, dtype=torch.uint8, device=self.device)
+            ws = (t.data_ptr(), size, t)
+            if not _capturing():
+                self._ws[what, s] = ws
         return ws
 
     def attend(self, q: torch.Tensor, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -109,20 +113,26 @@ class KVPages:
         if len(shape) != 3 or shape[0] != self.batch or shape[2] != self.head_dim or q.dtype != self.dtype:
             raise ValueError(f"q ({self.batch}, q_heads, {self.head_dim}) {self.dtype} expected, got {tuple(shape)} "
                              f"{q.dtype}")
-        if q.device != self.device or torch.cuda.current_device() != self.device.index:
+        if q.device != self.device or torch.cuda.current_device() != self._index:
             raise ValueError(f"q on {q.device}; the cache is on {self.device}, which has to be current")
-        if q.stride(2) != 1:
+        st = q.stride()
+        if st[2] != 1:
             q = q.contiguous()
+            st = q.stride()
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=self.device)
+            out = q.new_empty(shape)
         elif out.shape != shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous():
             raise ValueError(f"out: contiguous {tuple(shape)} {q.dtype} expected")
-        s, heads = stream(), shape[1]
-        ws = self._workspace(("attend", heads), s,
-                             lambda: self._lib.sc_decode_attention_workspace(self._ref, heads))
-        check(self._lib.sc_decode_attention(self._ref, q.data_ptr(), q.stride(0), q.stride(1), heads,
-                                            self.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), ws[0],
-                                            ws[1], self._err, s), "decode_attention")
+        s, heads = _stream(self._index), shape[1]
+        size = self._sizes.get(heads)
+        if size is None:
+            size = self._sizes[heads] = self._lib.sc_decode_attention_workspace(self._ref, heads)
+        ws = self._workspace("attend", size, s)
+        rc = self._lib.sc_decode_attention(self._ref, q.data_ptr(), st[0], st[1], heads,
+                                           self._scale if scale is None else scale, out.data_ptr(), ws[0], ws[1],
+                                           self._err, s)
+        if rc:
+            check(rc, "decode_attention")
         return out
 
     def evict(self, seen: torch.Tensor, keep: int, sinks: int = 4, recent: int = 0, out: tuple | None = None) -> None:
@@ -143,10 +153,10 @@ class KVPages:
                     or t.shape[1] < min(keep, self.slots)):
                 raise ValueError(f"out {name}: {dtype} ({self.batch}, at least {min(keep, self.slots)}) expected")
         _ints("out lengths", lengths, (self.batch,))
-        s = stream()
+        s = _stream(self._index)
         if keep < 0 or sinks < 0 or recent < 0 or sinks + recent > keep:
             raise ValueError(f"sinks {sinks} and recent {recent} have to fit in keep {keep}")
-        ws = self._workspace(("evict", keep), s, lambda: self._lib.sc_evict_workspace(self._ref, keep))
+        ws = self._workspace("evict", self._lib.sc_evict_workspace(self._ref, keep), s)
         check(self._lib.sc_evict(self._ref, seen.data_ptr(), keep, sinks, recent, weight.data_ptr(), weight.stride(0),
                                  position.data_ptr(), position.stride(0), lengths.data_ptr(), ws[0], ws[1], self._err,
                                  s), "evict")
@@ -159,38 +169,45 @@ def decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: t
     return KVPages(k, v, table, lengths, weight).attend(q, scale, out)
 
 
-def _linear(q, k, v, decay, state, scale) -> tuple:
-    """The checked call as an SCLinear without its outputs, and what has to stay alive until it is enqueued."""
-    device = _here(q, k, v, decay, state)
+_LINEAR = struct.Struct("@8Q12q7if")  # sc_linear (include/strata_cuda.h), field by field
+
+
+def _refuse_linear(q, k, v, decay, state, nd: int) -> None:
+    """Names what is wrong with a linear attention call's tensors."""
+    _here(q, k, v, decay, state)
     if q.dtype not in _TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"q, k and v all bfloat16 or all float16 expected, got {q.dtype}, {k.dtype}, {v.dtype}")
-    lead = tuple(q.shape[:-2])
-    if k.shape != q.shape or tuple(v.shape[:-2]) != lead or q.shape[-2] == 0 or v.shape[-2] % q.shape[-2]:
-        raise ValueError(f"q and k alike, v of the same tokens with a multiple of their heads expected, got "
-                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    hv, dk, dv = v.shape[-2], q.shape[-1], v.shape[-1]
-    if decay.dtype != torch.float32 or tuple(decay.shape) != (*lead, hv):
-        raise ValueError(f"decay: float32 {(*lead, hv)} expected, got {decay.dtype} {tuple(decay.shape)}")
-    if state is not None and (state.dtype != torch.float32 or tuple(state.shape) != (lead[0], hv, dk, dv)
-                              or not state.is_contiguous()):
-        raise ValueError(f"state: contiguous float32 {(lead[0], hv, dk, dv)} expected")
-    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
-    A = _lib.SCLinear()
-    A.q, A.k, A.v, A.decay = q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr()
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        st = t.stride()
-        setattr(A, name + "_row", st[0])
-        setattr(A, name + "_head", st[-2])
-        if len(lead) == 2:
-            setattr(A, name + "_token", st[1])
-    st = decay.stride()
-    A.decay_row, A.decay_head = st[0], st[-1]
-    if len(lead) == 2:
-        A.decay_token = st[1]
-    A.batch, A.tokens = lead[0], lead[1] if len(lead) == 2 else 1
-    A.k_heads, A.v_heads, A.k_dim, A.v_dim, A.dtype = q.shape[-2], hv, dk, dv, _TYPES[q.dtype]
-    A.scale = dk ** -0.5 if scale is None else scale
-    return A, (q, k, v), device
+    axes = "(batch, tokens, heads, dim)" if nd == 4 else "(batch, heads, dim)"
+    if q.dim() != nd or v.dim() != nd or k.shape != q.shape or v.shape[:-2] != q.shape[:-2]:
+        raise ValueError(f"q, k and v {axes}, q and k alike, v of the same tokens expected, got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    if q.shape[-2] == 0 or v.shape[-2] % q.shape[-2]:
+        raise ValueError(f"{v.shape[-2]} value heads are not a multiple of {q.shape[-2]} key heads")
+    if decay.dtype != torch.float32 or decay.shape != v.shape[:-1]:
+        raise ValueError(f"decay: float32 {tuple(v.shape[:-1])} expected, got {decay.dtype} {tuple(decay.shape)}")
+    raise ValueError(f"state: contiguous float32 {(v.shape[0], v.shape[-2], q.shape[-1], v.shape[-1])} expected")
+
+
+def _linear(q, k, v, decay, state, nd: int) -> tuple:
+    """Checks a call's tensors in one pass; returns them with their values adjacent, and sc_linear's integers."""
+    qs, vs, dtype, index = q.shape, v.shape, q.dtype, q.get_device()
+    code = _TYPES.get(dtype)
+    if (index < 0 or k.get_device() != index or v.get_device() != index or decay.get_device() != index
+            or torch.cuda.current_device() != index or code is None or k.dtype != dtype or v.dtype != dtype
+            or len(qs) != nd or len(vs) != nd or k.shape != qs or vs[:-2] != qs[:-2] or qs[-2] == 0
+            or vs[-2] % qs[-2] or decay.dtype != torch.float32 or decay.shape != vs[:-1]
+            or (state is not None and (state.get_device() != index or state.dtype != torch.float32
+                                       or state.shape != (vs[0], vs[-2], qs[-1], vs[-1])
+                                       or not state.is_contiguous()))):
+        _refuse_linear(q, k, v, decay, state, nd)
+    a, b, c, d = q.stride(), k.stride(), v.stride(), decay.stride()
+    if a[-1] != 1 or b[-1] != 1 or c[-1] != 1:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        a, b, c = q.stride(), k.stride(), v.stride()
+    if nd == 3:
+        return q, k, v, (a[0], 0, a[1], b[0], 0, b[1], c[0], 0, c[1], d[0], 0, d[1], qs[0], 1, qs[1], vs[1], qs[2],
+                         vs[2], code), index
+    return q, k, v, (*a[:3], *b[:3], *c[:3], *d, qs[0], qs[1], qs[2], vs[2], qs[3], vs[3], code), index
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
@@ -202,20 +219,23 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     logarithms, of any strides (a fixed decay a head is an expanded view). state (batch, v_heads, k_dim, v_dim)
     float32, zeros when None, is left as it was. lengths (batch,) int32: tokens past a sequence's length are not read,
     their outputs zeros. scale defaults to k_dim ** -0.5. Returns (out of v's shape, the state after the last token)."""
-    if q.dim() != 4 or v.dim() != 4:
-        raise ValueError("q, k, v (batch, tokens, heads, dim) expected")
-    A, keep, device = _linear(q, k, v, decay, state, scale)
+    q, k, v, sizes, index = _linear(q, k, v, decay, state, 4)
     if lengths is not None:
         _here(q, lengths)
-        _ints("lengths", lengths, (A.batch,))
-        A.lengths = lengths.data_ptr()
-    out = torch.empty(v.shape, dtype=v.dtype, device=device)
-    new = torch.empty((A.batch, A.v_heads, A.k_dim, A.v_dim), dtype=torch.float32, device=device)
-    A.state_in, A.state_out, A.out = ptr(state), new.data_ptr(), out.data_ptr()
-    lib, ref = _lib.lib(), ctypes.addressof(A)
-    n = lib.sc_linear_attention_workspace(ref)
-    ws = torch.empty(max(n, 16), dtype=torch.uint8, device=device)
-    check(lib.sc_linear_attention(ref, ws.data_ptr(), n, ptr(_lib.error_word(device)), stream()), "linear_attention")
+        _ints("lengths", lengths, (sizes[12],))
+    out = v.new_empty(v.shape)
+    new = decay.new_empty((sizes[12], sizes[15], sizes[16], sizes[17]))
+    lib = _lib.lib()
+    call = _LINEAR.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(),
+                        0 if state is None else state.data_ptr(), new.data_ptr(),
+                        0 if lengths is None else lengths.data_ptr(), out.data_ptr(), *sizes,
+                        sizes[16] ** -0.5 if scale is None else scale)
+    size = lib.sc_linear_attention_workspace(call)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    rc = lib.sc_linear_attention(call, 0 if ws is None else ws.data_ptr(), size, ptr(_lib.error_word(q.device)),
+                                 _stream(index))
+    if rc:
+        check(rc, "linear_attention")
     return out, new
 
 
@@ -223,14 +243,17 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dec
                           scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """linear_attention for one token a sequence: q, k (batch, k_heads, k_dim), v (batch, v_heads, v_dim), decay (batch,
     v_heads); state (batch, v_heads, k_dim, v_dim) float32 is updated in place. Returns out (batch, v_heads, v_dim)."""
-    if q.dim() != 3 or v.dim() != 3 or state is None:
-        raise ValueError("q, k, v (batch, heads, dim) and a state expected")
-    A, keep, device = _linear(q, k, v, decay, state, scale)
+    if state is None:
+        raise ValueError("a step needs the state it updates")
+    q, k, v, sizes, index = _linear(q, k, v, decay, state, 3)
     if out is None:
-        out = torch.empty(v.shape, dtype=v.dtype, device=device)
-    elif out.shape != v.shape or out.dtype != v.dtype or out.device != device or not out.is_contiguous():
+        out = v.new_empty(v.shape)
+    elif out.shape != v.shape or out.dtype != v.dtype or out.device != v.device or not out.is_contiguous():
         raise ValueError(f"out: contiguous {tuple(v.shape)} {v.dtype} expected")
-    A.state_in = A.state_out = state.data_ptr()
-    A.out = out.data_ptr()
-    check(_lib.lib().sc_linear_attention_step(ctypes.addressof(A), stream()), "linear_attention_step")
+    S = state.data_ptr()
+    rc = _lib.lib().sc_linear_attention_step(
+        _LINEAR.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), S, S, 0, out.data_ptr(), *sizes,
+                     sizes[16] ** -0.5 if scale is None else scale), _stream(index))
+    if rc:
+        check(rc, "linear_attention_step")
     return out

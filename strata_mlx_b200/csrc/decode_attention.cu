@@ -130,30 +130,45 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
   const int ht = blockIdx.y;
   const int64_t x = blockIdx.x;
   pdl_launch_dependents();
-  const int64_t U = units_before<THREADS>(A, UNIT, A.batch, s_sum, A.err), X = min(int64_t(A.columns), U);
+  // the units in all, and the sequence that holds this block's first one (a single pass up to THREADS sequences)
+  int64_t U, to;
+  const int first = tid < A.batch ? (length_of(A.pages, tid, A.err) + UNIT - 1) / UNIT : 0;
+  if (A.batch == 1) {
+    U = to = (length_of(A.pages, 0, nullptr) + UNIT - 1) / UNIT;
+  } else {
+    to = block_scan<THREADS>(first, s_sum, U);
+    if (A.batch > THREADS) U = units_before<THREADS>(A, UNIT, A.batch, s_sum, A.err);
+  }
+  U *= A.kv_heads;
+  const int64_t X = min(int64_t(A.columns), U);
   if (x >= X) return;
   int64_t u = x * U / X;
   const int64_t u1 = (x + 1) * U / X;
-  // the sequence that holds unit u
-  {
-    int64_t before = 0;
+  int b = 0;
+  int64_t before = 0;
+  if (A.batch > 1) {
     if (tid == 0) s_b = -1;
-    for (int b0 = 0; b0 < A.batch; b0 += THREADS) {
-      const int mine = b0 + tid < A.batch ? (length_of(A.pages, b0 + tid, nullptr) + UNIT - 1) / UNIT : 0;
-      int64_t total;
-      const int64_t to = before + block_scan<THREADS>(mine, s_sum, total);
+    __syncthreads();
+    int mine = first;
+    for (int b0 = 0;;) {
       if (u >= (to - mine) * A.kv_heads && u < to * A.kv_heads) s_b = b0 + tid, s_before = to - mine;
       __syncthreads();
-      if (s_b >= 0) break;
-      before += total;
+      b0 += THREADS;
+      if (s_b >= 0 || b0 >= A.batch) break;
+      int64_t total;
+      if (tid == THREADS - 1) s_before = to;  // where the next sequences begin
+      __syncthreads();
+      const int64_t from = s_before;
+      mine = b0 + tid < A.batch ? (length_of(A.pages, b0 + tid, nullptr) + UNIT - 1) / UNIT : 0;
+      to = from + block_scan<THREADS>(mine, s_sum, total);
     }
+    b = s_b, before = s_before;
+    if (b < 0) return;  // the lengths changed under the kernel
   }
-  int b = s_b;
-  if (b < 0) return;  // the lengths changed under the kernel
   int hk, ul;
   {
     const int n = (length_of(A.pages, b, nullptr) + UNIT - 1) / UNIT;
-    const int64_t in = u - s_before * A.kv_heads;
+    const int64_t in = u - before * A.kv_heads;
     hk = int(in / n), ul = int(in % n);
   }
   const Pages& P = A.pages;

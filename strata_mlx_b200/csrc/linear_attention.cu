@@ -96,10 +96,11 @@ int launch(const sc_linear& a, void* stream) {
 
 using namespace sc;
 
-extern "C" size_t sc_linear_attention_workspace(const sc_linear* a) { return la::check(a) ? 0 : 16; }
+extern "C" size_t sc_linear_attention_workspace(const sc_linear* a) { return la::check(a) || a->batch == 0 ? 0 : 16; }
 
 extern "C" int sc_linear_attention(const sc_linear* a, void* workspace, size_t workspace_bytes, int* err, void* stream) {
   if (int rc = la::check(a)) return rc;
+  if (a->batch == 0) return SC_OK;
   if (!workspace) return SC_ERR_ARG;
   if (workspace_bytes < sc_linear_attention_workspace(a)) return SC_ERR_WORKSPACE;
   return la::launch(*a, stream);

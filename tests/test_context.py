@@ -116,6 +116,14 @@ def test_linear_attention_workspace_and_the_step_form():
     assert lib.sc_linear_attention(ctypes.addressof(linear(batch=0)), FAKE, n, None, None) == 0
 
 
+def test_the_packed_call_is_the_structure():
+    """linear_attention packs sc_linear field by field: the same bytes as the structure."""
+    A = linear(tokens=7, batch=3, scale=0.25)
+    for i, (name, kind) in enumerate(A._fields_):
+        setattr(A, name, i + 1)
+    assert context._LINEAR.pack(*(getattr(A, name) for name, _ in A._fields_)) == bytes(A)
+
+
 def test_calls_refuse_tensors_off_the_gpu():
     k = torch.zeros((2, 16, 1, 64), dtype=torch.bfloat16)
     table, lengths = torch.zeros((1, 2), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
