@@ -34,7 +34,6 @@ constexpr int BLOCKS_PER_SM = 2;
 constexpr int SMS = 148;
 constexpr float SLACK = 8.f;   // log2 by which a score may pass the running maximum
 constexpr int JOIN_THREADS = 256;
-constexpr int JOIN_SLOTS = 1024;  // slots of a weight block
 
 struct Args {
   Pages pages;
@@ -181,16 +180,6 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
       continue;
     }
     const int ue = int(min(int64_t(n_units), ul + (u1 - u)));
-    // ---- the heads' queries, in the products' order
-    for (int i = tid; i < KC * 32; i += THREADS) {
-      const int c = (i / 32) * 4 + (i & 3), h = (i & 31) >> 2;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (h < heads && c < chunks)
-        v = *reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + b * A.q_row +
-                                            int64_t(hk * A.group + ht * HEADS + h) * A.q_head + 8 * c);
-      s_q[i / 32][i & 31] = v;
-    }
-    __syncthreads();
     // ---- this warp's tiles
     const int end = min(len, ue * UNIT);
     int base = (ul * WARPS + warp) * TILE;
@@ -252,13 +241,25 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
     float m0 = -INFINITY, m1 = -INFINITY, b0 = 0.f, b1 = 0.f, l0 = 0.f, l1 = 0.f;  // of heads 2t and 2t + 1
     int id[IDS], next[IDS];
     load_ids(base, id);
+    // the heads' queries, in the products' order
+    for (int i = tid; i < KC * 32; i += THREADS) {
+      const int c = (i / 32) * 4 + (i & 3), h = (i & 31) >> 2;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (h < heads && c < chunks)
+        v = *reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + b * A.q_row +
+                                            int64_t(hk * A.group + ht * HEADS + h) * A.q_head + 8 * c);
+      s_q[i / 32][i & 31] = v;
+    }
     uint32_t valid = load_k(base, id);
     load_v(base, id);
     load_ids(base + UNIT, next);
+    __syncthreads();
     for (; base < end; base += UNIT) {
-      float s[SUB][4];
+      float s[SUB][4], s2[SUB][4];  // two chains of products
 #pragma unroll
-      for (int i = 0; i < SUB; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+      for (int i = 0; i < SUB; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][e] = s2[i][e] = 0.f;
 #pragma unroll
       for (int j = 0; j < KC; ++j) {
         const uint4 q = s_q[j][lane];
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
           const uint4 &ka = kf[i][0][j], &kc = kf[i][1][j];
           const uint32_t a0[4] = {ka.x, kc.x, ka.y, kc.y}, a1[4] = {ka.z, kc.z, ka.w, kc.w};
           mma16816<T>(s[i], a0, q.x, q.y);
-          mma16816<T>(s[i], a1, q.z, q.w);
+          mma16816<T>(s2[i], a1, q.z, q.w);
         }
       }
       const uint32_t in = valid;
@@ -278,8 +279,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const bool ok = (in >> (2 * i + r)) & 1;
-          s[i][2 * r] = ok ? s[i][2 * r] * A.scale_log2 : -INFINITY;
-          s[i][2 * r + 1] = ok ? s[i][2 * r + 1] * A.scale_log2 : -INFINITY;
+          s[i][2 * r] = ok ? (s[i][2 * r] + s2[i][2 * r]) * A.scale_log2 : -INFINITY;
+          s[i][2 * r + 1] = ok ? (s[i][2 * r + 1] + s2[i][2 * r + 1]) * A.scale_log2 : -INFINITY;
           x0 = fmaxf(x0, s[i][2 * r]);
           x1 = fmaxf(x1, s[i][2 * r + 1]);
         }
@@ -407,52 +408,32 @@ struct Share {
 };
 template <int N>
 __device__ __forceinline__ Share share_of(const Args& A, int unit, int b, int64_t* sh) {
-  int64_t all = 0, before = 0;
-  for (int i = threadIdx.x; i < A.batch; i += N) {
-    const int64_t n = (length_of(A.pages, i, nullptr) + unit - 1) / unit;
-    all += n;
-    if (i < b) before += n;
-  }
   Share s;
-  s.U = block_sum<N>(all, sh) * A.kv_heads;
-  s.X = min(int64_t(A.columns), s.U);
-  s.before = block_sum<N>(before, sh) * A.kv_heads;
   s.n = (length_of(A.pages, b, nullptr) + unit - 1) / unit;
+  if (A.batch == 1) {
+    s.U = s.n, s.before = 0;
+  } else {
+    int64_t all = 0, before = 0;
+    for (int i = threadIdx.x; i < A.batch; i += N) {
+      const int64_t n = (length_of(A.pages, i, nullptr) + unit - 1) / unit;
+      all += n;
+      if (i < b) before += n;
+    }
+    s.U = block_sum<N>(all, sh), s.before = block_sum<N>(before, sh);
+  }
+  s.U *= A.kv_heads, s.before *= A.kv_heads;
+  s.X = min(int64_t(A.columns), s.U);
   return s;
 }
 
-// a warp: the joint maximum (finite) and sum of query head h, from its partial results or the one whole one
-__device__ __forceinline__ float2 joint(const Args& A, const Share& s, int b, int h, float* terms) {
-  const int lane = threadIdx.x & 31, hk = h / A.group, ht = (h % A.group) / HEADS, hr = (h % A.group) % HEADS;
-  const int first = s.first(hk), last = s.last(hk);
-  if (first == last) return A.whole_ml[int64_t(b) * A.q_heads + h];
-  auto at = [&](int x) { return ((int64_t(ht) * A.columns + x) * 2 + (x == first)) * HEADS + hr; };
-  float M = -INFINITY, L = 0.f;
-#pragma unroll 4
-  for (int x = first + lane; x <= last; x += 32) M = fmaxf(M, A.part_ml[at(x)].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  M = finite_or_0(M);
-#pragma unroll 4
-  for (int x = first + lane; x <= last; x += 32) {
-    const float2 ml = A.part_ml[at(x)];
-    const float c = exp2f(ml.x - M);
-    if (terms) terms[x - first] = c;
-    L += ml.y * c;
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-  return make_float2(M, L);
-}
-
 // Blocks 0 .. batch x q_heads - 1: a query head's output from its partial results (zeros for an empty sequence). The
-// rest, with weights: JOIN_SLOTS slots of a sequence.
-template <typename T, int DP>
+// rest, with weights: JOIN_THREADS slots of a sequence, a thread a slot, PACK scores at a time.
+template <typename T, int DP, int PACK>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int unit, int slot_blocks) {
   constexpr int LANES = DP / 4, GROUPS = JOIN_THREADS / LANES;  // threads of a row, and rows read side by side
   __shared__ int64_t sh[JOIN_THREADS / 32];
   __shared__ __align__(16) float s_o[GROUPS][DP];
-  __shared__ float s_c[BLOCKS_PER_SM * SMS], s_l;
+  __shared__ float2 s_gml[GROUPS];
   extern __shared__ float2 s_ml[];  // of every query head (weights)
   const int tid = threadIdx.x;
   const int outs = A.batch * A.q_heads;
@@ -468,53 +449,132 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int un
       return;
     }
     if (first == last) return;  // one block covered it
-    if (tid < 32) {
-      const float2 ml = joint(A, s, b, h, s_c);
-      if (tid == 0) s_l = ml.y;
-    }
-    __syncthreads();
+    // each row of threads an online join of every GROUPS-th partial result, four at a time
     const int row = tid / LANES, d = 4 * (tid % LANES);
-    const float* from = A.part_o + (int64_t(ht) * A.columns * 2 * HEADS + hr) * DP + d;
+    const int64_t base = int64_t(ht) * A.columns * 2 * HEADS + hr;
+    float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int x = first + row; x <= last; x += GROUPS) {
-      const float4 v = *reinterpret_cast<const float4*>(from + (int64_t(x) * 2 + (x == first)) * HEADS * DP);
-      const float c = s_c[x - first];
-      o.x += v.x * c, o.y += v.y * c, o.z += v.z * c, o.w += v.w * c;
+    for (int x0 = first + row; x0 <= last; x0 += 4 * GROUPS) {
+      float2 ml[4];
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int x = x0 + i * GROUPS;
+        ml[i] = make_float2(-INFINITY, 0.f);
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (x <= last) {
+          const int64_t at = base + (int64_t(x) * 2 + (x == first)) * HEADS;
+          ml[i] = A.part_ml[at];
+          v[i] = *reinterpret_cast<const float4*>(A.part_o + at * DP + d);
+        }
+      }
+      const float top = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), M), mb = finite_or_0(top);
+      const float c = exp2f(M - mb);
+      M = top;
+      L *= c, o.x *= c, o.y *= c, o.z *= c, o.w *= c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = exp2f(ml[i].x - mb);
+        L += ml[i].y * e;
+        o.x += v[i].x * e, o.y += v[i].y * e, o.z += v[i].z * e, o.w += v[i].w * e;
+      }
     }
     *reinterpret_cast<float4*>(&s_o[row][d]) = o;
+    if (d == 0) s_gml[row] = make_float2(M, L);
     __syncthreads();
     if (row == 0 && d < A.dim) {
 #pragma unroll
-      for (int i = 1; i < GROUPS; ++i) {
+      for (int i = 1; i < GROUPS; ++i) M = fmaxf(M, s_gml[i].x);
+      const float mb = finite_or_0(M);
+      L = 0.f;
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) {
         const float4 v = *reinterpret_cast<const float4*>(&s_o[i][d]);
-        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+        const float e = exp2f(s_gml[i].x - mb);
+        L += s_gml[i].y * e;
+        o.x += v.x * e, o.y += v.y * e, o.z += v.z * e, o.w += v.w * e;
       }
-      const float inv = s_l == 0.f ? 0.f : 1.f / s_l;
+      const float inv = L == 0.f ? 0.f : 1.f / L;
       *reinterpret_cast<uint2*>(out + d) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
     }
     return;
   }
-  const int e = blockIdx.x - outs, b = e / slot_blocks, s0 = (e % slot_blocks) * JOIN_SLOTS;
+  const int e = blockIdx.x - outs, b = e / slot_blocks, s0 = (e % slot_blocks) * JOIN_THREADS, s = s0 + tid;
   const int len = length_of(A.pages, b, nullptr);
   if (s0 >= len) return;
   const Share share = share_of<JOIN_THREADS>(A, unit, b, sh);
+  const int tiles = A.kv_heads * A.head_tiles;
+  const float* from = A.scores + (int64_t(b) * tiles * A.slots + s) * PACK;
+  const bool live = s < len;
   pdl_wait();
-  for (int h = tid / 32; h < A.q_heads; h += JOIN_THREADS / 32) {
-    const float2 ml = joint(A, share, b, h, nullptr);
-    if (tid % 32 == 0) s_ml[h] = make_float2(ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y);
+  // the scores of the first tiles load while the heads' statistics are worked out
+  constexpr int AHEAD = PACK == 8 ? 4 : 8;
+  float x[AHEAD][PACK];
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const float* p = from + int64_t(t0 + i) * A.slots * PACK;
+#pragma unroll
+      for (int h = 0; h < PACK; ++h) x[i][h] = -INFINITY;
+      if (live && t0 + i < tiles) {
+        if constexpr (PACK == 1) {
+          x[i][0] = *p;
+        } else if constexpr (PACK == 2) {
+          const float2 v = *reinterpret_cast<const float2*>(p);
+          x[i][0] = v.x, x[i][1] = v.y;
+        } else {
+#pragma unroll
+          for (int h = 0; h < PACK; h += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + h);
+            x[i][h] = v.x, x[i][h + 1] = v.y, x[i][h + 2] = v.z, x[i][h + 3] = v.w;
+          }
+        }
+      }
+    }
+  };
+  load(0);
+  const float old = live ? A.weight[b * A.weight_row + s] : 0.f;
+  // s_ml: (tiles, PACK) the heads' maxima and the inverses of their sums, zeros for heads that there are not
+  for (int i = tid; i < tiles * PACK; i += JOIN_THREADS) {
+    const int hk = i / PACK / A.head_tiles, ht = i / PACK % A.head_tiles, hh = ht * HEADS + i % PACK;
+    float2 ml = make_float2(0.f, 0.f);
+    if (hh < A.group) {
+      const int first = share.first(hk), last = share.last(hk);
+      if (first == last) {
+        ml = A.whole_ml[int64_t(b) * A.q_heads + hk * A.group + hh];
+      } else {
+        const int64_t base = int64_t(ht) * A.columns * 2 * HEADS + i % PACK;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll 8
+        for (int k = first; k <= last; ++k) {
+          const float2 v = A.part_ml[base + (int64_t(k) * 2 + (k == first)) * HEADS];
+          const float top = fmaxf(M, v.x), mb = finite_or_0(top);
+          L = L * exp2f(M - mb) + v.y * exp2f(v.x - mb);
+          M = top;
+        }
+        ml = make_float2(finite_or_0(M), L);
+      }
+      ml.y = ml.y == 0.f ? 0.f : 1.f / ml.y;
+    }
+    s_ml[i] = ml;
   }
   __syncthreads();
-  for (int s = s0 + tid; s < min(len, s0 + JOIN_SLOTS); s += JOIN_THREADS) {
-    float sum = 0.f;
-    for (int hk = 0; hk < A.kv_heads; ++hk)
-      for (int ht = 0; ht < A.head_tiles; ++ht) {
-        const float* x = A.scores + (((int64_t(b) * A.kv_heads + hk) * A.head_tiles + ht) * A.slots + s) * A.pack;
-        const float2* ml = s_ml + hk * A.group + ht * HEADS;
-        for (int h = 0; h < min(HEADS, A.group - ht * HEADS); ++h) sum += exp2f(x[h] - ml[h].x) * ml[h].y;
-      }
-    A.weight[b * A.weight_row + s] += sum;
+  float sum = 0.f;
+  for (int t0 = 0;;) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (t0 + i < tiles)
+#pragma unroll
+        for (int h = 0; h < PACK; ++h) {
+          const float2 ml = s_ml[(t0 + i) * PACK + h];
+          if (ml.y != 0.f) sum += exp2f(x[i][h] - ml.x) * ml.y;
+        }
+    t0 += AHEAD;
+    if (t0 >= tiles) break;
+    load(t0);
   }
+  if (live) A.weight[b * A.weight_row + s] = old + sum;
 }
 
 // ---- host
@@ -558,7 +618,7 @@ inline Layout layout(const sc_kv_pages& c, int q_heads) {
 using namespace sc;
 
 extern "C" size_t sc_decode_attention_workspace(const sc_kv_pages* kv, int q_heads) {
-  if (check_pages(kv) || q_heads < 1 || q_heads % kv->kv_heads || q_heads > 4096) return 0;
+  if (check_pages(kv) || q_heads < 1 || q_heads % kv->kv_heads || q_heads > 2048) return 0;
   return da::layout(*kv, q_heads).bytes;
 }
 
@@ -567,7 +627,7 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
                                    void* stream) {
   if (int rc = check_pages(kv)) return rc;
   if (kv->batch && (!q || !out || !workspace)) return SC_ERR_ARG;
-  if (q_heads < 1 || q_heads % kv->kv_heads || q_heads > 4096) return SC_ERR_SHAPE;
+  if (q_heads < 1 || q_heads % kv->kv_heads || q_heads > 2048) return SC_ERR_SHAPE;
   if (((q_row | q_head) & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & 15))
     return SC_ERR_ALIGN;
@@ -592,7 +652,7 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
   }
   A.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int slot_blocks = kv->weight ? int(ceil_div(A.slots, da::JOIN_SLOTS)) : 0;
+  const int slot_blocks = kv->weight ? int(ceil_div(A.slots, da::JOIN_THREADS)) : 0;
   const int64_t join_blocks = int64_t(kv->batch) * (q_heads + slot_blocks);
   if (join_blocks > INT32_MAX) return SC_ERR_SHAPE;
   auto run = [&](auto t, auto dp, auto sub) -> int {
@@ -603,14 +663,16 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(join_blocks));
     cfg.blockDim = dim3(da::JOIN_THREADS);
-    cfg.dynamicSmemBytes = kv->weight ? size_t(q_heads) * 8 : 0;
+    cfg.dynamicSmemBytes = kv->weight ? size_t(kv->kv_heads) * l.head_tiles * l.pack * 8 : 0;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaError_t e = cudaLaunchKernelEx(&cfg, da::join_kernel<T, DP>, A, l.unit, slot_blocks))
+    const auto join = l.pack == 1 ? da::join_kernel<T, DP, 1> : l.pack == 2 ? da::join_kernel<T, DP, 2>
+                    : l.pack == 4 ? da::join_kernel<T, DP, 4> : da::join_kernel<T, DP, 8>;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, join, A, l.unit, slot_blocks))
       return cuda_failed(e, "decode attention join launch");
     if (cudaError_t e = cudaGetLastError()) return cuda_failed(e, "decode attention launch");
     return SC_OK;
