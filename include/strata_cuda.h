@@ -367,7 +367,7 @@ typedef struct sc_linear {
 SC_API int sc_linear_attention(const sc_linear* a, void* workspace, size_t workspace_bytes, int* err, void* stream);
 SC_API size_t sc_linear_attention_workspace(const sc_linear* a);
 
-/* One token a sequence (tokens = 1, lengths NULL): the recurrence itself. */
+/* One token a sequence (tokens = 1, lengths NULL, state_in given): the recurrence itself. */
 SC_API int sc_linear_attention_step(const sc_linear* a, void* stream);
 
 /* No counterpart in strata-mlx: an addition for callers that cannot allocate device memory.

@@ -64,13 +64,82 @@ __global__ void __launch_bounds__(COLS * PARTS) recurrent_kernel(const sc_linear
   }
 }
 
+// One token a sequence. The states' bytes bound it, read and written once: a block per (sequence, value head, 32 value
+// dimensions), a thread four of them in every 32nd row, all its rows' loads in flight before the first is used. The
+// rows' parts of the output meet by shuffles and in shared memory. Blocks of 32 columns (128-byte pieces of rows)
+// give one sequence's 16 heads four blocks each.
+constexpr int STEP_THREADS = 256, STEP_ROWS = STEP_THREADS / 8;
+
+template <typename T>
+__global__ void __launch_bounds__(STEP_THREADS) step_kernel(const sc_linear A) {
+  __shared__ float4 s_o[STEP_THREADS / 32][8];
+  const int h = blockIdx.y, b = blockIdx.z, hk = h / (A.v_heads / A.k_heads);
+  const int col = blockIdx.x * 32 + 4 * (threadIdx.x & 7), row = threadIdx.x >> 3;
+  const bool live = col < A.v_dim;
+  const int64_t at = (int64_t(b) * A.v_heads + h) * A.k_dim * A.v_dim + col;
+  float4 S[MAXK / STEP_ROWS];
+#pragma unroll
+  for (int i = 0; i < MAXK / STEP_ROWS; ++i) {
+    const int r = row + STEP_ROWS * i;
+    if (live && r < A.k_dim) S[i] = *reinterpret_cast<const float4*>(A.state_in + at + int64_t(r) * A.v_dim);
+  }
+  const float g = A.decay[b * A.decay_row + h * A.decay_head];
+  const T* q = static_cast<const T*>(A.q) + b * A.q_row + hk * A.q_head;
+  const T* k = static_cast<const T*>(A.k) + b * A.k_row + hk * A.k_head;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
+    const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const T*>(A.v) + b * A.v_row + h * A.v_head + col);
+    const T* xv = reinterpret_cast<const T*>(&x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = to_f32(xv[e]);
+  }
+  // as in the recurrence over a prompt: the difference form near 1
+  const bool near = g > -0.69314718f;
+  const float a = near ? expm1f(g) : expf(g);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < MAXK / STEP_ROWS; ++i) {
+    const int r = row + STEP_ROWS * i;
+    if (live && r < A.k_dim) {
+      const float kr = to_f32(k[r]), qr = to_f32(q[r]);
+      float* s = reinterpret_cast<float*>(&S[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] = fmaf(kr, v[e], near ? fmaf(a, s[e], s[e]) : a * s[e]);
+      o.x = fmaf(qr, S[i].x, o.x), o.y = fmaf(qr, S[i].y, o.y), o.z = fmaf(qr, S[i].z, o.z), o.w = fmaf(qr, S[i].w, o.w);
+      *reinterpret_cast<float4*>(A.state_out + at + int64_t(r) * A.v_dim) = S[i];
+    }
+  }
+#pragma unroll
+  for (int w = 8; w < 32; w <<= 1) {
+    o.x += __shfl_xor_sync(0xffffffffu, o.x, w);
+    o.y += __shfl_xor_sync(0xffffffffu, o.y, w);
+    o.z += __shfl_xor_sync(0xffffffffu, o.z, w);
+    o.w += __shfl_xor_sync(0xffffffffu, o.w, w);
+  }
+  if ((threadIdx.x & 31) < 8) s_o[threadIdx.x >> 5][threadIdx.x & 7] = o;
+  __syncthreads();
+  if (threadIdx.x < 8 && live) {
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < STEP_THREADS / 32; ++w) {
+      const float4 p = s_o[w][threadIdx.x];
+      o.x += p.x, o.y += p.y, o.z += p.z, o.w += p.w;
+    }
+    uint2 x;
+    T* to = reinterpret_cast<T*>(&x);
+    to[0] = from_f32<T>(o.x * A.scale), to[1] = from_f32<T>(o.y * A.scale);
+    to[2] = from_f32<T>(o.z * A.scale), to[3] = from_f32<T>(o.w * A.scale);
+    *reinterpret_cast<uint2*>(static_cast<T*>(A.out) + (int64_t(b) * A.v_heads + h) * A.v_dim + col) = x;
+  }
+}
+
 inline int check(const sc_linear* a) {
   if (!a || a->batch < 0 || a->tokens < 0 || (a->batch && !a->state_out) ||
       (a->batch && a->tokens && (!a->q || !a->k || !a->v || !a->decay || !a->out)))
     return SC_ERR_ARG;
   if (a->dtype != SC_F16 && a->dtype != SC_BF16) return SC_ERR_DTYPE;
   if (a->k_heads < 1 || a->v_heads < 1 || a->v_heads % a->k_heads || a->k_dim < 8 || a->k_dim % 8 || a->k_dim > MAXK ||
-      a->v_dim < 8 || a->v_dim % 8 || a->v_dim > 128 || a->batch > 65535)
+      a->v_dim < 8 || a->v_dim % 8 || a->v_dim > 128 || a->batch > 65535 || a->v_heads > 65535)
     return SC_ERR_SHAPE;
   const int64_t strides = a->q_row | a->q_token | a->q_head | a->k_row | a->k_token | a->k_head | a->v_row | a->v_token |
                           a->v_head;
@@ -109,5 +178,12 @@ extern "C" int sc_linear_attention(const sc_linear* a, void* workspace, size_t w
 extern "C" int sc_linear_attention_step(const sc_linear* a, void* stream) {
   if (int rc = la::check(a)) return rc;
   if (a->tokens != 1 || a->lengths) return SC_ERR_SHAPE;
-  return la::launch(*a, stream);
+  if (a->batch == 0) return SC_OK;
+  if (!a->state_in) return SC_ERR_ARG;
+  const dim3 grid(unsigned((a->v_dim + 31) / 32), unsigned(a->v_heads), unsigned(a->batch));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->dtype == SC_BF16) la::step_kernel<__nv_bfloat16><<<grid, la::STEP_THREADS, 0, s>>>(*a);
+  else la::step_kernel<__half><<<grid, la::STEP_THREADS, 0, s>>>(*a);
+  if (cudaError_t e = cudaGetLastError()) return cuda_failed(e, "linear attention step launch");
+  return SC_OK;
 }
