@@ -42,7 +42,7 @@ def _here(*ts) -> torch.device:
 
 
 def _ints(name: str, t: torch.Tensor, shape: tuple) -> None:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name}: contiguous int32 {shape} expected, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -89,6 +89,7 @@ class KVPages:
         self._lib, self._err = _lib.lib(), ptr(_lib.error_word(self.device))
         self._ws: dict = {}
         self._sizes: dict = {}  # of attend's workspace, by the query heads
+        self._evict_sizes: dict = {}  # of evict's, by the budget
         self._index, self._scale = self.device.index, self.head_dim ** -0.5
 
     def _workspace(self, what: str, size: int, s: int) -> tuple:
@@ -144,22 +145,31 @@ class KVPages:
         theirs until all are done). Slots past the new length keep what they held."""
         if self.weight is None or self.position is None:
             raise ValueError("evict needs the cache's weight and position")
-        _here(self.k, seen)
-        _ints("seen", seen, (self.batch,))
-        weight, position, lengths = (self.weight, self.position, self.lengths) if out is None else out
-        _here(self.k, weight, position, lengths)
-        for name, t, dtype in (("weight", weight, torch.float32), ("position", position, torch.int32)):
-            if (t.dtype != dtype or t.dim() != 2 or t.shape[0] != self.batch or t.stride(1) != 1
-                    or t.shape[1] < min(keep, self.slots)):
-                raise ValueError(f"out {name}: {dtype} ({self.batch}, at least {min(keep, self.slots)}) expected")
-        _ints("out lengths", lengths, (self.batch,))
-        s = _stream(self._index)
         if keep < 0 or sinks < 0 or recent < 0 or sinks + recent > keep:
             raise ValueError(f"sinks {sinks} and recent {recent} have to fit in keep {keep}")
-        ws = self._workspace("evict", self._lib.sc_evict_workspace(self._ref, keep), s)
-        check(self._lib.sc_evict(self._ref, seen.data_ptr(), keep, sinks, recent, weight.data_ptr(), weight.stride(0),
-                                 position.data_ptr(), position.stride(0), lengths.data_ptr(), ws[0], ws[1], self._err,
-                                 s), "evict")
+        weight, position, lengths = (self.weight, self.position, self.lengths) if out is None else out
+        index, n, room = self._index, self.batch, min(keep, self.slots)
+        if seen.get_device() != index or torch.cuda.current_device() != index:
+            raise ValueError(f"seen on {seen.device}; the cache is on {self.device}, which has to be current")
+        _ints("seen", seen, (n,))
+        if out is not None:
+            for name, t, dtype in (("weight", weight, torch.float32), ("position", position, torch.int32)):
+                shape = t.shape
+                if (t.get_device() != index or t.dtype != dtype or len(shape) != 2 or shape[0] != n or shape[1] < room
+                        or t.stride(1) != 1):
+                    raise ValueError(f"out {name}: {dtype} ({n}, at least {room}) on {self.device} expected")
+            if lengths.get_device() != index:
+                raise ValueError(f"out lengths: on {self.device} expected")
+            _ints("out lengths", lengths, (n,))
+        s = _stream(index)
+        size = self._evict_sizes.get(keep)
+        if size is None:
+            size = self._evict_sizes[keep] = self._lib.sc_evict_workspace(self._ref, keep)
+        ws = self._workspace("evict", size, s)
+        rc = self._lib.sc_evict(self._ref, seen.data_ptr(), keep, sinks, recent, weight.data_ptr(), weight.stride(0),
+                                position.data_ptr(), position.stride(0), lengths.data_ptr(), ws[0], ws[1], self._err, s)
+        if rc:
+            check(rc, "evict")
 
 
 def decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,

@@ -27,6 +27,7 @@ constexpr int BINS = 2048, BITS = 11;
 constexpr int MAX_CLUSTER = 8;
 constexpr int PER_BLOCK = 16384;  // slots of a block before the cluster grows
 constexpr int MOST = 50 * 1024;   // slots a block can hold the keys of (200 KB); past 8 such blocks keys are made anew
+constexpr int FETCH = 8;          // weights and positions a thread loads at a time
 constexpr int MOVE_WARPS = 8;
 constexpr uint32_t KEPT = 0xffffffffu;
 
@@ -90,22 +91,33 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const Args A) {
   // this block's slots, a whole number of them to each warp
   const int per = ((n + blocks - 1) / blocks + THREADS - 1) / THREADS * THREADS;
   const int s0 = min(n, rank * per), mine = min(n, s0 + per) - s0, span = per / WARPS;
-  if (n <= keep) {
-    for (int i = tid; i < mine; i += THREADS) {
-      const float x = w[s0 + i];
-      const int32_t p = pos[s0 + i];
-      wo[s0 + i] = x;
-      po[s0 + i] = p;
+  // a batch of this block's weights and positions, loaded together; those below the budget are copied at once (the
+  // evicted among them are overwritten when their slots are filled)
+  auto fetch = [&](auto f) {
+    for (int i0 = tid; i0 < mine; i0 += FETCH * THREADS) {
+      float x[FETCH];
+      int32_t p[FETCH];
+#pragma unroll
+      for (int u = 0; u < FETCH; ++u)
+        if (i0 + u * THREADS < mine) x[u] = w[s0 + i0 + u * THREADS], p[u] = pos[s0 + i0 + u * THREADS];
+#pragma unroll
+      for (int u = 0; u < FETCH; ++u) {
+        const int i = i0 + u * THREADS;
+        if (i < mine) {
+          if (s0 + i < keep) wo[s0 + i] = x[u], po[s0 + i] = p[u];
+          f(i, x[u], p[u]);
+        }
+      }
     }
+  };
+  if (n <= keep) {
+    fetch([](int, float, int32_t) {});
     cluster.sync();  // lengths_out may be the lengths themselves
     if (rank == 0 && tid == 0) A.count[b] = 0, A.lengths_out[b] = n;
     return;
   }
   const int64_t from = int64_t(A.seen[b]) - A.recent;
-  auto safe_at = [&](int i) {
-    const int32_t p = pos[s0 + i];
-    return p < A.sinks || p >= from;
-  };
+  auto is_safe = [&](int32_t p) { return p < A.sinks || p >= from; };
   // every block's sum of a value, and the sums of the blocks before this one
   auto cluster_sum = [&](int v, int use, int& before) {
     const int t = block_sum(v, s_warp);
@@ -123,17 +135,17 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const Args A) {
   };
   // ---- keys: first with the kept places above all weights
   int c = 0;
-  for (int i = tid; i < mine; i += THREADS) {
-    const bool safe = safe_at(i);
+  fetch([&](int i, float x, int32_t p) {
+    const bool safe = is_safe(p);
     c += safe;
-    if constexpr (HELD) s_key[i] = safe ? KEPT : order_of(w[s0 + i]);
-  }
+    if constexpr (HELD) s_key[i] = safe ? KEPT : order_of(x);
+  });
   int none;
   const int safes = cluster_sum(c, 0, none);
   // more kept places than slots stay (positions that repeat): only they are ranked, by weight
   const bool crowded = safes > keep;
   auto make = [&](int i) -> uint32_t {
-    const bool safe = safe_at(i);
+    const bool safe = is_safe(pos[s0 + i]);
     return crowded ? (safe ? order_of(w[s0 + i]) : 0u) : safe ? KEPT : order_of(w[s0 + i]);
   };
   if (HELD && crowded)
@@ -240,12 +252,6 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const Args A) {
     if (hole) A.dst[int64_t(b) * A.cap + hole0 + __popc(h & below)] = s;
     if (mover) A.src[int64_t(b) * A.cap + mover0 + __popc(m & below)] = s;
     hole0 += __popc(h), mover0 += __popc(m);
-    if (stays && s < keep) {
-      const float x = w[s];
-      const int32_t p = pos[s];
-      wo[s] = x;
-      po[s] = p;
-    }
   });
   cluster.sync();  // no block leaves while another may read its shared memory; and the lengths are read
   if (rank == 0 && tid == 0) A.count[b] = all_movers, A.lengths_out[b] = keep;

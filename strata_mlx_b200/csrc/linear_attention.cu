@@ -77,15 +77,18 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(const sc_linear A) {
   const int col = blockIdx.x * 32 + 4 * (threadIdx.x & 7), row = threadIdx.x >> 3;
   const bool live = col < A.v_dim;
   const int64_t at = (int64_t(b) * A.v_heads + h) * A.k_dim * A.v_dim + col;
+  const T* q = static_cast<const T*>(A.q) + b * A.q_row + hk * A.q_head;
+  const T* k = static_cast<const T*>(A.k) + b * A.k_row + hk * A.k_head;
   float4 S[MAXK / STEP_ROWS];
+  float kr[MAXK / STEP_ROWS], qr[MAXK / STEP_ROWS];
 #pragma unroll
   for (int i = 0; i < MAXK / STEP_ROWS; ++i) {
     const int r = row + STEP_ROWS * i;
+    kr[i] = r < A.k_dim ? to_f32(k[r]) : 0.f, qr[i] = r < A.k_dim ? to_f32(q[r]) : 0.f;
+    S[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live && r < A.k_dim) S[i] = *reinterpret_cast<const float4*>(A.state_in + at + int64_t(r) * A.v_dim);
   }
   const float g = A.decay[b * A.decay_row + h * A.decay_head];
-  const T* q = static_cast<const T*>(A.q) + b * A.q_row + hk * A.q_head;
-  const T* k = static_cast<const T*>(A.k) + b * A.k_row + hk * A.k_head;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   if (live) {
     const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const T*>(A.v) + b * A.v_row + h * A.v_head + col);
@@ -100,14 +103,11 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(const sc_linear A) {
 #pragma unroll
   for (int i = 0; i < MAXK / STEP_ROWS; ++i) {
     const int r = row + STEP_ROWS * i;
-    if (live && r < A.k_dim) {
-      const float kr = to_f32(k[r]), qr = to_f32(q[r]);
-      float* s = reinterpret_cast<float*>(&S[i]);
+    float* s = reinterpret_cast<float*>(&S[i]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] = fmaf(kr, v[e], near ? fmaf(a, s[e], s[e]) : a * s[e]);
-      o.x = fmaf(qr, S[i].x, o.x), o.y = fmaf(qr, S[i].y, o.y), o.z = fmaf(qr, S[i].z, o.z), o.w = fmaf(qr, S[i].w, o.w);
-      *reinterpret_cast<float4*>(A.state_out + at + int64_t(r) * A.v_dim) = S[i];
-    }
+    for (int e = 0; e < 4; ++e) s[e] = fmaf(kr[i], v[e], near ? fmaf(a, s[e], s[e]) : a * s[e]);
+    o.x = fmaf(qr[i], s[0], o.x), o.y = fmaf(qr[i], s[1], o.y), o.z = fmaf(qr[i], s[2], o.z), o.w = fmaf(qr[i], s[3], o.w);
+    if (live && r < A.k_dim) *reinterpret_cast<float4*>(A.state_out + at + int64_t(r) * A.v_dim) = S[i];
   }
 #pragma unroll
   for (int w = 8; w < 32; w <<= 1) {
