@@ -3,10 +3,10 @@
 //   plan_kernel  a cluster of blocks a sequence, each with a stretch of its slots. A slot's key is its weight as an
 //                unsigned integer of the same order, the largest integer where its place keeps it; keys stay in shared
 //                memory. The key of the last slot that stays is found digit by digit below the bits that all keys
-//                share: a histogram of 2048 digits a round in every block, summed over the cluster through distributed
-//                shared memory. Then each warp ranks its slots in slot order (ballots, sums over warps and blocks) and
-//                lists the holes (evicted slots below the budget) and the movers (kept slots past it): as many of one
-//                as of the other. Latency bounds it: a round is two barriers and a walk over the histogram.
+//                share: a histogram of 512 digits a round in every block, summed over the cluster through distributed
+//                shared memory, until so few keys are left that they are ranked one against another. Then each warp counts and lists, in slot order, the holes (evicted slots below the
+//                budget) and the movers (kept slots past it): as many of one as of the other. Latency bounds it: a
+//                round is two barriers and a walk over the histogram.
 //   move_kernel  mover i's keys, values, weight and position into hole i. Sources lie at or past the budget and
 //                destinations below it, so no row is read that another warp writes, and the order is free. Bandwidth
 //                bounds it: a warp fetches the list entries and page ids of its rows at once and keeps four 16-byte
@@ -22,12 +22,14 @@ namespace ev {
 
 namespace cg = cooperative_groups;
 
-constexpr int THREADS = 1024, WARPS = THREADS / 32;
-constexpr int BINS = 2048, BITS = 11;
+constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int BITS = 9, BINS = 1 << BITS;  // a digit a thread
+constexpr int FEW = 256;          // keys that are ranked one against another
 constexpr int MAX_CLUSTER = 8;
-constexpr int PER_BLOCK = 16384;  // slots of a block before the cluster grows
+constexpr int STRETCH = 128 * WARPS;  // a block's slots are a multiple
+constexpr int PER_BLOCK = 2 * STRETCH;  // slots of a block before the cluster grows
 constexpr int MOST = 50 * 1024;   // slots a block can hold the keys of (200 KB); past 8 such blocks keys are made anew
-constexpr int FETCH = 8;          // weights and positions a thread loads at a time
+constexpr int FETCH = 16;         // weights and positions a thread loads at a time
 constexpr int MOVE_WARPS = 8;
 constexpr uint32_t KEPT = 0xffffffffu;
 
@@ -53,15 +55,6 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// sums and scans over a block; `sh` holds WARPS values
-__device__ __forceinline__ int block_sum(int v, int* sh) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int t = __reduce_add_sync(0xffffffffu, sh[threadIdx.x & 31]);
-  __syncthreads();
-  return t;
-}
 __device__ __forceinline__ int warp_scan(int v) {  // inclusive
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -74,11 +67,11 @@ __device__ __forceinline__ int warp_scan(int v) {  // inclusive
 
 template <bool HELD>
 __global__ void __launch_bounds__(THREADS) plan_kernel(const Args A) {
-  extern __shared__ uint32_t s_key[];
-  __shared__ int s_hist[2][BINS];
-  __shared__ int s_warp[WARPS], s_pick[2];
-  __shared__ int s_out[4][2];         // read by the other blocks, a pair for each use
-  __shared__ uint32_t s_span[2];
+  extern __shared__ __align__(16) uint32_t s_key[];
+  __shared__ __align__(16) int s_hist[2][BINS];
+  __shared__ int s_warp[4][WARPS], s_pick[3], s_n;
+  __shared__ uint32_t s_few[2][FEW];  // this block's, and the cluster's
+  __shared__ int4 s_mine[3], s_all[2];  // what the other blocks read; sums over the cluster
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
   const int b = blockIdx.x / blocks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -88,11 +81,15 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const Args A) {
   const int32_t* pos = A.position + b * A.position_row;
   float* wo = A.weight_out + b * A.weight_out_row;
   int32_t* po = A.position_out + b * A.position_out_row;
-  // this block's slots, a whole number of them to each warp
-  const int per = ((n + blocks - 1) / blocks + THREADS - 1) / THREADS * THREADS;
-  const int s0 = min(n, rank * per), mine = min(n, s0 + per) - s0, span = per / WARPS;
-  // a batch of this block's weights and positions, loaded together; those below the budget are copied at once (the
-  // evicted among them are overwritten when their slots are filled)
+  // this block's slots, a whole number of steps of 128 to each warp
+  const int per = ((n + blocks - 1) / blocks + STRETCH - 1) / STRETCH * STRETCH;
+  const int s0 = min(n, rank * per), mine = min(n, s0 + per) - s0;
+  auto sync = [&] {
+    if (blocks > 1) cluster.sync();
+    else __syncthreads();
+  };
+  // weights and positions, FETCH a thread at a time; those below the budget are copied at once (the evicted among
+  // them are overwritten when their slots are filled)
   auto fetch = [&](auto f) {
     for (int i0 = tid; i0 < mine; i0 += FETCH * THREADS) {
       float x[FETCH];
@@ -112,148 +109,217 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const Args A) {
   };
   if (n <= keep) {
     fetch([](int, float, int32_t) {});
-    cluster.sync();  // lengths_out may be the lengths themselves
+    sync();  // lengths_out may be the lengths themselves
     if (rank == 0 && tid == 0) A.count[b] = 0, A.lengths_out[b] = n;
     return;
   }
   const int64_t from = int64_t(A.seen[b]) - A.recent;
   auto is_safe = [&](int32_t p) { return p < A.sinks || p >= from; };
-  // every block's sum of a value, and the sums of the blocks before this one
-  auto cluster_sum = [&](int v, int use, int& before) {
-    const int t = block_sum(v, s_warp);
-    before = 0;
-    if (blocks == 1) return t;
-    if (tid == 0) s_out[use][0] = t;
-    cluster.sync();
-    int all = 0;
-    for (int r = 0; r < blocks; ++r) {
-      const int x = *cluster.map_shared_rank(&s_out[use][0], r);
-      if (r < rank) before += x;
-      all += x;
-    }
-    return all;
-  };
-  // ---- keys: first with the kept places above all weights
-  int c = 0;
+  for (int i = tid; i < 2 * BINS; i += THREADS) s_hist[0][i] = 0;
+  // ---- keys; how many slots are kept by their place, and the least and largest of the other keys
+  int safes = 0;
+  uint32_t lo = KEPT, hi = 0;
   fetch([&](int i, float x, int32_t p) {
     const bool safe = is_safe(p);
-    c += safe;
-    if constexpr (HELD) s_key[i] = safe ? KEPT : order_of(x);
+    const uint32_t k = safe ? KEPT : order_of(x);
+    safes += safe;
+    if (!safe) lo = min(lo, k), hi = max(hi, k);
+    if constexpr (HELD) s_key[i] = k;
   });
-  int none;
-  const int safes = cluster_sum(c, 0, none);
+  if constexpr (HELD) {  // a step's end holds no slot's key
+    const int end = (mine + 127) / 128 * 128;
+    for (int i = mine + tid; i < end; i += THREADS) s_key[i] = 0;
+  }
+  safes = __reduce_add_sync(0xffffffffu, safes);
+  lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) s_warp[0][warp] = safes, s_warp[1][warp] = int(lo), s_warp[2][warp] = int(hi);
+  __syncthreads();
+  if (warp == 0) {
+    const bool in = lane < WARPS;
+    const int4 v = make_int4(__reduce_add_sync(0xffffffffu, in ? s_warp[0][lane] : 0),
+                             int(__reduce_min_sync(0xffffffffu, in ? uint32_t(s_warp[1][lane]) : KEPT)),
+                             int(__reduce_max_sync(0xffffffffu, in ? uint32_t(s_warp[2][lane]) : 0u)), 0);
+    if (lane == 0) s_mine[0] = v;
+  }
+  sync();
+  if (warp == 0) {
+    const int4 v = lane < blocks ? *cluster.map_shared_rank(&s_mine[0], lane) : make_int4(0, int(KEPT), 0, 0);
+    const int4 r = make_int4(__reduce_add_sync(0xffffffffu, v.x), int(__reduce_min_sync(0xffffffffu, uint32_t(v.y))),
+                             int(__reduce_max_sync(0xffffffffu, uint32_t(v.z))), 0);
+    if (lane == 0) s_all[0] = r;
+  }
+  __syncthreads();
+  safes = s_all[0].x, lo = uint32_t(s_all[0].y), hi = uint32_t(s_all[0].z);
   // more kept places than slots stay (positions that repeat): only they are ranked, by weight
   const bool crowded = safes > keep;
   auto make = [&](int i) -> uint32_t {
     const bool safe = is_safe(pos[s0 + i]);
     return crowded ? (safe ? order_of(w[s0 + i]) : 0u) : safe ? KEPT : order_of(w[s0 + i]);
   };
-  if (HELD && crowded)
-    for (int i = tid; i < mine; i += THREADS) s_key[i] = make(i);
-  __syncthreads();
+  if (crowded) {
+    lo = 0, hi = KEPT - 1;
+    if constexpr (HELD) {
+      for (int i = tid; i < mine; i += THREADS) s_key[i] = make(i);
+      __syncthreads();
+    }
+  }
   auto key_at = [&](int i) { return HELD ? s_key[i] : make(i); };
-  // ---- the bits that the keys below KEPT share
-  uint32_t lo = KEPT, hi = 0;
-  for (int i = tid; i < mine; i += THREADS) {
-    const uint32_t k = key_at(i);
-    if (k != KEPT) lo = min(lo, k), hi = max(hi, k);
-  }
-  lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
-  if (tid == 0) s_span[0] = KEPT, s_span[1] = 0;
-  __syncthreads();
-  if (lane == 0) atomicMin(&s_span[0], lo), atomicMax(&s_span[1], hi);
-  for (int i = tid; i < 2 * BINS; i += THREADS) s_hist[0][i] = 0;
-  if (blocks > 1) cluster.sync();
-  else __syncthreads();
-  lo = KEPT, hi = 0;
-  for (int r = 0; r < blocks; ++r) {
-    lo = min(lo, *cluster.map_shared_rank(&s_span[0], r));
-    hi = max(hi, *cluster.map_shared_rank(&s_span[1], r));
-  }
-  int want = crowded ? keep : keep - safes;  // how many of the slots below KEPT stay
-  uint32_t key = KEPT;                       // slots above it stay, `want` of those at it
+  // ---- the key of the last slot that stays: slots above it stay, `want` of those at it
+  int want = crowded ? keep : keep - safes;
+  uint32_t key = KEPT;
   if (want > 0) {
-    int bits = hi > lo ? 32 - __clz(hi ^ lo) : 0;  // not shared
+    int bits = hi > lo ? 32 - __clz(hi ^ lo) : 0;  // those that the keys below KEPT do not share
     key = bits < 32 ? (hi >> bits) << bits : 0u;
-    for (int round = 0; bits > 0; ++round) {
+    int left = INT32_MAX;  // keys that begin as `key` does
+    for (int round = 0; bits > 0 && left > FEW; ++round) {
       const int take = min(bits, BITS), shift = bits - take;
       const uint32_t known = bits < 32 ? ~0u << bits : 0u, digit = (1u << take) - 1;
       int* hist = s_hist[round & 1];
+#pragma unroll 4
       for (int i = tid; i < mine; i += THREADS) {
         const uint32_t k = key_at(i);
         if (k != KEPT && (k & known) == key) atomicAdd(&hist[(k >> shift) & digit], 1);
       }
-      if (blocks > 1) cluster.sync();
-      else __syncthreads();
-      // thread t takes the digits 2047 - 2t and 2046 - 2t, so that a scan counts from the top
-      const int d1 = BINS - 1 - 2 * tid, d0 = d1 - 1;
-      int n1 = 0, n0 = 0;
-      for (int r = 0; r < blocks; ++r) {
-        const int2 v = *reinterpret_cast<const int2*>(cluster.map_shared_rank(hist, r) + d0);
-        n0 += v.x, n1 += v.y;
-      }
-      const int inc = warp_scan(n0 + n1);
-      if (lane == 31) s_warp[warp] = inc;
+      sync();
+      // a digit a thread, from the top down
+      const int d = BINS - 1 - tid;
+      int v = 0;
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r)
+        if (r < blocks) v += *cluster.map_shared_rank(hist + d, r);
+      s_hist[(round + 1) & 1][d] = 0;  // which no block reads any more: the next round's
+      const int inc = warp_scan(v);
+      if (lane == 31) s_warp[0][warp] = inc;
       __syncthreads();
-      const int sums = s_warp[lane], upto = __shfl_sync(0xffffffffu, warp_scan(sums) - sums, warp) + inc - n0 - n1;
-      if (upto < want && want <= upto + n1) s_pick[0] = d1, s_pick[1] = upto;
-      if (upto + n1 < want && want <= upto + n1 + n0) s_pick[0] = d0, s_pick[1] = upto + n1;
-      // the other histogram, which no block reads any more, is the next round's
-      for (int i = tid; i < BINS; i += THREADS) s_hist[(round + 1) & 1][i] = 0;
+      int upto = inc - v;
+#pragma unroll
+      for (int q = 0; q < WARPS; ++q) upto += q < warp ? s_warp[0][q] : 0;
+      if (upto < want && want <= upto + v) s_pick[0] = d, s_pick[1] = upto, s_pick[2] = v;
       __syncthreads();
       key |= uint32_t(s_pick[0]) << shift;
       want -= s_pick[1];
+      left = s_pick[2];
       bits = shift;
     }
+    if (bits > 0) {  // few keys are left: each counts those above it
+      const uint32_t known = ~0u << bits;
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (int i = tid; i < mine; i += THREADS) {
+        const uint32_t k = key_at(i);
+        if (k != KEPT && (k & known) == key) s_few[0][atomicAdd(&s_n, 1)] = k;
+      }
+      sync();
+      if (warp < blocks) {
+        int at = 0, m = 0;
+        for (int r = 0; r <= warp; ++r) at += m, m = *cluster.map_shared_rank(&s_n, r);
+        const uint32_t* from = cluster.map_shared_rank(&s_few[0][0], warp);
+        for (int i = lane; i < m; i += 32) s_few[1][at + i] = from[i];
+      }
+      __syncthreads();
+      if (tid < left) {
+        const uint32_t k = s_few[1][tid];
+        int above = 0, equal = 0;
+        for (int i = 0; i < left; ++i) above += s_few[1][i] > k, equal += s_few[1][i] == k;
+        if (above < want && want <= above + equal) s_pick[0] = int(k), s_pick[1] = above;  // equal keys write alike
+      }
+      __syncthreads();
+      key = uint32_t(s_pick[0]);
+      want -= s_pick[1];
+    }
   }
-  // ---- in slot order: which of the slots at `key` stay, then the lists. Warp w has slots w span .. of this block's.
-  const int w0 = warp * span, w1 = min(mine, w0 + span);
-  auto each = [&](auto f) {
-    for (int i = w0; i < w1; i += 32) f(i + lane, i + lane < w1);
+  // ---- the lists, in slot order: warp w has a stretch of this block's slots, a lane four of them at a step
+  const int span = per / WARPS, w0 = warp * span, w1 = min(mine, w0 + span);
+  auto keys_at = [&](int i) -> uint4 {  // zeros past the end
+    if constexpr (HELD) {
+      uint4 k = *reinterpret_cast<const uint4*>(s_key + i);
+      return k;
+    } else {
+      return make_uint4(i < mine ? make(i) : 0u, i + 1 < mine ? make(i + 1) : 0u, i + 2 < mine ? make(i + 2) : 0u,
+                        i + 3 < mine ? make(i + 3) : 0u);
+    }
   };
-  int ties = 0;
-  each([&](int i, bool in) { ties += __popc(__ballot_sync(0xffffffffu, in && key_at(i) == key)); });
-  int before_blocks, at;
-  const int all_ties = cluster_sum(lane == 0 ? ties : 0, 1, before_blocks);
-  auto warps_before = [&](int v) {  // the sum over the warps before this one
-    if (lane == 0) s_warp[warp] = v;
+  // per warp: its slots at `key`, those of them below the budget, and the holes and movers without them
+  int ties = 0, low = 0, holes = 0, movers = 0;
+  for (int i0 = w0; i0 < w1; i0 += 128) {
+    const uint4 k4 = keys_at(i0 + 4 * lane);
+    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + 4 * lane + e;
+      if (i < w1) {
+        const bool below = s0 + i < keep;
+        ties += k[e] == key, low += below && k[e] == key;
+        holes += below && k[e] < key, movers += !below && k[e] > key;
+      }
+    }
+  }
+  ties = __reduce_add_sync(0xffffffffu, ties), low = __reduce_add_sync(0xffffffffu, low);
+  holes = __reduce_add_sync(0xffffffffu, holes), movers = __reduce_add_sync(0xffffffffu, movers);
+  // what the warps and blocks before this one have of x and y; the whole cluster's in s_all
+  auto before = [&](int use, int x, int y) -> int2 {
+    if (lane == 0) s_warp[1][warp] = x, s_warp[2][warp] = y;
     __syncthreads();
-    const int x = s_warp[lane];
-    const int r = __shfl_sync(0xffffffffu, warp_scan(x) - x, warp);
+    if (warp == 0) {
+      const int xs = lane < WARPS ? s_warp[1][lane] : 0, ys = lane < WARPS ? s_warp[2][lane] : 0;
+      const int xi = warp_scan(xs), yi = warp_scan(ys);
+      if (lane < WARPS) s_warp[1][lane] = xi - xs, s_warp[2][lane] = yi - ys;
+      if (lane == 31) s_mine[use] = make_int4(xi, yi, 0, 0);
+    }
+    sync();
+    if (warp == 0) {
+      const int4 v = lane < blocks ? *cluster.map_shared_rank(&s_mine[use], lane) : make_int4(0, 0, 0, 0);
+      const int4 r = make_int4(__reduce_add_sync(0xffffffffu, v.x), __reduce_add_sync(0xffffffffu, v.y),
+                               __reduce_add_sync(0xffffffffu, lane < rank ? v.x : 0),
+                               __reduce_add_sync(0xffffffffu, lane < rank ? v.y : 0));
+      if (lane == 0) s_all[1] = r;
+    }
     __syncthreads();
+    const int2 r = make_int2(s_warp[1][warp] + s_all[1].z, s_warp[2][warp] + s_all[1].w);
     return r;
   };
-  const int stay_ties = key == KEPT ? all_ties : want;  // of KEPT all, or none are there
-  const int tie0 = before_blocks + warps_before(ties);
-  at = tie0;
-  auto stays_at = [&](int i, bool in) {  // for the slots in order
-    const uint32_t k = in ? key_at(i) : 0u;
-    const unsigned tie = __ballot_sync(0xffffffffu, in && k == key);
-    const int r = at + __popc(tie & ((1u << lane) - 1));
-    at += __popc(tie);
-    return in && (k > key || (k == key && r < stay_ties));
-  };
-  int holes = 0, movers = 0;
-  each([&](int i, bool in) {
-    const bool stays = stays_at(i, in);
-    holes += __popc(__ballot_sync(0xffffffffu, in && !stays && s0 + i < keep));
-    movers += __popc(__ballot_sync(0xffffffffu, stays && s0 + i >= keep));
-  });
-  int hole0, mover0;
-  const int all_movers = cluster_sum(lane == 0 ? movers : 0, 2, mover0);
-  cluster_sum(lane == 0 ? holes : 0, 3, hole0);
-  hole0 += warps_before(holes), mover0 += warps_before(movers);
-  at = tie0;
-  each([&](int i, bool in) {
-    const bool stays = stays_at(i, in);
-    const int s = s0 + i;
-    const bool hole = in && !stays && s < keep, mover = stays && s >= keep;
-    const unsigned h = __ballot_sync(0xffffffffu, hole), m = __ballot_sync(0xffffffffu, mover), below = (1u << lane) - 1;
-    if (hole) A.dst[int64_t(b) * A.cap + hole0 + __popc(h & below)] = s;
-    if (mover) A.src[int64_t(b) * A.cap + mover0 + __popc(m & below)] = s;
-    hole0 += __popc(h), mover0 += __popc(m);
-  });
-  cluster.sync();  // no block leaves while another may read its shared memory; and the lengths are read
+  // of the slots at `key` the lowest `stay` stay; in slot order, so a warp's below the budget before its others
+  int tie = before(1, ties, 0).x;
+  const int stay = key == KEPT ? s_all[1].x : want;
+  const int here = min(max(stay - tie, 0), ties), here_low = min(here, low);
+  __syncthreads();  // s_all has been read
+  const int2 at = before(2, holes + low - here_low, movers + here - here_low);
+  const int all_movers = s_all[1].y;
+  int32_t* dst = A.dst + int64_t(b) * A.cap + at.x;
+  int32_t* src = A.src + int64_t(b) * A.cap + at.y;
+  for (int i0 = w0; i0 < w1; i0 += 128) {
+    const uint4 k4 = keys_at(i0 + 4 * lane);
+    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+    unsigned stays = 0, equal = 0, in = 0, below = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + 4 * lane + e;
+      stays |= unsigned(k[e] > key) << e, equal |= unsigned(k[e] == key) << e;
+      in |= unsigned(i < w1) << e, below |= unsigned(s0 + i < keep) << e;
+    }
+    equal &= in;
+    if (here == ties) {
+      stays |= equal;
+    } else if (here > 0) {  // one warp of the cluster
+      const int c = __popc(equal), inc = warp_scan(c);
+      int r = tie + inc - c;
+      tie += __shfl_sync(0xffffffffu, inc, 31);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((equal >> e) & 1) stays |= unsigned(r++ < stay) << e;
+    }
+    const unsigned h = in & below & ~stays, m = in & ~below & stays;
+    const int c = __popc(h) | __popc(m) << 16, inc = warp_scan(c), ex = inc - c, sum = __shfl_sync(0xffffffffu, inc, 31);
+    int32_t *hp = dst + (ex & 0xffff), *mp = src + (ex >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if ((h >> e) & 1) *hp++ = s0 + i0 + 4 * lane + e;
+      if ((m >> e) & 1) *mp++ = s0 + i0 + 4 * lane + e;
+    }
+    dst += sum & 0xffff, src += sum >> 16;
+  }
+  sync();  // no block leaves while another may read its shared memory; and the lengths are read
   if (rank == 0 && tid == 0) A.count[b] = all_movers, A.lengths_out[b] = keep;
 }
 
@@ -354,7 +420,7 @@ extern "C" int sc_evict(const sc_kv_pages* kv, const int32_t* seen, int keep, in
   const int64_t slots = int64_t(kv->max_pages) * kv->page;
   int cluster = 1;
   while (cluster < ev::MAX_CLUSTER && slots > int64_t(cluster) * ev::PER_BLOCK) cluster *= 2;
-  const int64_t hold = ceil_div(ceil_div(slots, cluster), ev::THREADS) * ev::THREADS;
+  const int64_t hold = ceil_div(ceil_div(slots, cluster), ev::STRETCH) * ev::STRETCH;
   const bool held = hold <= ev::MOST;
   const int smem = held ? int(hold) * 4 : 0;
   const auto plan = held ? ev::plan_kernel<true> : ev::plan_kernel<false>;
