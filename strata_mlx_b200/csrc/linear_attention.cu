@@ -2,11 +2,12 @@
 //   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t
 // as it stands. A block per (sequence, value head, 32 value dimensions) holds its columns of S in registers, a thread
 // 1/8 of a column, and walks the tokens; the eight parts of o_t meet in shared memory.
-#include "common.cuh"
+#include "linear.cuh"
 
 namespace sc {
 namespace la {
 
+constexpr int FEW = 8;  // tokens that the recurrence takes
 constexpr int COLS = 32, PARTS = 8, MAXK = 128, PER = MAXK / PARTS;
 
 template <typename T>
@@ -165,13 +166,22 @@ int launch(const sc_linear& a, void* stream) {
 
 using namespace sc;
 
-extern "C" size_t sc_linear_attention_workspace(const sc_linear* a) { return la::check(a) || a->batch == 0 ? 0 : 16; }
+// Prompts of bfloat16 go to the tensor cores; float16 ones, whose states can pass what float16 terms hold, and a few
+// tokens, which a chunk's products would mostly pad, to the recurrence.
+static bool chunked(const sc_linear& a) { return a.dtype == SC_BF16 && a.tokens > la::FEW; }
+
+extern "C" size_t sc_linear_attention_workspace(const sc_linear* a) {
+  if (la::check(a) || a->batch == 0) return 0;
+  return chunked(*a) ? lc::workspace(*a) : 16;
+}
 
 extern "C" int sc_linear_attention(const sc_linear* a, void* workspace, size_t workspace_bytes, int* err, void* stream) {
   if (int rc = la::check(a)) return rc;
   if (a->batch == 0) return SC_OK;
   if (!workspace) return SC_ERR_ARG;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return SC_ERR_ALIGN;
   if (workspace_bytes < sc_linear_attention_workspace(a)) return SC_ERR_WORKSPACE;
+  if (chunked(*a)) return lc::launch(*a, workspace, err, static_cast<cudaStream_t>(stream));
   return la::launch(*a, stream);
 }
 
