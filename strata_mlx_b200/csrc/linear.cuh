@@ -6,6 +6,7 @@
 
 namespace sc {
 namespace lc {
+bool takes(const sc_linear& a);
 size_t workspace(const sc_linear& a);
 int launch(const sc_linear& a, void* workspace, int* err, cudaStream_t stream);
 }  // namespace lc

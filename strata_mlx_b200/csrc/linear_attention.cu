@@ -166,9 +166,9 @@ int launch(const sc_linear& a, void* stream) {
 
 using namespace sc;
 
-// Prompts of bfloat16 go to the tensor cores; float16 ones, whose states can pass what float16 terms hold, and a few
-// tokens, which a chunk's products would mostly pad, to the recurrence.
-static bool chunked(const sc_linear& a) { return a.dtype == SC_BF16 && a.tokens > la::FEW; }
+// Prompts of bfloat16 go to the tensor cores; float16 ones, whose states can pass what float16 terms hold, broadcast
+// axes, and a few tokens, which a chunk's products would mostly pad, to the recurrence.
+static bool chunked(const sc_linear& a) { return a.tokens > la::FEW && lc::takes(a); }
 
 extern "C" size_t sc_linear_attention_workspace(const sc_linear* a) {
   if (la::check(a) || a->batch == 0) return 0;

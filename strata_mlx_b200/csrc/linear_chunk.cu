@@ -11,10 +11,11 @@
 // The state stays in float32 registers: S = a S + D. A decay a near 1 enters as S + (a - 1) S, as its own rounding
 // would be repeated every chunk.
 //
-// A block per (segment of the tokens, value head, sequence); 17 warps:
-//   0-3    P from A, and the outputs            4-11   the state (a lane a value dimension, half of k_dim each)
-//   12-15  loads (cp.async, three chunks in flight: any strides, zeros past a length), decays, w K
-//   16     one lane issues the products
+// A block per (segment of the tokens, value head, sequence); 19 warps:
+//   0-3    P from A, and the outputs (stored by TMA through a tile of tokens by value dimensions)
+//   4-11   the state (a lane a value dimension, half of k_dim each)
+//   12-15  w K; zeros over the values past a length
+//   16     one lane issues the products      17  the chunks' decays      18  loads by TMA, three chunks in flight
 // Tensor memory: A, I, X, D and the two terms of S^T, 448 of 512 columns.
 //
 // One sequence's heads fill few SMs, so a long prompt is cut into segments: a first launch works out what each
@@ -26,6 +27,7 @@
 #include <type_traits>
 
 #include "linear.cuh"
+#include "tensor_map.cuh"
 #include "tcgen05.cuh"
 
 namespace sc {
@@ -35,10 +37,10 @@ using namespace tc;
 
 constexpr int C = 64;        // tokens of a chunk
 constexpr int STAGES = 3;    // chunks loaded ahead
-constexpr int RING = 4;      // chunks whose decays are held: one more, as outputs are read after a stage is free
+constexpr int RING = 4;      // chunks whose decays are held
 constexpr int HALF = C * 128;  // bytes of 64 columns of a chunk's rows
-constexpr int STATE_WARP = 4, LOAD_WARP = 12, MMA_WARP = 16;
-constexpr int THREADS = (MMA_WARP + 1) * 32;
+constexpr int STATE_WARP = 4, KW_WARP = 12, MMA_WARP = 16, DECAY_WARP = 17, LOAD_WARP = 18;
+constexpr int THREADS = (LOAD_WARP + 1) * 32;
 constexpr int SMS = 148;
 constexpr float LEAST = -30.f;  // a token's decay below e^-30 is taken as e^-30: past it nothing is left in float32
 
@@ -51,7 +53,7 @@ struct Decays {
 };
 
 struct Bars {
-  uint64_t full[STAGES], empty[STAGES];
+  uint64_t full[STAGES], empty[STAGES], dec_full[RING], dec_empty[RING];
   uint64_t a_full, a_empty, p_full, p_empty, o_full, o_empty, kw_full, kw_empty, d_full, d_empty, s_full, s_empty, done;
   uint32_t tmem;
   int bail;
@@ -61,7 +63,7 @@ template <int DK>
 struct Shape {
   static constexpr int K_BYTES = DK / 64 * HALF, V_BYTES = 2 * HALF;
   static constexpr int STAGE = 2 * K_BYTES + V_BYTES;
-  static constexpr int KW = STAGES * STAGE, P = KW + 3 * K_BYTES, DEC = P + HALF, BARS = DEC + RING * int(sizeof(Decays));
+  static constexpr int KW = STAGES * STAGE, P = KW + 3 * K_BYTES, OUT = P + HALF, DEC = OUT + 2 * HALF, BARS = DEC + RING * int(sizeof(Decays));
   static constexpr int BYTES = BARS + int(sizeof(Bars)) + 1024;  // and to align the start
 };
 
@@ -73,10 +75,30 @@ struct Args {
   int* err;
 };
 
-__device__ __forceinline__ void load16(uint32_t dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+struct Maps {  // (dim, heads, tokens, batch), boxes of 64 x 1 x 64 x 1, 128-byte swizzle
+  CUtensorMap q, k, v, out;
+};
+
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int h, int t, int b, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(h), "r"(t), "r"(b), "r"(smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the loading warps
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, const void* src, int x, int h, int t, int b) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(h), "r"(t), "r"(b), "r"(smem_u32(src))
+               : "memory");
+}
+// four 8 x 8 fragments, transposed, to the rows whose addresses the lanes give
+__device__ __forceinline__ void store_transposed(uint32_t at, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r0), "r"(r1), "r"(r2),
+               "r"(r3)
+               : "memory");
+}
+__device__ __forceinline__ void out_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the output warps
 
 __device__ __forceinline__ uint32_t bits_of(__nv_bfloat162 v) { return *reinterpret_cast<uint32_t*>(&v); }
 __device__ __forceinline__ float lo_f(uint32_t v) { return __uint_as_float(v << 16); }
@@ -91,7 +113,8 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t& t0, uint32_t&
 }
 
 template <int DK, bool WHOLE>
-__global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant__ Args A) {
+__global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant__ Args A,
+                                                               const __grid_constant__ Maps maps) {
   using L = Shape<DK>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -105,6 +128,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   const int n = max(0, min(c1, (len + C - 1) / C) - c0);  // this segment's chunks with tokens
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], 4 + 1);
+    for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], WHOLE ? 16 : 12);
     mbar_init(&B.a_full, 1), mbar_init(&B.a_empty, 4), mbar_init(&B.p_full, 4), mbar_init(&B.p_empty, 1);
     mbar_init(&B.o_full, 1), mbar_init(&B.o_empty, 4), mbar_init(&B.kw_full, 4), mbar_init(&B.kw_empty, 1);
     mbar_init(&B.d_full, 1), mbar_init(&B.d_empty, 8), mbar_init(&B.s_full, 8), mbar_init(&B.s_empty, 1);
@@ -117,9 +141,13 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // columns past the dimensions are never loaded: zeros
-  for (int i = tid; i < L::KW / 16; i += THREADS) *reinterpret_cast<uint4*>(smem + 16 * i) = make_uint4(0, 0, 0, 0);
-  fence_async();
+  if (a.v_dim <= 64) {  // the second half of the values is never loaded: zeros
+    for (int i = tid; i < STAGES * HALF / 16; i += THREADS) {
+      uint8_t* half = smem + i / (HALF / 16) * L::STAGE + 2 * L::K_BYTES + HALF;
+      *reinterpret_cast<uint4*>(half + 16 * (i % (HALF / 16))) = make_uint4(0, 0, 0, 0);
+    }
+    fence_async();
+  }
   fence_before();
   __syncthreads();
   fence_after();
@@ -142,7 +170,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       const int g = lane >> 2, t = lane & 3, r0 = 16 * warp + g;
       uint8_t* p = smem + L::P;
       auto make_p = [&](int i) -> bool {
-        if (!wait(&B.a_full, i)) return false;
+        if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.a_full, i)) return false;
         fence_after();
         uint32_t r[32];
         ld_frag64(lanes + COL_A, r);
@@ -171,35 +199,63 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         arrive(&B.p_full);
         return true;
       };
-      const int dv = int(quarter) + lane;
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (int64_t(b) * a.tokens * a.v_heads + h) * a.v_dim + dv;
-      const int64_t row = int64_t(a.v_heads) * a.v_dim;
+      uint8_t* tile = smem + L::OUT;
+      // where this lane's rows of transposed fragments go: token (lane / 16) 8 + lane % 8 of 16, pieces of 8 values
+      const int token = (lane >> 4) * 8 + (lane & 7), piece = 4 * warp + ((lane >> 3) & 1);
       bool ok = n == 0 || make_p(0);
       for (int i = 0; i < n && ok; ++i) {
         if (i + 1 < n && !(ok = make_p(i + 1))) break;
         if (!(ok = wait(&B.o_full, i))) break;
         fence_after();
-        const int t0 = (c0 + i) * C;
+        if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        out_sync();  // the tile's last store has read it
+        const int t0 = (c0 + i) * C, m = len - t0;
         const float* eg = dec[i % RING].eg;
 #pragma unroll
-        for (int q = 0; q < C; q += 16) {
-          uint32_t x[16], y[16];
-          ld16(lanes + COL_X + q, x);
-          ld16(lanes + COL_I + q, y);
+        for (int hf = 0; hf < 2; ++hf) {  // 16 value dimensions at a time
+          uint32_t x[32], y[32];
+          ld_frag64(lanes + (uint32_t(16 * hf) << 16) + COL_X, x);
+          ld_frag64(lanes + (uint32_t(16 * hf) << 16) + COL_I, y);
           wait_ld();
+          if (hf == 1) {
+            fence_before();
+            arrive(&B.o_empty);
+          }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float o = fmaf(eg[q + e], __uint_as_float(x[e]), __uint_as_float(y[e])) * a.scale;
-            if (dv < a.v_dim && t0 + q + e < a.tokens) out[(t0 + q + e) * row] = __float2bfloat16_rn(o);
+          for (int j = 0; j < 8; j += 2) {
+            uint32_t f[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int col = 8 * (j + e) + 2 * t;
+              const float2 s = *reinterpret_cast<const float2*>(eg + col);
+              auto o = [&](int r, float d, bool in) {
+                return in ? fmaf(d, __uint_as_float(x[4 * (j + e) + r]), __uint_as_float(y[4 * (j + e) + r])) * a.scale : 0.f;
+              };
+              f[2 * e] = bits_of(__floats2bfloat162_rn(o(0, s.x, col < m), o(1, s.y, col + 1 < m)));
+              f[2 * e + 1] = bits_of(__floats2bfloat162_rn(o(2, s.x, col < m), o(3, s.y, col + 1 < m)));
+            }
+            const int row = 8 * j + token, pc = piece + 2 * hf;
+            store_transposed(smem_u32(tile) + (pc >> 3) * HALF + row * 128 + (((pc & 7) ^ (row & 7)) << 4), f[0], f[1], f[2], f[3]);
           }
         }
-        fence_before();
-        arrive(&B.o_empty);
+        arrive(&B.dec_empty[i % RING]);
+        fence_async();
+        out_sync();
+        if (tid == 0) {
+          tma_store(&maps.out, tile, 0, h, t0, b);
+          if (a.v_dim > 64) tma_store(&maps.out, tile + HALF, 64, h, t0, b);
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
       }
-      if (dv < a.v_dim)  // zeros past the last chunk with tokens
-        for (int t1 = (c0 + n) * C; t1 < min(a.tokens, c1 * C); ++t1) out[t1 * row] = __float2bfloat16_rn(0.f);
+      // zeros past the last chunk with tokens, 16 bytes at a time
+      const int t1 = (c0 + n) * C, pieces = a.v_dim / 8, rows = max(0, min(a.tokens, c1 * C) - t1);
+      for (int e = tid; e < rows * pieces; e += 128)
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) +
+                                  ((int64_t(b) * a.tokens + t1 + e / pieces) * a.v_heads + h) * a.v_dim + 8 * (e % pieces)) =
+            make_uint4(0, 0, 0, 0);
+      if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
-  } else if (warp < LOAD_WARP) {
+  } else if (warp < KW_WARP) {
     // ---- the state: value dimension `dv`, key dimensions k0 .. k0 + DK / 2 - 1
     constexpr int N = DK / 2;
     const int dv = int(quarter) + lane, k0 = (warp - STATE_WARP) / 4 * N;
@@ -232,7 +288,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     if (WHOLE && n > 0) publish();
     float log = 0.f;
     for (int i = 0; i < n; ++i) {
-      if (!wait(&B.d_full, i)) break;
+      if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.d_full, i)) break;
       fence_after();
       const float d = dec[i % RING].a, one = dec[i % RING].one;
 #pragma unroll
@@ -246,6 +302,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       if (!WHOLE) log += dec[i % RING].g2[C - 1];
       fence_before();
       arrive(&B.d_empty);
+      arrive(&B.dec_empty[i % RING]);
       if (WHOLE && i + 1 < n) {
         if (!wait(&B.s_empty, i)) break;
         fence_after();
@@ -264,77 +321,21 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         if (dv < a.v_dim && k0 + k < a.k_dim) to[int64_t(k0 + k) * a.v_dim] = S[k];
     }
   } else if (warp < MMA_WARP) {
-    // ---- loads, decays, w K
-    const int lt = tid - LOAD_WARP * 32;
-    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + b * a.q_row + hk * a.q_head;
-    const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.k) + b * a.k_row + hk * a.k_head;
-    const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v) + b * a.v_row + h * a.v_head;
-    const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
-    auto issue = [&](int i) {
-      const int t0 = (c0 + i) * C, m = min(C, len - t0);
-      const uint32_t st = smem_u32(smem + (i % STAGES) * L::STAGE);
-      auto rows = [&](uint32_t dst, const __nv_bfloat16* src, int64_t token, int pieces, auto width) {
-        constexpr int W = decltype(width)::value / 8;  // 16-byte pieces of a row
-#pragma unroll 4
-        for (int j = lt; j < C * W; j += 128) {
-          const int r = j / W, p = j % W;
-          const bool in = r < m;
-          if (p < pieces) load16(dst + (p >> 3) * HALF + r * 128 + (((p & 7) ^ (r & 7)) << 4), in ? src + (t0 + r) * token + 8 * p : src, in);
-        }
-      };
-      rows(st + L::K_BYTES, k, a.k_token, a.k_dim / 8, std::integral_constant<int, DK>{});
-      if (WHOLE) rows(st, q, a.q_token, a.k_dim / 8, std::integral_constant<int, DK>{});
-      rows(st + 2 * L::K_BYTES, v, a.v_token, a.v_dim / 8, std::integral_constant<int, 128>{});
-    };
-    auto commit_group = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-    auto decay_of = [&](int i, int e) -> float {
-      const int t = (c0 + i) * C + 2 * lane + e;
-      return i < n && t < len ? fmaxf(decay[int64_t(t) * a.decay_token], LEAST) : 0.f;
-    };
-    float d0 = 0.f, d1 = 0.f;
-    if (warp == LOAD_WARP) d0 = decay_of(0, 0), d1 = decay_of(0, 1);
-    for (int i = 0; i < STAGES - 1; ++i) {
-      if (i < n) issue(i);
-      commit_group();
-    }
+    // ---- w K
+    const int lt = tid - KW_WARP * 32;
     for (int i = 0; i < n; ++i) {
-      Decays& D = dec[i % RING];
-      if (warp == LOAD_WARP) {  // tokens 2 lane and 2 lane + 1: sums from the front, and from the back
-        const float g0 = d0, g1 = d1, pair = g0 + g1;
-        d0 = decay_of(i + 1, 0), d1 = decay_of(i + 1, 1);
-        float up = pair, down = pair;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const float x = __shfl_up_sync(0xffffffffu, up, o), y = __shfl_down_sync(0xffffffffu, down, o);
-          if (lane >= o) up += x;
-          if (lane + o < 32) down += y;
-        }
-        float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
-        if (lane == 0) before = 0.f;
-        if (lane == 31) after = 0.f;
-        constexpr float LOG2E = 1.4426950408889634f;
-        const float e0 = (before + g0) * LOG2E, e1 = up * LOG2E;
-        *reinterpret_cast<float2*>(&D.g2[2 * lane]) = make_float2(e0, e1);
-        *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(exp2f(e0), exp2f(e1));
-        *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(exp2f((after + g1) * LOG2E), exp2f(after * LOG2E));
-        if (lane == 31) {
-          const bool near = up > -0.69314718f;
-          D.a = near ? expm1f(up) : expf(up), D.one = near ? 1.f : 0.f;
-        }
-      }
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-      fence_async();
-      group_sync();
-      const int st = i % STAGES;
-      if (lt == 0) mbar_arrive(&B.full[st]);
-      if (!wait(&B.kw_empty, i + 1)) break;
-      const uint8_t* kr = smem + st * L::STAGE + L::K_BYTES;
+      const int st = i % STAGES, m = len - (c0 + i) * C;
+      if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.full[st], i / STAGES) || !wait(&B.kw_empty, i + 1)) break;
+      uint8_t* stage = smem + st * L::STAGE;
+      const uint8_t* kr = stage + L::K_BYTES;
       uint8_t* kw = smem + L::KW;
-#pragma unroll 2
+      const float* w_of = dec[i % RING].w;
+#pragma unroll 4
       for (int j = lt; j < C * DK / 8; j += 128) {  // 16 bytes of K at a time, the terms to the same places
         const int at = j * 16, r = (at % HALF) / 128;
-        const uint4 x = *reinterpret_cast<const uint4*>(kr + at);
-        const float w = D.w[r];
+        uint4 x = *reinterpret_cast<const uint4*>(kr + at);
+        const float w = w_of[r];
+        if (r >= m) x = make_uint4(0, 0, 0, 0);
         uint4 t0, t1, t2;
         split3(lo_f(x.x) * w, hi_f(x.x) * w, t0.x, t1.x, t2.x);
         split3(lo_f(x.y) * w, hi_f(x.y) * w, t0.y, t1.y, t2.y);
@@ -344,18 +345,73 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         *reinterpret_cast<uint4*>(kw + L::K_BYTES + at) = t1;
         *reinterpret_cast<uint4*>(kw + 2 * L::K_BYTES + at) = t2;
       }
+      if (m < C)  // values past the length meet zeros of P and w K, which a NaN would spoil
+        for (int j = lt; j < 2 * HALF / 16; j += 128)
+          if ((j * 16 % HALF) / 128 >= m) *reinterpret_cast<uint4*>(stage + 2 * L::K_BYTES + 16 * j) = make_uint4(0, 0, 0, 0);
       fence_async();
       arrive(&B.kw_full);
       arrive(&B.empty[st]);  // K has been read
-      // the next chunk's loads, into the stage of the chunk before this one
-      const int ahead = i + STAGES - 1;
-      if (ahead < n) {
-        if (ahead >= STAGES && !wait(&B.empty[ahead % STAGES], ahead / STAGES - 1)) break;
-        issue(ahead);
-      }
-      commit_group();
+      arrive(&B.dec_empty[i % RING]);
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == DECAY_WARP) {
+    // ---- a chunk's decays: a lane tokens 2 lane and 2 lane + 1, sums from the front and from the back
+    const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
+    auto decay_of = [&](int i, int e) -> float {
+      const int t = (c0 + i) * C + 2 * lane + e;
+      return i < n && t < len ? fmaxf(decay[int64_t(t) * a.decay_token], LEAST) : 0.f;
+    };
+    float d0 = decay_of(0, 0), d1 = decay_of(0, 1);
+    for (int i = 0; i < n; ++i) {
+      const float g0 = d0, g1 = d1, pair = g0 + g1;
+      d0 = decay_of(i + 1, 0), d1 = decay_of(i + 1, 1);
+      float up = pair, down = pair;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float x = __shfl_up_sync(0xffffffffu, up, o), y = __shfl_down_sync(0xffffffffu, down, o);
+        if (lane >= o) up += x;
+        if (lane + o < 32) down += y;
+      }
+      float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
+      if (lane == 0) before = 0.f;
+      if (lane == 31) after = 0.f;
+      constexpr float LOG2E = 1.4426950408889634f;
+      const float e0 = (before + g0) * LOG2E, e1 = up * LOG2E;
+      Decays& D = dec[i % RING];
+      if (!wait(&B.dec_empty[i % RING], i / RING + 1)) break;
+      *reinterpret_cast<float2*>(&D.g2[2 * lane]) = make_float2(e0, e1);
+      *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(exp2f(e0), exp2f(e1));
+      *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(exp2f((after + g1) * LOG2E), exp2f(after * LOG2E));
+      if (lane == 31) {
+        const bool near = up > -0.69314718f;
+        D.a = near ? expm1f(up) : expf(up), D.one = near ? 1.f : 0.f;
+      }
+      arrive(&B.dec_full[i % RING]);
+    }
+  } else if (warp == LOAD_WARP) {
+    // ---- loads
+    const bool leader = elect_one();
+    const uint32_t bytes = uint32_t((WHOLE ? 2 : 1) * L::K_BYTES + (a.v_dim > 64 ? 2 : 1) * HALF);
+    int issued = 0;
+    for (int i = 0; i < n; ++i) {
+      const int st = i % STAGES, t0 = (c0 + i) * C;
+      if (!wait(&B.empty[st], i / STAGES + 1)) break;
+      if (leader) {
+        uint8_t* stage = smem + st * L::STAGE;
+        mbar_arrive_expect_tx(&B.full[st], bytes);
+#pragma unroll
+        for (int x = 0; x < DK; x += 64) {
+          if (WHOLE) tma_load(stage + x / 64 * HALF, &maps.q, x, hk, t0, b, &B.full[st]);
+          tma_load(stage + L::K_BYTES + x / 64 * HALF, &maps.k, x, hk, t0, b, &B.full[st]);
+        }
+        tma_load(stage + 2 * L::K_BYTES, &maps.v, 0, h, t0, b, &B.full[st]);
+        if (a.v_dim > 64) tma_load(stage + 2 * L::K_BYTES + HALF, &maps.v, 64, h, t0, b, &B.full[st]);
+      }
+      __syncwarp();
+      issued = i + 1;
+    }
+    // copies in flight land before the block may end
+    for (int i = max(0, issued - STAGES); i < issued; ++i)
+      mbar_wait_sleep(&B.full[i % STAGES], uint32_t(i / STAGES) & 1, nullptr, 20000000LL);
   } else {
     // ---- the products
     const bool leader = elect_one();
@@ -379,6 +435,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       const int st = i % STAGES;
       const uint8_t* stage = smem + st * L::STAGE;
       const uint64_t vt = desc_mn(stage + 2 * L::K_BYTES, HALF);
+      if (WHOLE && i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
+        if (!(ok = wait(&B.full[(i + 1) % STAGES], (i + 1) / STAGES))) break;
+        if (!(ok = wait(&B.a_empty, i))) break;
+        fence_after();
+        a_product(i + 1);
+      }
       if (!(ok = wait(&B.full[st], i / STAGES))) break;
       if (!(ok = wait(&B.kw_full, i))) break;
       if (!(ok = wait(&B.d_empty, i + 1))) break;
@@ -409,12 +471,6 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
           commit(&B.s_empty);
         }
         __syncwarp();
-        if (i + 1 < n) {
-          if (!(ok = wait(&B.full[(i + 1) % STAGES], (i + 1) / STAGES))) break;
-          if (!(ok = wait(&B.a_empty, i))) break;
-          fence_after();
-          a_product(i + 1);
-        }
         if (!(ok = wait(&B.p_full, i))) break;
         fence_after();
         if (leader) {
@@ -479,9 +535,31 @@ inline size_t parts_bytes(const sc_linear& a, int segments) {
 
 size_t workspace(const sc_linear& a) { return parts_bytes(a, segments_of(a)) + 16; }
 
+// a tensor of (batch, tokens, heads, dim) as a map; the strides of axes of one entry are not looked at
+inline int map_of(CUtensorMap* m, const void* p, int dim, int heads, int tokens, int batch, int64_t head, int64_t token, int64_t row) {
+  const cuuint64_t dims[4] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(tokens), cuuint64_t(batch)};
+  const cuuint64_t any = cuuint64_t(dim) * 2;
+  const cuuint64_t strides[3] = {heads > 1 ? cuuint64_t(head) * 2 : any, tokens > 1 ? cuuint64_t(token) * 2 : any,
+                                 batch > 1 ? cuuint64_t(row) * 2 : any};
+  const cuuint32_t box[4] = {64, 1, C, 1}, each[4] = {1, 1, 1, 1};
+  const EncodeTiled encode = encode_tiled();
+  return encode && encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, box, each,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? SC_OK
+             : SC_ERR_CUDA;
+}
+
 template <int DK>
 int run(const Args& A, cudaStream_t s) {
   const sc_linear& a = A.a;
+  Maps maps;
+  const int64_t token = int64_t(a.v_heads) * a.v_dim;
+  if (map_of(&maps.q, a.q, a.k_dim, a.k_heads, a.tokens, a.batch, a.q_head, a.q_token, a.q_row) ||
+      map_of(&maps.k, a.k, a.k_dim, a.k_heads, a.tokens, a.batch, a.k_head, a.k_token, a.k_row) ||
+      map_of(&maps.v, a.v, a.v_dim, a.v_heads, a.tokens, a.batch, a.v_head, a.v_token, a.v_row) ||
+      map_of(&maps.out, a.out, a.v_dim, a.v_heads, a.tokens, a.batch, a.v_dim, token, token * a.tokens))
+    return cuda_failed(cudaErrorInvalidValue, "linear attention tensor map");
   const dim3 grid(unsigned(A.segments), unsigned(a.v_heads), unsigned(a.batch));
   constexpr int smem = Shape<DK>::BYTES;
   static_assert(smem <= 227 * 1024, "shared memory of a block");
@@ -490,12 +568,20 @@ int run(const Args& A, cudaStream_t s) {
   if (A.segments > 1) {
     if (int rc = raise_smem(reinterpret_cast<const void*>(chunk_kernel<DK, false>), smem, "linear attention smem attribute"))
       return rc;
-    chunk_kernel<DK, false><<<dim3(grid.x - 1, grid.y, grid.z), THREADS, smem, s>>>(A);
+    chunk_kernel<DK, false><<<dim3(grid.x - 1, grid.y, grid.z), THREADS, smem, s>>>(A, maps);
     scan_kernel<DK><<<dim3(unsigned(a.batch) * unsigned(a.v_heads), DK * 128 / 256), 256, 0, s>>>(A);
   }
-  chunk_kernel<DK, true><<<grid, THREADS, smem, s>>>(A);
+  chunk_kernel<DK, true><<<grid, THREADS, smem, s>>>(A, maps);
   if (cudaError_t e = cudaGetLastError()) return cuda_failed(e, "linear attention launch");
   return SC_OK;
+}
+
+// a map takes no stride of zero (a broadcast axis) and none past 2^40 bytes
+bool takes(const sc_linear& a) {
+  auto fits = [&](int n, int64_t stride) { return n < 2 || (stride > 0 && stride < (int64_t(1) << 38)); };
+  return a.dtype == SC_BF16 && a.tokens > 0 && fits(a.k_heads, a.q_head) && fits(a.k_heads, a.k_head) &&
+         fits(a.v_heads, a.v_head) && fits(a.tokens, a.q_token) && fits(a.tokens, a.k_token) && fits(a.tokens, a.v_token) &&
+         fits(a.batch, a.q_row) && fits(a.batch, a.k_row) && fits(a.batch, a.v_row);
 }
 
 int launch(const sc_linear& a, void* ws, int* err, cudaStream_t s) {

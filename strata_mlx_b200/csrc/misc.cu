@@ -5,7 +5,7 @@
 #include <mutex>
 #include <utility>
 
-#include "common.cuh"
+#include "tensor_map.cuh"
 
 namespace sc {
 int cuda_failed(cudaError_t e, const char* where) {
@@ -30,6 +30,19 @@ int raise_smem(const void* kern, int bytes, const char* where) {
     return cuda_failed(e, where);
   now = bytes;
   return SC_OK;
+}
+
+EncodeTiled encode_tiled() {
+  static EncodeTiled fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(p);
+  });
+  return fn;
 }
 }  // namespace sc
 

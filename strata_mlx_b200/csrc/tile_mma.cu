@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "decode.cuh"
+#include "tensor_map.cuh"
 #include "tiles.cuh"
 
 namespace sc {
@@ -663,24 +664,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 #ifdef SC_TRACE
   if (tid == 0) asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(g_tt[15][blockIdx.x % 1024]));
 #endif
-}
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no link-time dependence on its version)
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiled encode_tiled() {
-  static EncodeTiled fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiled>(p);
-  });
-  return fn;
 }
 
 static int sm_count() {
