@@ -11,11 +11,11 @@
 // The state stays in float32 registers: S = a S + D. A decay a near 1 enters as S + (a - 1) S, as its own rounding
 // would be repeated every chunk.
 //
-// A block per (segment of the tokens, value head, sequence); 19 warps:
-//   0-3    P from A, and the outputs (stored by TMA through a tile of tokens by value dimensions)
-//   4-11   the state (a lane a value dimension, half of k_dim each)
-//   12-15  w K; zeros over the values past a length
-//   16     one lane issues the products      17  the chunks' decays      18  loads by TMA, three chunks in flight
+// A block per (segment of the tokens, value head, sequence); 24 warps in six groups, each with its share of registers:
+//   0-3    P from A                             4-7    the outputs, stored by TMA through a tile in shared memory
+//   8-15   the state (a lane a value dimension, half of k_dim each)
+//   16-19  w K, in halves of 32 tokens so that D's products run behind it; zeros over the values past a length
+//   20     one lane issues the products      21  the chunks' decays      22  loads by TMA, three chunks in flight
 // Tensor memory: A, I, X, D and the two terms of S^T, 448 of 512 columns.
 //
 // One sequence's heads fill few SMs, so a long prompt is cut into segments: a first launch works out what each
@@ -39,8 +39,11 @@ constexpr int C = 64;        // tokens of a chunk
 constexpr int STAGES = 3;    // chunks loaded ahead
 constexpr int RING = 4;      // chunks whose decays are held
 constexpr int HALF = C * 128;  // bytes of 64 columns of a chunk's rows
-constexpr int STATE_WARP = 4, KW_WARP = 12, MMA_WARP = 16, DECAY_WARP = 17, LOAD_WARP = 18;
-constexpr int THREADS = (LOAD_WARP + 1) * 32;
+constexpr int OUT_WARP = 4, STATE_WARP = 8, KW_WARP = 16, MMA_WARP = 20, DECAY_WARP = 21, LOAD_WARP = 22;
+constexpr int THREADS = 24 * 32;
+// registers a thread: 80 at launch; the groups' shares add up to as many
+constexpr int P_REGS = 72, OUT_REGS = 72, STATE_REGS = 112, KW_REGS = 72, CONTROL_REGS = 40;
+static_assert(P_REGS + OUT_REGS + 2 * STATE_REGS + KW_REGS + CONTROL_REGS == 6 * 80, "a block's registers");
 constexpr int SMS = 148;
 constexpr float LEAST = -30.f;  // a token's decay below e^-30 is taken as e^-30: past it nothing is left in float32
 
@@ -48,13 +51,14 @@ constexpr float LEAST = -30.f;  // a token's decay below e^-30 is taken as e^-30
 constexpr uint32_t COL_A = 0, COL_I = 64, COL_X = 128, COL_D = 192, COL_S = 320;
 
 struct Decays {
-  float g2[C], eg[C], w[C];  // G_i log2(e), e^{G_i}, e^{G_63 - G_i}
+  float g2[C], eg[C], w[C];  // G_i log2(e), scale e^{G_i}, e^{G_63 - G_i}
   float a, one;              // the chunk's decay as S' = a S + one S + D
 };
 
 struct Bars {
   uint64_t full[STAGES], empty[STAGES], dec_full[RING], dec_empty[RING];
-  uint64_t a_full, a_empty, p_full, p_empty, o_full, o_empty, kw_full, kw_empty, d_full, d_empty, s_full, s_empty, done;
+  uint64_t a_full, a_empty, p_full, p_empty, o_full, o_empty, kw_full[2], kw_empty[2], d_full, d_empty, s_full, s_empty,
+      done;
   uint32_t tmem;
   int bail;
 };
@@ -104,6 +108,15 @@ __device__ __forceinline__ uint32_t bits_of(__nv_bfloat162 v) { return *reinterp
 __device__ __forceinline__ float lo_f(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_f(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// 2^x to 2^-22 of it, as P is rounded to eight bits
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // the three bfloat16 terms of two float32 values
 __device__ __forceinline__ void split3(float x, float y, uint32_t& t0, uint32_t& t1, uint32_t& t2) {
   t0 = bits_of(__floats2bfloat162_rn(x, y));
@@ -116,6 +129,7 @@ template <int DK, bool WHOLE>
 __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant__ Args A,
                                                                const __grid_constant__ Maps maps) {
   using L = Shape<DK>;
+  constexpr int KW_GROUPS = WHOLE ? 1 : 3;  // without outputs, those warps make w K too
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   Decays* dec = reinterpret_cast<Decays*>(smem + L::DEC);
@@ -127,10 +141,11 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   const int c0 = seg * A.per, all = (a.tokens + C - 1) / C, c1 = min(all, c0 + A.per);
   const int n = max(0, min(c1, (len + C - 1) / C) - c0);  // this segment's chunks with tokens
   if (tid == 0) {
-    for (int i = 0; i < STAGES; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], 4 + 1);
-    for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], WHOLE ? 16 : 12);
+    for (int i = 0; i < STAGES; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], KW_GROUPS * 4 + 1);
+    for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], 20);
     mbar_init(&B.a_full, 1), mbar_init(&B.a_empty, 4), mbar_init(&B.p_full, 4), mbar_init(&B.p_empty, 1);
-    mbar_init(&B.o_full, 1), mbar_init(&B.o_empty, 4), mbar_init(&B.kw_full, 4), mbar_init(&B.kw_empty, 1);
+    mbar_init(&B.o_full, 1), mbar_init(&B.o_empty, 4);
+    for (int i = 0; i < 2; ++i) mbar_init(&B.kw_full[i], KW_GROUPS * 4), mbar_init(&B.kw_empty[i], 1);
     mbar_init(&B.d_full, 1), mbar_init(&B.d_empty, 8), mbar_init(&B.s_full, 8), mbar_init(&B.s_empty, 1);
     mbar_init(&B.done, 1);
     B.bail = 0;
@@ -164,32 +179,84 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   };
   const uint32_t quarter = uint32_t(warp & 3) * 32, lanes = tmem + (quarter << 16);
 
+  auto make_kw = [&](int lt) {  // `lt` of 128 KW_GROUPS threads
+    for (int i = 0; i < n; ++i) {
+      const int st = i % STAGES, m = len - (c0 + i) * C;
+      if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.full[st], i / STAGES)) break;
+      uint8_t* stage = smem + st * L::STAGE;
+      const uint8_t* kr = stage + L::K_BYTES;
+      uint8_t* kw = smem + L::KW;
+      const float* w_of = dec[i % RING].w;
+      bool ok = true;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        if (!(ok = wait(&B.kw_empty[hf], i + 1))) break;
+#pragma unroll 4
+        for (int j = lt; j < C / 2 * DK / 8; j += 128 * KW_GROUPS) {  // 16 bytes of K, the terms to the same place
+          const int r = C / 2 * hf + j / 8 % (C / 2), at = j / (C / 2 * 8) * HALF + r * 128 + j % 8 * 16;
+          uint4 x = *reinterpret_cast<const uint4*>(kr + at);
+          const float w = w_of[r];
+          if (r >= m) x = make_uint4(0, 0, 0, 0);
+          uint4 t0, t1, t2;
+          split3(lo_f(x.x) * w, hi_f(x.x) * w, t0.x, t1.x, t2.x);
+          split3(lo_f(x.y) * w, hi_f(x.y) * w, t0.y, t1.y, t2.y);
+          split3(lo_f(x.z) * w, hi_f(x.z) * w, t0.z, t1.z, t2.z);
+          split3(lo_f(x.w) * w, hi_f(x.w) * w, t0.w, t1.w, t2.w);
+          *reinterpret_cast<uint4*>(kw + at) = t0;
+          *reinterpret_cast<uint4*>(kw + L::K_BYTES + at) = t1;
+          *reinterpret_cast<uint4*>(kw + 2 * L::K_BYTES + at) = t2;
+        }
+        if (hf == 0 && m < C)  // values past the length meet zeros of P and w K, which a NaN would spoil
+          for (int j = lt; j < 2 * HALF / 16; j += 128 * KW_GROUPS)
+            if ((j * 16 % HALF) / 128 >= m) *reinterpret_cast<uint4*>(stage + 2 * L::K_BYTES + 16 * j) = make_uint4(0, 0, 0, 0);
+        fence_async();
+        arrive(&B.kw_full[hf]);
+      }
+      if (!ok) break;
+      arrive(&B.empty[st]);  // K has been read
+      arrive(&B.dec_empty[i % RING]);
+    }
+  };
+
   if (warp < STATE_WARP) {
-    if constexpr (WHOLE) {
-      // ---- P of the next chunk, then the outputs of this one
+    if constexpr (!WHOLE) {
+      fewer_registers<KW_REGS>();
+      make_kw(tid);
+    } else if (warp < OUT_WARP) {
+      // ---- P
+      fewer_registers<P_REGS>();
       const int g = lane >> 2, t = lane & 3, r0 = 16 * warp + g;
       uint8_t* p = smem + L::P;
-      auto make_p = [&](int i) -> bool {
-        if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.a_full, i)) return false;
+      // the scale goes with the decays: 2^(G_i + log2 |scale| - G_j), its sign last
+      const float shift = log2f(fabsf(a.scale));
+      const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+      for (int i = 0; i < n; ++i) {
+        if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.a_full, i)) break;
         fence_after();
         uint32_t r[32];
         ld_frag64(lanes + COL_A, r);
+        const float* g2 = dec[i % RING].g2;
+        const float ga = g2[r0] + shift, gb = g2[r0 + 8] + shift;
         wait_ld();
         fence_before();
         arrive(&B.a_empty);
-        const float* g2 = dec[i % RING].g2;
-        const float ga = g2[r0], gb = g2[r0 + 8];
         uint32_t pk[16];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+          pk[2 * j] = pk[2 * j + 1] = 0;
+          if (8 * j > 16 * warp + 15) continue;  // above the diagonal
           const float2 gj = *reinterpret_cast<const float2*>(g2 + 8 * j + 2 * t);
           const int col = 8 * j + 2 * t;
-          auto term = [&](uint32_t x, float gi, float gk, bool in) { return in ? __uint_as_float(x) * exp2f(gi - gk) : 0.f; };
-          pk[2 * j] = bits_of(__floats2bfloat162_rn(term(r[4 * j], ga, gj.x, col <= r0), term(r[4 * j + 1], ga, gj.y, col + 1 <= r0)));
-          pk[2 * j + 1] = bits_of(__floats2bfloat162_rn(term(r[4 * j + 2], gb, gj.x, col <= r0 + 8),
-                                                        term(r[4 * j + 3], gb, gj.y, col + 1 <= r0 + 8)));
+          float x0 = __uint_as_float(r[4 * j]) * fast_exp2(ga - gj.x), x1 = __uint_as_float(r[4 * j + 1]) * fast_exp2(ga - gj.y);
+          float y0 = __uint_as_float(r[4 * j + 2]) * fast_exp2(gb - gj.x), y1 = __uint_as_float(r[4 * j + 3]) * fast_exp2(gb - gj.y);
+          if (8 * j + 7 > 16 * warp) {  // on it
+            x0 = col <= r0 ? x0 : 0.f, x1 = col + 1 <= r0 ? x1 : 0.f;
+            y0 = col <= r0 + 8 ? y0 : 0.f, y1 = col + 1 <= r0 + 8 ? y1 : 0.f;
+          }
+          pk[2 * j] = bits_of(__floats2bfloat162_rn(x0, x1)) ^ sign, pk[2 * j + 1] = bits_of(__floats2bfloat162_rn(y0, y1)) ^ sign;
         }
-        if (!wait(&B.p_empty, i + 1)) return false;
+        arrive(&B.dec_empty[i % RING]);
+        if (!wait(&B.p_empty, i + 1)) break;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {  // r0 and r0 + 8 have one place in the swizzle
           *reinterpret_cast<uint32_t*>(p + r0 * 128 + ((j ^ g) << 4) + 4 * t) = pk[2 * j];
@@ -197,51 +264,57 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         }
         fence_async();
         arrive(&B.p_full);
-        return true;
-      };
+      }
+    } else {
+      // ---- the outputs
+      fewer_registers<OUT_REGS>();
+      const int t = lane & 3, ot = tid - OUT_WARP * 32;
       uint8_t* tile = smem + L::OUT;
       // where this lane's rows of transposed fragments go: token (lane / 16) 8 + lane % 8 of 16, pieces of 8 values
-      const int token = (lane >> 4) * 8 + (lane & 7), piece = 4 * warp + ((lane >> 3) & 1);
-      bool ok = n == 0 || make_p(0);
-      for (int i = 0; i < n && ok; ++i) {
-        if (i + 1 < n && !(ok = make_p(i + 1))) break;
-        if (!(ok = wait(&B.o_full, i))) break;
+      const int token = (lane >> 4) * 8 + (lane & 7), piece = 4 * (warp & 3) + ((lane >> 3) & 1);
+      for (int i = 0; i < n; ++i) {
+        if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.o_full, i)) break;
         fence_after();
-        if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        if (ot == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         out_sync();  // the tile's last store has read it
         const int t0 = (c0 + i) * C, m = len - t0;
         const float* eg = dec[i % RING].eg;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {  // 16 value dimensions at a time
-          uint32_t x[32], y[32];
-          ld_frag64(lanes + (uint32_t(16 * hf) << 16) + COL_X, x);
-          ld_frag64(lanes + (uint32_t(16 * hf) << 16) + COL_I, y);
+        for (int q = 0; q < 4; ++q) {  // 16 value dimensions by 32 tokens at a time
+          const int hf = q >> 1, j0 = 4 * (q & 1);
+          uint32_t x[16], y[16];
+          ld_frag32(lanes + (uint32_t(16 * hf) << 16) + COL_X + 8 * j0, x);
+          ld_frag32(lanes + (uint32_t(16 * hf) << 16) + COL_I + 8 * j0, y);
           wait_ld();
-          if (hf == 1) {
+          if (q == 3) {
             fence_before();
             arrive(&B.o_empty);
           }
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
+          for (int j = 0; j < 4; j += 2) {
             uint32_t f[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int col = 8 * (j + e) + 2 * t;
+              const int k = 4 * (j + e), col = 8 * (j0 + j + e) + 2 * t;
               const float2 s = *reinterpret_cast<const float2*>(eg + col);
-              auto o = [&](int r, float d, bool in) {
-                return in ? fmaf(d, __uint_as_float(x[4 * (j + e) + r]), __uint_as_float(y[4 * (j + e) + r])) * a.scale : 0.f;
-              };
-              f[2 * e] = bits_of(__floats2bfloat162_rn(o(0, s.x, col < m), o(1, s.y, col + 1 < m)));
-              f[2 * e + 1] = bits_of(__floats2bfloat162_rn(o(2, s.x, col < m), o(3, s.y, col + 1 < m)));
+              float o[4];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[r] = fmaf(r & 1 ? s.y : s.x, __uint_as_float(x[k + r]), __uint_as_float(y[k + r]));
+              if (m < C) {  // zeros past the length
+                if (col >= m) o[0] = o[2] = 0.f;
+                if (col + 1 >= m) o[1] = o[3] = 0.f;
+              }
+              f[2 * e] = bits_of(__floats2bfloat162_rn(o[0], o[1]));
+              f[2 * e + 1] = bits_of(__floats2bfloat162_rn(o[2], o[3]));
             }
-            const int row = 8 * j + token, pc = piece + 2 * hf;
+            const int row = 8 * (j0 + j) + token, pc = piece + 2 * hf;
             store_transposed(smem_u32(tile) + (pc >> 3) * HALF + row * 128 + (((pc & 7) ^ (row & 7)) << 4), f[0], f[1], f[2], f[3]);
           }
         }
         arrive(&B.dec_empty[i % RING]);
         fence_async();
         out_sync();
-        if (tid == 0) {
+        if (ot == 0) {
           tma_store(&maps.out, tile, 0, h, t0, b);
           if (a.v_dim > 64) tma_store(&maps.out, tile + HALF, 64, h, t0, b);
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -249,15 +322,16 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       }
       // zeros past the last chunk with tokens, 16 bytes at a time
       const int t1 = (c0 + n) * C, pieces = a.v_dim / 8, rows = max(0, min(a.tokens, c1 * C) - t1);
-      for (int e = tid; e < rows * pieces; e += 128)
+      for (int e = ot; e < rows * pieces; e += 128)
         *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) +
                                   ((int64_t(b) * a.tokens + t1 + e / pieces) * a.v_heads + h) * a.v_dim + 8 * (e % pieces)) =
             make_uint4(0, 0, 0, 0);
-      if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      if (ot == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   } else if (warp < KW_WARP) {
     // ---- the state: value dimension `dv`, key dimensions k0 .. k0 + DK / 2 - 1
     constexpr int N = DK / 2;
+    more_registers<STATE_REGS>();
     const int dv = int(quarter) + lane, k0 = (warp - STATE_WARP) / 4 * N;
     float S[N];
     const int64_t head = int64_t(b) * a.v_heads + h;
@@ -322,38 +396,11 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     }
   } else if (warp < MMA_WARP) {
     // ---- w K
-    const int lt = tid - KW_WARP * 32;
-    for (int i = 0; i < n; ++i) {
-      const int st = i % STAGES, m = len - (c0 + i) * C;
-      if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.full[st], i / STAGES) || !wait(&B.kw_empty, i + 1)) break;
-      uint8_t* stage = smem + st * L::STAGE;
-      const uint8_t* kr = stage + L::K_BYTES;
-      uint8_t* kw = smem + L::KW;
-      const float* w_of = dec[i % RING].w;
-#pragma unroll 4
-      for (int j = lt; j < C * DK / 8; j += 128) {  // 16 bytes of K at a time, the terms to the same places
-        const int at = j * 16, r = (at % HALF) / 128;
-        uint4 x = *reinterpret_cast<const uint4*>(kr + at);
-        const float w = w_of[r];
-        if (r >= m) x = make_uint4(0, 0, 0, 0);
-        uint4 t0, t1, t2;
-        split3(lo_f(x.x) * w, hi_f(x.x) * w, t0.x, t1.x, t2.x);
-        split3(lo_f(x.y) * w, hi_f(x.y) * w, t0.y, t1.y, t2.y);
-        split3(lo_f(x.z) * w, hi_f(x.z) * w, t0.z, t1.z, t2.z);
-        split3(lo_f(x.w) * w, hi_f(x.w) * w, t0.w, t1.w, t2.w);
-        *reinterpret_cast<uint4*>(kw + at) = t0;
-        *reinterpret_cast<uint4*>(kw + L::K_BYTES + at) = t1;
-        *reinterpret_cast<uint4*>(kw + 2 * L::K_BYTES + at) = t2;
-      }
-      if (m < C)  // values past the length meet zeros of P and w K, which a NaN would spoil
-        for (int j = lt; j < 2 * HALF / 16; j += 128)
-          if ((j * 16 % HALF) / 128 >= m) *reinterpret_cast<uint4*>(stage + 2 * L::K_BYTES + 16 * j) = make_uint4(0, 0, 0, 0);
-      fence_async();
-      arrive(&B.kw_full);
-      arrive(&B.empty[st]);  // K has been read
-      arrive(&B.dec_empty[i % RING]);
-    }
-  } else if (warp == DECAY_WARP) {
+    fewer_registers<KW_REGS>();
+    make_kw(WHOLE ? tid - KW_WARP * 32 : 256 + tid - KW_WARP * 32);
+  } else {
+  fewer_registers<CONTROL_REGS>();
+  if (warp == DECAY_WARP) {
     // ---- a chunk's decays: a lane tokens 2 lane and 2 lane + 1, sums from the front and from the back
     const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
     auto decay_of = [&](int i, int e) -> float {
@@ -379,7 +426,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       Decays& D = dec[i % RING];
       if (!wait(&B.dec_empty[i % RING], i / RING + 1)) break;
       *reinterpret_cast<float2*>(&D.g2[2 * lane]) = make_float2(e0, e1);
-      *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(exp2f(e0), exp2f(e1));
+      *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(exp2f(e0) * a.scale, exp2f(e1) * a.scale);
       *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(exp2f((after + g1) * LOG2E), exp2f(after * LOG2E));
       if (lane == 31) {
         const bool near = up > -0.69314718f;
@@ -412,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     // copies in flight land before the block may end
     for (int i = max(0, issued - STAGES); i < issued; ++i)
       mbar_wait_sleep(&B.full[i % STAGES], uint32_t(i / STAGES) & 1, nullptr, 20000000LL);
-  } else {
+  } else if (warp == MMA_WARP) {
     // ---- the products
     const bool leader = elect_one();
     auto k_major = [&](const uint8_t* p, int s) { return desc_k(p + (s / 4) * HALF) + 2 * (s % 4); };
@@ -442,18 +489,25 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         a_product(i + 1);
       }
       if (!(ok = wait(&B.full[st], i / STAGES))) break;
-      if (!(ok = wait(&B.kw_full, i))) break;
       if (!(ok = wait(&B.d_empty, i + 1))) break;
-      fence_after();
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        if (!(ok = wait(&B.kw_full[hf], i))) break;
+        fence_after();
+        if (leader) {
+#pragma unroll
+          for (int term = 2; term >= 0; --term)  // the small ones first
+#pragma unroll
+            for (int s = 2 * hf; s < 2 * hf + 2; ++s)
+              mma_ss(tmem + COL_D, vt + 128 * s, desc_mn(smem + L::KW + term * L::K_BYTES, HALF) + 128 * s,
+                     idesc_bf16(128, DK, true, true), hf > 0 || term < 2 || s > 0);
+          commit(&B.kw_empty[hf]);
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
       if (leader) {
-#pragma unroll
-        for (int term = 2; term >= 0; --term)  // the small ones first
-#pragma unroll
-          for (int s = 0; s < C / 16; ++s)
-            mma_ss(tmem + COL_D, vt + 128 * s, desc_mn(smem + L::KW + term * L::K_BYTES, HALF) + 128 * s,
-                   idesc_bf16(128, DK, true, true), term < 2 || s > 0);
         commit(&B.d_full);
-        commit(&B.kw_empty);
         if (!WHOLE) commit(&B.empty[st]);
       }
       __syncwarp();
@@ -490,6 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     }
     __syncwarp();
   }
+  }
   fence_before();
   __syncthreads();
   fence_after();
@@ -504,25 +559,33 @@ __global__ void __launch_bounds__(256) scan_kernel(const Args A) {
   const int e = blockIdx.y * 256 + threadIdx.x, k = e / 128, dv = e % 128;
   float* part = A.parts + head * A.segments * DK * 128 + e;
   float S = a.state_in && k < a.k_dim && dv < a.v_dim ? a.state_in[(head * a.k_dim + k) * a.v_dim + dv] : 0.f;
-#pragma unroll 4
-  for (int s = 0; s + 1 < A.segments; ++s) {
-    const float log = A.logs[head * A.segments + s], add = part[int64_t(s) * DK * 128];
-    part[int64_t(s) * DK * 128] = S;
-    S = log > -0.69314718f ? fmaf(expm1f(log), S, S + add) : fmaf(expf(log), S, add);
+  const int last = A.segments - 1;
+  for (int s0 = 0; s0 < last; s0 += 8) {
+    float log[8], add[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (s0 + i < last) log[i] = A.logs[head * A.segments + s0 + i], add[i] = part[int64_t(s0 + i) * DK * 128];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (s0 + i < last) {
+        part[int64_t(s0 + i) * DK * 128] = S;
+        S = log[i] > -0.69314718f ? fmaf(expm1f(log[i]), S, S + add[i]) : fmaf(expf(log[i]), S, add[i]);
+      }
   }
-  part[int64_t(A.segments - 1) * DK * 128] = S;
+  part[int64_t(last) * DK * 128] = S;
 }
 
-// The segments that cost least: waves of blocks times a segment's chunks, those of the first launch (about two fifths
-// of the whole's work each) added, and 10 chunks' time for the two more launches.
+// The segments that cost least, in chunks' time of an SM: waves of blocks times a segment's chunks (and about three
+// to start and end a block), the first launch's at three fifths, and the scan over the segments' states.
 inline int segments_of(const sc_linear& a) {
   const int64_t heads = int64_t(a.batch) * a.v_heads;
   const int chunks = int(ceil_div(a.tokens, C));
   int best = 1;
   double least = 1e30;
-  for (int s = 1; s <= std::min(chunks / 4, SMS) || s == 1; ++s) {
-    const double per = double(ceil_div(chunks, s)), waves = double(ceil_div(heads * s, SMS));
-    const double cost = waves * per + (s > 1 ? 0.4 * double(ceil_div(heads * (s - 1), SMS)) * per + 10 : 0);
+  for (int s = 1; s <= std::max(1, std::min(chunks / 4, SMS)); ++s) {
+    const double per = double(ceil_div(chunks, s)) + 3;
+    double cost = double(ceil_div(heads * s, SMS)) * per;
+    if (s > 1) cost += 0.6 * double(ceil_div(heads * (s - 1), SMS)) * per + 2 + 0.02 * double(heads * s);
     if (cost < least) least = cost, best = s;
   }
   return best;

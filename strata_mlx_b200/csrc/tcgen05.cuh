@@ -95,6 +95,14 @@ __device__ __forceinline__ void ld_frag64(uint32_t addr, uint32_t (&r)[32]) {
       : SC_R8(r, 0), SC_R8(r, 8), SC_R8(r, 16), SC_R8(r, 24)
       : "r"(addr));
 }
+// the same, 32 columns
+__device__ __forceinline__ void ld_frag32(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : SC_R8(r, 0), SC_R8(r, 8)
+      : "r"(addr));
+}
 __device__ __forceinline__ void st8(uint32_t addr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), SC_W8(r, 0)
                : "memory");
