@@ -168,10 +168,29 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   fence_after();
   const uint32_t tmem = B.tmem;
   volatile int* bail = &B.bail;
-  auto wait = [&](uint64_t* bar, int phase) -> bool {  // for the whole warp
-    const bool ok = __all_sync(0xffffffffu, mbar_wait_sleep(bar, uint32_t(phase) & 1, A.err));
-    if (!ok) *bail = 1;
-    return ok && !*bail;
+  // a wait that gave up, or that another warp's giving up ends; `done` says whether the wait is over
+  auto slow_wait = [&](uint64_t* bar, uint32_t parity, auto done) -> bool {
+    const long long start = clock64();
+    while (!done(mbar_try_wait_sleep(bar, parity, 1000000))) {
+      if (*bail) return false;
+      if (clock64() - start > 2000000000LL) {
+        record_error(A.err, SC_ERR_TIMEOUT);
+        *bail = 1;
+        return false;
+      }
+    }
+    return true;
+  };
+  auto wait = [&](uint64_t* bar, int phase) -> bool {  // for a whole warp: all of its lanes go on, or none
+    const uint32_t parity = uint32_t(phase) & 1;
+    auto all = [](bool ok) { return bool(__all_sync(0xffffffffu, ok)); };
+    if (all(mbar_try_wait(bar, parity))) return true;
+    return slow_wait(bar, parity, [&](bool ok) { return all(ok); });
+  };
+  auto wait_alone = [&](uint64_t* bar, int phase) -> bool {  // for one thread
+    const uint32_t parity = uint32_t(phase) & 1;
+    if (mbar_try_wait(bar, parity)) return true;
+    return slow_wait(bar, parity, [](bool ok) { return ok; });
   };
   auto arrive = [&](uint64_t* bar) {
     __syncwarp();
@@ -435,14 +454,13 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       arrive(&B.dec_full[i % RING]);
     }
   } else if (warp == LOAD_WARP) {
-    // ---- loads
-    const bool leader = elect_one();
-    const uint32_t bytes = uint32_t((WHOLE ? 2 : 1) * L::K_BYTES + (a.v_dim > 64 ? 2 : 1) * HALF);
-    int issued = 0;
-    for (int i = 0; i < n; ++i) {
-      const int st = i % STAGES, t0 = (c0 + i) * C;
-      if (!wait(&B.empty[st], i / STAGES + 1)) break;
-      if (leader) {
+    // ---- loads, all of one thread
+    if (elect_one()) {
+      const uint32_t bytes = uint32_t((WHOLE ? 2 : 1) * L::K_BYTES + (a.v_dim > 64 ? 2 : 1) * HALF);
+      int issued = 0;
+      for (; issued < n; ++issued) {
+        const int st = issued % STAGES, t0 = (c0 + issued) * C;
+        if (!wait_alone(&B.empty[st], issued / STAGES + 1)) break;
         uint8_t* stage = smem + st * L::STAGE;
         mbar_arrive_expect_tx(&B.full[st], bytes);
 #pragma unroll
@@ -453,48 +471,41 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         tma_load(stage + 2 * L::K_BYTES, &maps.v, 0, h, t0, b, &B.full[st]);
         if (a.v_dim > 64) tma_load(stage + 2 * L::K_BYTES + HALF, &maps.v, 64, h, t0, b, &B.full[st]);
       }
-      __syncwarp();
-      issued = i + 1;
+      // copies in flight land before the block may end
+      for (int i = max(0, issued - STAGES); i < issued; ++i)
+        mbar_wait_sleep(&B.full[i % STAGES], uint32_t(i / STAGES) & 1, nullptr, 20000000LL);
     }
-    // copies in flight land before the block may end
-    for (int i = max(0, issued - STAGES); i < issued; ++i)
-      mbar_wait_sleep(&B.full[i % STAGES], uint32_t(i / STAGES) & 1, nullptr, 20000000LL);
+    __syncwarp();
   } else if (warp == MMA_WARP) {
-    // ---- the products
-    const bool leader = elect_one();
-    auto k_major = [&](const uint8_t* p, int s) { return desc_k(p + (s / 4) * HALF) + 2 * (s % 4); };
-    auto a_product = [&](int i) {
-      const uint8_t* st = smem + (i % STAGES) * L::STAGE;
-      if (leader) {
+    // ---- the products, all of one thread
+    if (elect_one()) {
+      auto k_major = [&](const uint8_t* p, int s) { return desc_k(p + (s / 4) * HALF) + 2 * (s % 4); };
+      auto a_product = [&](int i) {
+        const uint8_t* st = smem + (i % STAGES) * L::STAGE;
 #pragma unroll
         for (int s = 0; s < DK / 16; ++s)
           mma_ss(tmem + COL_A, k_major(st, s), k_major(st + L::K_BYTES, s), idesc_bf16(64, 64, false, false), s > 0);
         commit(&B.a_full);
-      }
-      __syncwarp();
-    };
-    bool ok = true;
-    if (WHOLE && n > 0 && (ok = wait(&B.full[0], 0))) {
-      fence_after();
-      a_product(0);
-    }
-    for (int i = 0; i < n && ok; ++i) {
-      const int st = i % STAGES;
-      const uint8_t* stage = smem + st * L::STAGE;
-      const uint64_t vt = desc_mn(stage + 2 * L::K_BYTES, HALF);
-      if (WHOLE && i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
-        if (!(ok = wait(&B.full[(i + 1) % STAGES], (i + 1) / STAGES))) break;
-        if (!(ok = wait(&B.a_empty, i))) break;
+      };
+      bool ok = true;
+      if (WHOLE && n > 0 && (ok = wait_alone(&B.full[0], 0))) {
         fence_after();
-        a_product(i + 1);
+        a_product(0);
       }
-      if (!(ok = wait(&B.full[st], i / STAGES))) break;
-      if (!(ok = wait(&B.d_empty, i + 1))) break;
+      for (int i = 0; i < n && ok; ++i) {
+        const int st = i % STAGES;
+        const uint8_t* stage = smem + st * L::STAGE;
+        const uint64_t vt = desc_mn(stage + 2 * L::K_BYTES, HALF);
+        if (WHOLE && i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
+          if (!(ok = wait_alone(&B.full[(i + 1) % STAGES], (i + 1) / STAGES) && wait_alone(&B.a_empty, i))) break;
+          fence_after();
+          a_product(i + 1);
+        }
+        if (!(ok = wait_alone(&B.full[st], i / STAGES) && wait_alone(&B.d_empty, i + 1))) break;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        if (!(ok = wait(&B.kw_full[hf], i))) break;
-        fence_after();
-        if (leader) {
+        for (int hf = 0; hf < 2; ++hf) {
+          if (!(ok = wait_alone(&B.kw_full[hf], i))) break;
+          fence_after();
 #pragma unroll
           for (int term = 2; term >= 0; --term)  // the small ones first
 #pragma unroll
@@ -503,19 +514,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
                      idesc_bf16(128, DK, true, true), hf > 0 || term < 2 || s > 0);
           commit(&B.kw_empty[hf]);
         }
-        __syncwarp();
-      }
-      if (!ok) break;
-      if (leader) {
+        if (!ok) break;
         commit(&B.d_full);
         if (!WHOLE) commit(&B.empty[st]);
-      }
-      __syncwarp();
-      if constexpr (WHOLE) {
-        if (!(ok = wait(&B.s_full, i))) break;
-        if (!(ok = wait(&B.o_empty, i + 1))) break;
-        fence_after();
-        if (leader) {
+        if constexpr (WHOLE) {
+          if (!(ok = wait_alone(&B.s_full, i) && wait_alone(&B.o_empty, i + 1))) break;
+          fence_after();
 #pragma unroll
           for (int term = 1; term >= 0; --term)
 #pragma unroll
@@ -523,11 +527,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
               mma_ts(tmem + COL_X, tmem + COL_S + term * (DK / 2) + 8 * s, k_major(stage, s), idesc_bf16(128, 64, false, false),
                      term < 1 || s > 0);
           commit(&B.s_empty);
-        }
-        __syncwarp();
-        if (!(ok = wait(&B.p_full, i))) break;
-        fence_after();
-        if (leader) {
+          if (!(ok = wait_alone(&B.p_full, i))) break;
+          fence_after();
 #pragma unroll
           for (int s = 0; s < C / 16; ++s)
             mma_ss(tmem + COL_I, vt + 128 * s, desc_k(smem + L::P) + 2 * s, idesc_bf16(128, 64, true, false), s > 0);
@@ -535,10 +536,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
           commit(&B.p_empty);
           commit(&B.empty[st]);
         }
-        __syncwarp();
       }
-    }
-    if (leader) {
       commit(&B.done);  // every product issued has finished
       mbar_wait(&B.done, 0, nullptr, 20000000LL);
     }
