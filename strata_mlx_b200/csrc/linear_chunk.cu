@@ -168,29 +168,24 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   fence_after();
   const uint32_t tmem = B.tmem;
   volatile int* bail = &B.bail;
-  // a wait that gave up, or that another warp's giving up ends; `done` says whether the wait is over
-  auto slow_wait = [&](uint64_t* bar, uint32_t parity, auto done) -> bool {
-    const long long start = clock64();
-    while (!done(mbar_try_wait_sleep(bar, parity, 1000000))) {
-      if (*bail) return false;
-      if (clock64() - start > 2000000000LL) {
-        record_error(A.err, SC_ERR_TIMEOUT);
-        *bail = 1;
-        return false;
-      }
-    }
+  // Waits, for a whole warp (all of its lanes go on, or none) and for one thread. Small in code, as there are many: the
+  // warps' instructions have to fit the cache.
+  auto gave_up = [&] {
+    record_error(A.err, SC_ERR_TIMEOUT);
+    *bail = 1;
+    return false;
+  };
+  auto wait = [&](uint64_t* bar, int phase) -> bool {
+    const uint32_t parity = uint32_t(phase) & 1, start = uint32_t(clock());
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+      if (*bail || uint32_t(clock()) - start > 2000000000u) return __any_sync(0xffffffffu, gave_up());
     return true;
   };
-  auto wait = [&](uint64_t* bar, int phase) -> bool {  // for a whole warp: all of its lanes go on, or none
-    const uint32_t parity = uint32_t(phase) & 1;
-    auto all = [](bool ok) { return bool(__all_sync(0xffffffffu, ok)); };
-    if (all(mbar_try_wait(bar, parity))) return true;
-    return slow_wait(bar, parity, [&](bool ok) { return all(ok); });
-  };
-  auto wait_alone = [&](uint64_t* bar, int phase) -> bool {  // for one thread
-    const uint32_t parity = uint32_t(phase) & 1;
-    if (mbar_try_wait(bar, parity)) return true;
-    return slow_wait(bar, parity, [](bool ok) { return ok; });
+  auto wait_alone = [&](uint64_t* bar, int phase) -> bool {
+    const uint32_t parity = uint32_t(phase) & 1, start = uint32_t(clock());
+    while (!mbar_try_wait(bar, parity))
+      if (*bail || uint32_t(clock()) - start > 2000000000u) return gave_up();
+    return true;
   };
   auto arrive = [&](uint64_t* bar) {
     __syncwarp();
@@ -207,10 +202,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       uint8_t* kw = smem + L::KW;
       const float* w_of = dec[i % RING].w;
       bool ok = true;
-#pragma unroll
+#pragma unroll 1
       for (int hf = 0; hf < 2; ++hf) {
         if (!(ok = wait(&B.kw_empty[hf], i + 1))) break;
-#pragma unroll 4
+#pragma unroll 2
         for (int j = lt; j < C / 2 * DK / 8; j += 128 * KW_GROUPS) {  // 16 bytes of K, the terms to the same place
           const int r = C / 2 * hf + j / 8 % (C / 2), at = j / (C / 2 * 8) * HALF + r * 128 + j % 8 * 16;
           uint4 x = *reinterpret_cast<const uint4*>(kr + at);
@@ -298,7 +293,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         out_sync();  // the tile's last store has read it
         const int t0 = (c0 + i) * C, m = len - t0;
         const float* eg = dec[i % RING].eg;
-#pragma unroll
+#pragma unroll 1
         for (int q = 0; q < 4; ++q) {  // 16 value dimensions by 32 tokens at a time
           const int hf = q >> 1, j0 = 4 * (q & 1);
           uint32_t x[16], y[16];
@@ -477,66 +472,83 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     }
     __syncwarp();
   } else if (warp == MMA_WARP) {
-    // ---- the products, all of one thread
-    if (elect_one()) {
-      auto k_major = [&](const uint8_t* p, int s) { return desc_k(p + (s / 4) * HALF) + 2 * (s % 4); };
-      auto a_product = [&](int i) {
-        const uint8_t* st = smem + (i % STAGES) * L::STAGE;
+    // ---- the products. The whole warp follows the loop, so that what a product is given is uniform; one lane issues.
+    // All 512 columns are this block's, so tensor memory starts at address 0.
+    const bool leader = elect_one();
+    auto k_major = [&](const uint8_t* p, int s) { return desc_k(p) + uint32_t((s >> 2) * (HALF >> 4) + 2 * (s & 3)); };
+    auto a_product = [&](int i) {
+      const uint8_t* st = smem + (i % STAGES) * L::STAGE;
+      if (leader) {
 #pragma unroll
         for (int s = 0; s < DK / 16; ++s)
-          mma_ss(tmem + COL_A, k_major(st, s), k_major(st + L::K_BYTES, s), idesc_bf16(64, 64, false, false), s > 0);
+          mma_ss(COL_A, k_major(st, s), k_major(st + L::K_BYTES, s), idesc_bf16(64, 64, false, false), s > 0);
         commit(&B.a_full);
-      };
-      bool ok = true;
-      if (WHOLE && n > 0 && (ok = wait_alone(&B.full[0], 0))) {
-        fence_after();
-        a_product(0);
       }
-      for (int i = 0; i < n && ok; ++i) {
-        const int st = i % STAGES;
-        const uint8_t* stage = smem + st * L::STAGE;
-        const uint64_t vt = desc_mn(stage + 2 * L::K_BYTES, HALF);
-        if (WHOLE && i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
-          if (!(ok = wait_alone(&B.full[(i + 1) % STAGES], (i + 1) / STAGES) && wait_alone(&B.a_empty, i))) break;
-          fence_after();
-          a_product(i + 1);
-        }
-        if (!(ok = wait_alone(&B.full[st], i / STAGES) && wait_alone(&B.d_empty, i + 1))) break;
+      __syncwarp();
+    };
+    bool ok = tmem == 0;
+    if (!ok) record_error(A.err, SC_ERR_CUDA), *bail = 1;
+    if (WHOLE && n > 0 && ok && (ok = wait(&B.full[0], 0))) {
+      fence_after();
+      a_product(0);
+    }
+    for (int i = 0; i < n && ok; ++i) {
+      const int st = i % STAGES;
+      const uint8_t* stage = smem + st * L::STAGE;
+      const uint64_t vt = desc_mn(stage + 2 * L::K_BYTES, HALF);
+      if (WHOLE && i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
+        if (!(ok = wait(&B.full[(i + 1) % STAGES], (i + 1) / STAGES) && wait(&B.a_empty, i))) break;
+        fence_after();
+        a_product(i + 1);
+      }
+      if (!(ok = wait(&B.full[st], i / STAGES) && wait(&B.d_empty, i + 1))) break;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          if (!(ok = wait_alone(&B.kw_full[hf], i))) break;
-          fence_after();
+      for (int hf = 0; hf < 2; ++hf) {
+        if (!(ok = wait(&B.kw_full[hf], i))) break;
+        fence_after();
+        if (leader) {
 #pragma unroll
           for (int term = 2; term >= 0; --term)  // the small ones first
 #pragma unroll
             for (int s = 2 * hf; s < 2 * hf + 2; ++s)
-              mma_ss(tmem + COL_D, vt + 128 * s, desc_mn(smem + L::KW + term * L::K_BYTES, HALF) + 128 * s,
+              mma_ss(COL_D, vt + 128 * s, desc_mn(smem + L::KW + term * L::K_BYTES, HALF) + 128 * s,
                      idesc_bf16(128, DK, true, true), hf > 0 || term < 2 || s > 0);
           commit(&B.kw_empty[hf]);
+          if (hf == 1) {
+            commit(&B.d_full);
+            if (!WHOLE) commit(&B.empty[st]);
+          }
         }
-        if (!ok) break;
-        commit(&B.d_full);
-        if (!WHOLE) commit(&B.empty[st]);
-        if constexpr (WHOLE) {
-          if (!(ok = wait_alone(&B.s_full, i) && wait_alone(&B.o_empty, i + 1))) break;
-          fence_after();
+        __syncwarp();
+      }
+      if (!ok) break;
+      if constexpr (WHOLE) {
+        if (!(ok = wait(&B.s_full, i) && wait(&B.o_empty, i + 1))) break;
+        fence_after();
+        if (leader) {
 #pragma unroll
           for (int term = 1; term >= 0; --term)
 #pragma unroll
             for (int s = 0; s < DK / 16; ++s)
-              mma_ts(tmem + COL_X, tmem + COL_S + term * (DK / 2) + 8 * s, k_major(stage, s), idesc_bf16(128, 64, false, false),
+              mma_ts(COL_X, COL_S + term * (DK / 2) + 8 * s, k_major(stage, s), idesc_bf16(128, 64, false, false),
                      term < 1 || s > 0);
           commit(&B.s_empty);
-          if (!(ok = wait_alone(&B.p_full, i))) break;
-          fence_after();
+        }
+        __syncwarp();
+        if (!(ok = wait(&B.p_full, i))) break;
+        fence_after();
+        if (leader) {
 #pragma unroll
           for (int s = 0; s < C / 16; ++s)
-            mma_ss(tmem + COL_I, vt + 128 * s, desc_k(smem + L::P) + 2 * s, idesc_bf16(128, 64, true, false), s > 0);
+            mma_ss(COL_I, vt + 128 * s, desc_k(smem + L::P) + 2 * s, idesc_bf16(128, 64, true, false), s > 0);
           commit(&B.o_full);
           commit(&B.p_empty);
           commit(&B.empty[st]);
         }
+        __syncwarp();
       }
+    }
+    if (leader) {
       commit(&B.done);  // every product issued has finished
       mbar_wait(&B.done, 0, nullptr, 20000000LL);
     }
