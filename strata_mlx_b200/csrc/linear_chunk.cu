@@ -15,11 +15,13 @@
 //   0-3    P from A                             4-7    the outputs, stored by TMA through a tile in shared memory
 //   8-15   the state (a lane a value dimension, half of k_dim each)
 //   16-19  w K, in halves of 32 tokens so that D's products run behind it; zeros over the values past a length
-//   20     one lane issues the products      21  the chunks' decays      22  loads by TMA, three chunks in flight
+//   20     one lane issues the products      21  the chunks' decays      22, 23  loads by TMA
 // Tensor memory: A, I, X, D and the two terms of S^T, 448 of 512 columns.
 //
 // One sequence's heads fill few SMs, so a long prompt is cut into segments: a first launch works out what each
-// segment adds to the state (D alone), a second adds up the states before the segments, a third is the whole.
+// segment adds to the state, a second adds up the states before the segments, a third is the whole. The first takes a
+// segment's chunks from the last to the first, the weights w running on from chunk to chunk, so that D of eight chunks
+// adds up in tensor memory and no state is carried between them.
 // What bounds it: a chunk's loads and stores are 64 KB at 128 dimensions (1.5 us of an SM's share of the measured
 // copy), its products about 1,800 tensor cycles, and its conversions about 7,000 warp instructions.
 // Every wait is bounded; one that gives up records SC_ERR_TIMEOUT and the block winds down.
@@ -36,14 +38,20 @@ namespace lc {
 using namespace tc;
 
 constexpr int C = 64;        // tokens of a chunk
-constexpr int STAGES = 3;    // chunks loaded ahead
+// chunks of queries, keys and values held: scores are made a chunk ahead and a chunk's queries are needed until its
+// last products, keys until w K is made, values for the chunk's own products only
+constexpr int QS = 4, KS = 3, VS = 2;
 constexpr int RING = 4;      // chunks whose decays are held
 constexpr int HALF = C * 128;  // bytes of 64 columns of a chunk's rows
-constexpr int OUT_WARP = 4, STATE_WARP = 8, KW_WARP = 16, MMA_WARP = 20, DECAY_WARP = 21, LOAD_WARP = 22;
 constexpr int THREADS = 24 * 32;
+constexpr int OUT_WARP = 4, STATE_WARP = 8, KW_WARP = 16, MMA_WARP = 20, DECAY_WARP = 21, LOAD_WARP = 22, VALUE_WARP = 23;
 // registers a thread: 80 at launch; the groups' shares add up to as many
 constexpr int P_REGS = 72, OUT_REGS = 72, STATE_REGS = 112, KW_REGS = 72, CONTROL_REGS = 40;
 static_assert(P_REGS + OUT_REGS + 2 * STATE_REGS + KW_REGS + CONTROL_REGS == 6 * 80, "a block's registers");
+// the first launch's: 12 warps make w K, 8 add up D, 3 control
+constexpr int ADD_SUM_WARP = 12, ADD_STAGES = 4, ADD_RUN = 8;  // chunks whose D adds up in tensor memory
+constexpr int SUM_REGS = 96;
+static_assert(3 * 80 + 2 * SUM_REGS + CONTROL_REGS <= 6 * 80, "a block's registers");
 constexpr int SMS = 148;
 constexpr float LEAST = -30.f;  // a token's decay below e^-30 is taken as e^-30: past it nothing is left in float32
 
@@ -56,9 +64,16 @@ struct Decays {
 };
 
 struct Bars {
-  uint64_t full[STAGES], empty[STAGES], dec_full[RING], dec_empty[RING];
+  uint64_t q_full[QS], q_empty[QS], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], dec_full[RING], dec_empty[RING];
   uint64_t a_full, a_empty, p_full, p_empty, o_full, o_empty, kw_full[2], kw_empty[2], d_full, d_empty, s_full, s_empty,
       done;
+  uint32_t tmem;
+  int bail;
+};
+
+struct AddBars {
+  uint64_t full[ADD_STAGES], empty[ADD_STAGES], dec_full[RING], dec_empty[RING], kw_full[2], kw_empty[2], d_full[2],
+      d_empty[2], done;
   uint32_t tmem;
   int bail;
 };
@@ -66,9 +81,15 @@ struct Bars {
 template <int DK>
 struct Shape {
   static constexpr int K_BYTES = DK / 64 * HALF, V_BYTES = 2 * HALF;
-  static constexpr int STAGE = 2 * K_BYTES + V_BYTES;
-  static constexpr int KW = STAGES * STAGE, P = KW + 3 * K_BYTES, OUT = P + HALF, DEC = OUT + 2 * HALF, BARS = DEC + RING * int(sizeof(Decays));
+  static constexpr int Q = 0, K = Q + QS * K_BYTES, V = K + KS * K_BYTES, KW = V + VS * V_BYTES, P = KW + 3 * K_BYTES;
+  static constexpr int OUT = P + HALF, DEC = OUT + V_BYTES, BARS = DEC + RING * int(sizeof(Decays));
   static constexpr int BYTES = BARS + int(sizeof(Bars)) + 1024;  // and to align the start
+};
+template <int DK>
+struct AddShape {
+  static constexpr int K_BYTES = DK / 64 * HALF, V_BYTES = 2 * HALF, STAGE = K_BYTES + V_BYTES;
+  static constexpr int KW = ADD_STAGES * STAGE, DEC = KW + 2 * 3 * K_BYTES, BARS = DEC + RING * C * 4;
+  static constexpr int BYTES = BARS + int(sizeof(AddBars)) + 1024;
 };
 
 struct Args {
@@ -125,11 +146,238 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t& t0, uint32_t&
   t2 = bits_of(__floats2bfloat162_rn(x - lo_f(t1), y - hi_f(t1)));
 }
 
-template <int DK, bool WHOLE>
-__global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant__ Args A,
-                                                               const __grid_constant__ Maps maps) {
+// Waits, for a whole warp (all of its lanes go on, or none) and for one thread. Small in code, as there are many: the
+// warps' instructions have to fit the cache.
+struct Waits {
+  int* err;
+  volatile int* bail;
+  __device__ __forceinline__ bool gave_up() const {
+    record_error(err, SC_ERR_TIMEOUT);
+    *bail = 1;
+    return false;
+  }
+  __device__ __forceinline__ bool operator()(uint64_t* bar, int phase) const {
+    const uint32_t parity = uint32_t(phase) & 1, start = uint32_t(clock());
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+      if (__any_sync(0xffffffffu, *bail || uint32_t(clock()) - start > 2000000000u)) return gave_up();
+    return true;
+  }
+  __device__ __forceinline__ bool alone(uint64_t* bar, int phase) const {
+    const uint32_t parity = uint32_t(phase) & 1, start = uint32_t(clock());
+    while (!mbar_try_wait(bar, parity))
+      if (*bail || uint32_t(clock()) - start > 2000000000u) return gave_up();
+    return true;
+  }
+};
+__device__ __forceinline__ void arrive(uint64_t* bar) {  // a warp's
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+__device__ __forceinline__ void tmem_alloc(uint32_t* at) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(at)), "r"(512) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(512));
+}
+
+// 16 bytes of K times w as three terms of 16 bytes, at one place of three tiles; zeros where `in` is not set
+__device__ __forceinline__ void split_piece(const uint8_t* k, float w, bool in, uint8_t* to, int term) {
+  uint4 x = *reinterpret_cast<const uint4*>(k);
+  if (!in) x = make_uint4(0, 0, 0, 0);
+  uint4 t0, t1, t2;
+  split3(lo_f(x.x) * w, hi_f(x.x) * w, t0.x, t1.x, t2.x);
+  split3(lo_f(x.y) * w, hi_f(x.y) * w, t0.y, t1.y, t2.y);
+  split3(lo_f(x.z) * w, hi_f(x.z) * w, t0.z, t1.z, t2.z);
+  split3(lo_f(x.w) * w, hi_f(x.w) * w, t0.w, t1.w, t2.w);
+  *reinterpret_cast<uint4*>(to) = t0;
+  *reinterpret_cast<uint4*>(to + term) = t1;
+  *reinterpret_cast<uint4*>(to + 2 * term) = t2;
+}
+
+// values past the length meet zeros of P and w K, which a NaN would spoil: zeros in their place, by `step` threads
+__device__ __forceinline__ void clear_values(uint8_t* v, int m, int thread, int step) {
+  for (int j = thread; j < 2 * HALF / 16; j += step)
+    if ((j * 16 % HALF) / 128 >= m) *reinterpret_cast<uint4*>(v + 16 * j) = make_uint4(0, 0, 0, 0);
+}
+
+// the second half of the values is not loaded where there are 64 or fewer: zeros
+__device__ __forceinline__ void clear_halves(uint8_t* v, int n, int apart) {
+  for (int i = threadIdx.x; i < n * HALF / 16; i += THREADS)
+    *reinterpret_cast<uint4*>(v + i / (HALF / 16) * apart + HALF + 16 * (i % (HALF / 16))) = make_uint4(0, 0, 0, 0);
+  fence_async();
+}
+
+// D += V^T (w K): the half `hf` of the tokens, the small terms first
+template <int DK>
+__device__ __forceinline__ void add_products(uint32_t d, uint64_t v, uint64_t kw, int hf, bool first) {
+#pragma unroll
+  for (int term = 2; term >= 0; --term)
+#pragma unroll
+    for (int s = 2 * hf; s < 2 * hf + 2; ++s)
+      mma_ss(d, v + 128 * s, kw + uint32_t(term * (DK / 64) * (HALF >> 4) + 128 * s), idesc_bf16(128, DK, true, true),
+             !first || term < 2 || s > 2 * hf);
+}
+
+// a lane's two decays of a chunk: tokens 2 lane and 2 lane + 1 from t0 on
+__device__ __forceinline__ float2 two_decays(const float* decay, int64_t token, int t0, int len) {
+  const int t = t0 + 2 * (threadIdx.x & 31);
+  return make_float2(t < len ? fmaxf(decay[t * token], LEAST) : 0.f, t + 1 < len ? fmaxf(decay[(t + 1) * token], LEAST) : 0.f);
+}
+
+// What a segment adds to the state, and its decay.
+template <int DK>
+__global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__ Args A, const __grid_constant__ Maps maps) {
+  using L = AddShape<DK>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  float* dec = reinterpret_cast<float*>(smem + L::DEC);  // (RING, C) weights
+  AddBars& B = *reinterpret_cast<AddBars*>(smem + L::BARS);
+  const sc_linear& a = A.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int seg = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / (a.v_heads / a.k_heads);
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.tokens) : a.tokens;
+  const int c0 = seg * A.per, n = max(0, min(c0 + A.per, (len + C - 1) / C) - c0);
+  if (tid == 0) {
+    for (int i = 0; i < ADD_STAGES; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], ADD_SUM_WARP + 1);
+    for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], ADD_SUM_WARP);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B.kw_full[i], ADD_SUM_WARP), mbar_init(&B.kw_empty[i], 1);
+      mbar_init(&B.d_full[i], 1), mbar_init(&B.d_empty[i], 8);
+    }
+    mbar_init(&B.done, 1);
+    B.bail = 0;
+    fence_mbar_init();
+  }
+  if (warp == MMA_WARP) tmem_alloc(&B.tmem);
+  if (a.v_dim <= 64) clear_halves(smem + L::K_BYTES, ADD_STAGES, L::STAGE);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = B.tmem;
+  const Waits wait{A.err, &B.bail};
+  auto chunk = [&](int i) { return c0 + n - 1 - i; };  // the last first
+  if (warp < ADD_SUM_WARP) {
+    for (int i = 0; i < n; ++i) {
+      const int st = i % ADD_STAGES, m = len - chunk(i) * C;
+      if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.full[st], i / ADD_STAGES) || !wait(&B.kw_empty[i & 1], i / 2 + 1))
+        break;
+      const float* w = dec + i % RING * C;
+      uint8_t* kw = smem + L::KW + (i & 1) * 3 * L::K_BYTES;
+#pragma unroll 2
+      for (int j = tid; j < C * DK / 8; j += ADD_SUM_WARP * 32) {
+        const int r = (j * 16 % HALF) / 128;
+        split_piece(smem + st * L::STAGE + 16 * j, w[r], r < m, kw + 16 * j, L::K_BYTES);
+      }
+      if (m < C) clear_values(smem + st * L::STAGE + L::K_BYTES, m, tid, ADD_SUM_WARP * 32);
+      fence_async();
+      arrive(&B.kw_full[i & 1]);
+      arrive(&B.empty[st]);
+      arrive(&B.dec_empty[i % RING]);
+    }
+  } else if (warp < MMA_WARP) {
+    // ---- the sums of ADD_RUN chunks into one
+    more_registers<SUM_REGS>();
+    constexpr int N = DK / 2;
+    const uint32_t quarter = uint32_t(warp & 3) * 32, lanes = tmem + (quarter << 16);
+    const int dv = int(quarter) + lane, k0 = (warp - ADD_SUM_WARP) / 4 * N;
+    float S[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) S[k] = 0.f;
+    for (int r = 0; r * ADD_RUN < n; ++r) {
+      if (!wait(&B.d_full[r & 1], r / 2)) break;
+      fence_after();
+#pragma unroll
+      for (int k = 0; k < N; k += 16) {
+        uint32_t x[16];
+        ld16(lanes + (r & 1) * 128 + k0 + k, x);
+        wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) S[k + e] += __uint_as_float(x[e]);
+      }
+      fence_before();
+      arrive(&B.d_empty[r & 1]);
+    }
+    float* to = A.parts + ((int64_t(b) * a.v_heads + h) * A.segments + seg) * DK * 128 + dv;
+#pragma unroll
+    for (int k = 0; k < N; ++k) to[int64_t(k0 + k) * 128] = S[k];
+  } else {
+    fewer_registers<CONTROL_REGS>();
+    if (warp == DECAY_WARP) {
+      const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
+      float later = 0.f;  // the decays of the chunks behind this one
+      float2 next = n ? two_decays(decay, a.decay_token, chunk(0) * C, len) : make_float2(0.f, 0.f);
+      bool ok = true;
+      for (int i = 0; i < n; ++i) {
+        const float2 g = next;
+        if (i + 1 < n) next = two_decays(decay, a.decay_token, chunk(i + 1) * C, len);
+        float down = g.x + g.y;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const float y = __shfl_down_sync(0xffffffffu, down, o);
+          if (lane + o < 32) down += y;
+        }
+        float after = __shfl_down_sync(0xffffffffu, down, 1);
+        if (lane == 31) after = 0.f;
+        after += later;
+        if (!(ok = wait(&B.dec_empty[i % RING], i / RING + 1))) break;
+        *reinterpret_cast<float2*>(dec + i % RING * C + 2 * lane) = make_float2(expf(after + g.y), expf(after));
+        later += __shfl_sync(0xffffffffu, down, 0);
+        arrive(&B.dec_full[i % RING]);
+      }
+      if (lane == 0) A.logs[(int64_t(b) * a.v_heads + h) * A.segments + seg] = later;
+    } else if (warp == LOAD_WARP) {
+      if (elect_one()) {
+        const uint32_t bytes = uint32_t(L::K_BYTES + (a.v_dim > 64 ? 2 : 1) * HALF);
+        int i = 0;
+        for (; i < n; ++i) {
+          const int st = i % ADD_STAGES, t0 = chunk(i) * C;
+          if (!wait.alone(&B.empty[st], i / ADD_STAGES + 1)) break;
+          uint8_t* stage = smem + st * L::STAGE;
+          mbar_arrive_expect_tx(&B.full[st], bytes);
+          for (int x = 0; x < DK; x += 64) tma_load(stage + x / 64 * HALF, &maps.k, x, hk, t0, b, &B.full[st]);
+          for (int x = 0; x < a.v_dim; x += 64) tma_load(stage + L::K_BYTES + x / 64 * HALF, &maps.v, x, h, t0, b, &B.full[st]);
+        }
+        // copies in flight land before the block may end
+        for (int k = max(0, i - ADD_STAGES); k < i; ++k)
+          mbar_wait(&B.full[k % ADD_STAGES], uint32_t(k / ADD_STAGES) & 1, nullptr, 20000000LL);
+      }
+    } else if (warp == MMA_WARP) {
+      const bool leader = elect_one();
+      bool ok = tmem == 0;  // all 512 columns are this block's
+      if (!ok) wait.gave_up();
+      for (int i = 0; i < n && ok; ++i) {
+        const int st = i % ADD_STAGES, run = i / ADD_RUN;
+        if (i % ADD_RUN == 0 && !(ok = wait(&B.d_empty[run & 1], run / 2 + 1))) break;
+        if (!(ok = wait(&B.full[st], i / ADD_STAGES) && wait(&B.kw_full[i & 1], i / 2))) break;
+        fence_after();
+        if (leader) {
+          const uint64_t v = desc_mn(smem + st * L::STAGE + L::K_BYTES, HALF), kw = desc_mn(smem + L::KW + (i & 1) * 3 * L::K_BYTES, HALF);
+          add_products<DK>((run & 1) * 128, v, kw, 0, i % ADD_RUN == 0);
+          add_products<DK>((run & 1) * 128, v, kw, 1, false);
+          commit(&B.kw_empty[i & 1]);
+          commit(&B.empty[st]);
+          if (i % ADD_RUN == ADD_RUN - 1 || i == n - 1) commit(&B.d_full[run & 1]);
+        }
+        __syncwarp();
+      }
+      if (leader) {
+        commit(&B.done);  // every product issued has finished
+        mbar_wait(&B.done, 0, nullptr, 20000000LL);
+      }
+    }
+    __syncwarp();
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == MMA_WARP) tmem_free(tmem);
+}
+
+template <int DK>
+__global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant__ Args A, const __grid_constant__ Maps maps) {
   using L = Shape<DK>;
-  constexpr int KW_GROUPS = WHOLE ? 1 : 3;  // without outputs, those warps make w K too
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   Decays* dec = reinterpret_cast<Decays*>(smem + L::DEC);
@@ -141,102 +389,29 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   const int c0 = seg * A.per, all = (a.tokens + C - 1) / C, c1 = min(all, c0 + A.per);
   const int n = max(0, min(c1, (len + C - 1) / C) - c0);  // this segment's chunks with tokens
   if (tid == 0) {
-    for (int i = 0; i < STAGES; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], KW_GROUPS * 4 + 1);
+    for (int i = 0; i < QS; ++i) mbar_init(&B.q_full[i], 1), mbar_init(&B.q_empty[i], 1);
+    for (int i = 0; i < KS; ++i) mbar_init(&B.k_full[i], 1), mbar_init(&B.k_empty[i], 4 + 1);
+    for (int i = 0; i < VS; ++i) mbar_init(&B.v_full[i], 1), mbar_init(&B.v_empty[i], 1);
     for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], 20);
     mbar_init(&B.a_full, 1), mbar_init(&B.a_empty, 4), mbar_init(&B.p_full, 4), mbar_init(&B.p_empty, 1);
     mbar_init(&B.o_full, 1), mbar_init(&B.o_empty, 4);
-    for (int i = 0; i < 2; ++i) mbar_init(&B.kw_full[i], KW_GROUPS * 4), mbar_init(&B.kw_empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&B.kw_full[i], 4), mbar_init(&B.kw_empty[i], 1);
     mbar_init(&B.d_full, 1), mbar_init(&B.d_empty, 8), mbar_init(&B.s_full, 8), mbar_init(&B.s_empty, 1);
     mbar_init(&B.done, 1);
     B.bail = 0;
     fence_mbar_init();
   }
-  if (warp == MMA_WARP) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B.tmem)), "r"(512)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  if (a.v_dim <= 64) {  // the second half of the values is never loaded: zeros
-    for (int i = tid; i < STAGES * HALF / 16; i += THREADS) {
-      uint8_t* half = smem + i / (HALF / 16) * L::STAGE + 2 * L::K_BYTES + HALF;
-      *reinterpret_cast<uint4*>(half + 16 * (i % (HALF / 16))) = make_uint4(0, 0, 0, 0);
-    }
-    fence_async();
-  }
+  if (warp == MMA_WARP) tmem_alloc(&B.tmem);
+  if (a.v_dim <= 64) clear_halves(smem + L::V, VS, L::V_BYTES);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = B.tmem;
-  volatile int* bail = &B.bail;
-  // Waits, for a whole warp (all of its lanes go on, or none) and for one thread. Small in code, as there are many: the
-  // warps' instructions have to fit the cache.
-  auto gave_up = [&] {
-    record_error(A.err, SC_ERR_TIMEOUT);
-    *bail = 1;
-    return false;
-  };
-  auto wait = [&](uint64_t* bar, int phase) -> bool {
-    const uint32_t parity = uint32_t(phase) & 1, start = uint32_t(clock());
-    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
-      if (*bail || uint32_t(clock()) - start > 2000000000u) return __any_sync(0xffffffffu, gave_up());
-    return true;
-  };
-  auto wait_alone = [&](uint64_t* bar, int phase) -> bool {
-    const uint32_t parity = uint32_t(phase) & 1, start = uint32_t(clock());
-    while (!mbar_try_wait(bar, parity))
-      if (*bail || uint32_t(clock()) - start > 2000000000u) return gave_up();
-    return true;
-  };
-  auto arrive = [&](uint64_t* bar) {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar);
-  };
+  const Waits wait{A.err, &B.bail};
   const uint32_t quarter = uint32_t(warp & 3) * 32, lanes = tmem + (quarter << 16);
 
-  auto make_kw = [&](int lt) {  // `lt` of 128 KW_GROUPS threads
-    for (int i = 0; i < n; ++i) {
-      const int st = i % STAGES, m = len - (c0 + i) * C;
-      if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.full[st], i / STAGES)) break;
-      uint8_t* stage = smem + st * L::STAGE;
-      const uint8_t* kr = stage + L::K_BYTES;
-      uint8_t* kw = smem + L::KW;
-      const float* w_of = dec[i % RING].w;
-      bool ok = true;
-#pragma unroll 1
-      for (int hf = 0; hf < 2; ++hf) {
-        if (!(ok = wait(&B.kw_empty[hf], i + 1))) break;
-#pragma unroll 2
-        for (int j = lt; j < C / 2 * DK / 8; j += 128 * KW_GROUPS) {  // 16 bytes of K, the terms to the same place
-          const int r = C / 2 * hf + j / 8 % (C / 2), at = j / (C / 2 * 8) * HALF + r * 128 + j % 8 * 16;
-          uint4 x = *reinterpret_cast<const uint4*>(kr + at);
-          const float w = w_of[r];
-          if (r >= m) x = make_uint4(0, 0, 0, 0);
-          uint4 t0, t1, t2;
-          split3(lo_f(x.x) * w, hi_f(x.x) * w, t0.x, t1.x, t2.x);
-          split3(lo_f(x.y) * w, hi_f(x.y) * w, t0.y, t1.y, t2.y);
-          split3(lo_f(x.z) * w, hi_f(x.z) * w, t0.z, t1.z, t2.z);
-          split3(lo_f(x.w) * w, hi_f(x.w) * w, t0.w, t1.w, t2.w);
-          *reinterpret_cast<uint4*>(kw + at) = t0;
-          *reinterpret_cast<uint4*>(kw + L::K_BYTES + at) = t1;
-          *reinterpret_cast<uint4*>(kw + 2 * L::K_BYTES + at) = t2;
-        }
-        if (hf == 0 && m < C)  // values past the length meet zeros of P and w K, which a NaN would spoil
-          for (int j = lt; j < 2 * HALF / 16; j += 128 * KW_GROUPS)
-            if ((j * 16 % HALF) / 128 >= m) *reinterpret_cast<uint4*>(stage + 2 * L::K_BYTES + 16 * j) = make_uint4(0, 0, 0, 0);
-        fence_async();
-        arrive(&B.kw_full[hf]);
-      }
-      if (!ok) break;
-      arrive(&B.empty[st]);  // K has been read
-      arrive(&B.dec_empty[i % RING]);
-    }
-  };
-
   if (warp < STATE_WARP) {
-    if constexpr (!WHOLE) {
-      fewer_registers<KW_REGS>();
-      make_kw(tid);
-    } else if (warp < OUT_WARP) {
+    if (warp < OUT_WARP) {
       // ---- P
       fewer_registers<P_REGS>();
       const int g = lane >> 2, t = lane & 3, r0 = 16 * warp + g;
@@ -349,13 +524,13 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     const int dv = int(quarter) + lane, k0 = (warp - STATE_WARP) / 4 * N;
     float S[N];
     const int64_t head = int64_t(b) * a.v_heads + h;
-    const bool started = WHOLE && A.segments > 1;
+    const bool started = A.segments > 1;
     const float* from = started ? A.parts + (head * A.segments + seg) * DK * 128 + dv
                                 : a.state_in + head * a.k_dim * a.v_dim + dv;
     const int ld = started ? 128 : a.v_dim;
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      S[k] = WHOLE && (started || (a.state_in && dv < a.v_dim && k0 + k < a.k_dim)) ? from[int64_t(k0 + k) * ld] : 0.f;
+      S[k] = started || (a.state_in && dv < a.v_dim && k0 + k < a.k_dim) ? from[int64_t(k0 + k) * ld] : 0.f;
     auto publish = [&] {  // S^T as two terms, the A operand of X
 #pragma unroll
       for (int k = 0; k < N; k += 16) {
@@ -373,8 +548,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       fence_before();
       arrive(&B.s_full);
     };
-    if (WHOLE && n > 0) publish();
-    float log = 0.f;
+    if (n > 0) publish();
     for (int i = 0; i < n; ++i) {
       if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.d_full, i)) break;
       fence_after();
@@ -387,22 +561,16 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
 #pragma unroll
         for (int e = 0; e < 16; ++e) S[k + e] = fmaf(d, S[k + e], fmaf(one, S[k + e], __uint_as_float(r[e])));
       }
-      if (!WHOLE) log += dec[i % RING].g2[C - 1];
       fence_before();
       arrive(&B.d_empty);
       arrive(&B.dec_empty[i % RING]);
-      if (WHOLE && i + 1 < n) {
+      if (i + 1 < n) {
         if (!wait(&B.s_empty, i)) break;
         fence_after();
         publish();
       }
     }
-    if (!WHOLE) {
-      float* to = A.parts + (head * A.segments + seg) * DK * 128 + dv;
-#pragma unroll
-      for (int k = 0; k < N; ++k) to[int64_t(k0 + k) * 128] = S[k];
-      if (warp == STATE_WARP && lane == 0) A.logs[head * A.segments + seg] = log * 0.69314718056f;
-    } else if (seg == A.segments - 1) {
+    if (seg == A.segments - 1) {
       float* to = a.state_out + head * a.k_dim * a.v_dim + dv;
 #pragma unroll
       for (int k = 0; k < N; ++k)
@@ -411,20 +579,41 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   } else if (warp < MMA_WARP) {
     // ---- w K
     fewer_registers<KW_REGS>();
-    make_kw(WHOLE ? tid - KW_WARP * 32 : 256 + tid - KW_WARP * 32);
+    const int lt = tid - KW_WARP * 32;
+    for (int i = 0; i < n; ++i) {
+      const int m = len - (c0 + i) * C;
+      if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.k_full[i % KS], i / KS)) break;
+      const uint8_t* k = smem + L::K + i % KS * L::K_BYTES;
+      const float* w = dec[i % RING].w;
+      if (m < C) {
+        if (!wait(&B.v_full[i % VS], i / VS)) break;
+        clear_values(smem + L::V + i % VS * L::V_BYTES, m, lt, 128);
+      }
+      bool ok = true;
+#pragma unroll 1
+      for (int hf = 0; hf < 2; ++hf) {
+        if (!(ok = wait(&B.kw_empty[hf], i + 1))) break;
+#pragma unroll 2
+        for (int j = lt; j < C / 2 * DK / 8; j += 128) {
+          const int r = C / 2 * hf + j / 8 % (C / 2), at = j / (C / 2 * 8) * HALF + r * 128 + j % 8 * 16;
+          split_piece(k + at, w[r], r < m, smem + L::KW + at, L::K_BYTES);
+        }
+        fence_async();
+        arrive(&B.kw_full[hf]);
+      }
+      if (!ok) break;
+      arrive(&B.k_empty[i % KS]);
+      arrive(&B.dec_empty[i % RING]);
+    }
   } else {
   fewer_registers<CONTROL_REGS>();
   if (warp == DECAY_WARP) {
     // ---- a chunk's decays: a lane tokens 2 lane and 2 lane + 1, sums from the front and from the back
     const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
-    auto decay_of = [&](int i, int e) -> float {
-      const int t = (c0 + i) * C + 2 * lane + e;
-      return i < n && t < len ? fmaxf(decay[int64_t(t) * a.decay_token], LEAST) : 0.f;
-    };
-    float d0 = decay_of(0, 0), d1 = decay_of(0, 1);
+    float2 next = two_decays(decay, a.decay_token, c0 * C, n ? len : 0);
     for (int i = 0; i < n; ++i) {
-      const float g0 = d0, g1 = d1, pair = g0 + g1;
-      d0 = decay_of(i + 1, 0), d1 = decay_of(i + 1, 1);
+      const float g0 = next.x, g1 = next.y, pair = g0 + g1;
+      if (i + 1 < n) next = two_decays(decay, a.decay_token, (c0 + i + 1) * C, len);
       float up = pair, down = pair;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -449,26 +638,38 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       arrive(&B.dec_full[i % RING]);
     }
   } else if (warp == LOAD_WARP) {
-    // ---- loads, all of one thread
+    // ---- keys and queries
     if (elect_one()) {
-      const uint32_t bytes = uint32_t((WHOLE ? 2 : 1) * L::K_BYTES + (a.v_dim > 64 ? 2 : 1) * HALF);
-      int issued = 0;
-      for (; issued < n; ++issued) {
-        const int st = issued % STAGES, t0 = (c0 + issued) * C;
-        if (!wait_alone(&B.empty[st], issued / STAGES + 1)) break;
-        uint8_t* stage = smem + st * L::STAGE;
-        mbar_arrive_expect_tx(&B.full[st], bytes);
-#pragma unroll
-        for (int x = 0; x < DK; x += 64) {
-          if (WHOLE) tma_load(stage + x / 64 * HALF, &maps.q, x, hk, t0, b, &B.full[st]);
-          tma_load(stage + L::K_BYTES + x / 64 * HALF, &maps.k, x, hk, t0, b, &B.full[st]);
+      int i = 0;
+      for (; i < n; ++i) {
+        const int t0 = (c0 + i) * C, ks = i % KS, qs = i % QS;
+        if (!wait.alone(&B.k_empty[ks], i / KS + 1)) break;
+        mbar_arrive_expect_tx(&B.k_full[ks], L::K_BYTES);
+        for (int x = 0; x < DK; x += 64) tma_load(smem + L::K + ks * L::K_BYTES + x / 64 * HALF, &maps.k, x, hk, t0, b, &B.k_full[ks]);
+        if (!wait.alone(&B.q_empty[qs], i / QS + 1)) {
+          mbar_wait(&B.k_full[ks], uint32_t(i / KS) & 1, nullptr, 20000000LL);
+          break;
         }
-        tma_load(stage + 2 * L::K_BYTES, &maps.v, 0, h, t0, b, &B.full[st]);
-        if (a.v_dim > 64) tma_load(stage + 2 * L::K_BYTES + HALF, &maps.v, 64, h, t0, b, &B.full[st]);
+        mbar_arrive_expect_tx(&B.q_full[qs], L::K_BYTES);
+        for (int x = 0; x < DK; x += 64) tma_load(smem + L::Q + qs * L::K_BYTES + x / 64 * HALF, &maps.q, x, hk, t0, b, &B.q_full[qs]);
       }
       // copies in flight land before the block may end
-      for (int i = max(0, issued - STAGES); i < issued; ++i)
-        mbar_wait_sleep(&B.full[i % STAGES], uint32_t(i / STAGES) & 1, nullptr, 20000000LL);
+      for (int k = max(0, i - KS); k < i; ++k) mbar_wait(&B.k_full[k % KS], uint32_t(k / KS) & 1, nullptr, 20000000LL);
+      for (int k = max(0, i - QS); k < i; ++k) mbar_wait(&B.q_full[k % QS], uint32_t(k / QS) & 1, nullptr, 20000000LL);
+    }
+    __syncwarp();
+  } else if (warp == VALUE_WARP) {
+    // ---- values
+    if (elect_one()) {
+      int i = 0;
+      for (; i < n; ++i) {
+        const int vs = i % VS;
+        if (!wait.alone(&B.v_empty[vs], i / VS + 1)) break;
+        mbar_arrive_expect_tx(&B.v_full[vs], (a.v_dim > 64 ? 2 : 1) * HALF);
+        for (int x = 0; x < a.v_dim; x += 64)
+          tma_load(smem + L::V + vs * L::V_BYTES + x / 64 * HALF, &maps.v, x, h, (c0 + i) * C, b, &B.v_full[vs]);
+      }
+      for (int k = max(0, i - VS); k < i; ++k) mbar_wait(&B.v_full[k % VS], uint32_t(k / VS) & 1, nullptr, 20000000LL);
     }
     __syncwarp();
   } else if (warp == MMA_WARP) {
@@ -477,76 +678,67 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     const bool leader = elect_one();
     auto k_major = [&](const uint8_t* p, int s) { return desc_k(p) + uint32_t((s >> 2) * (HALF >> 4) + 2 * (s & 3)); };
     auto a_product = [&](int i) {
-      const uint8_t* st = smem + (i % STAGES) * L::STAGE;
+      const uint8_t *q = smem + L::Q + i % QS * L::K_BYTES, *k = smem + L::K + i % KS * L::K_BYTES;
       if (leader) {
 #pragma unroll
-        for (int s = 0; s < DK / 16; ++s)
-          mma_ss(COL_A, k_major(st, s), k_major(st + L::K_BYTES, s), idesc_bf16(64, 64, false, false), s > 0);
+        for (int s = 0; s < DK / 16; ++s) mma_ss(COL_A, k_major(q, s), k_major(k, s), idesc_bf16(64, 64, false, false), s > 0);
         commit(&B.a_full);
+        commit(&B.k_empty[i % KS]);
       }
       __syncwarp();
     };
     bool ok = tmem == 0;
-    if (!ok) record_error(A.err, SC_ERR_CUDA), *bail = 1;
-    if (WHOLE && n > 0 && ok && (ok = wait(&B.full[0], 0))) {
+    if (!ok) wait.gave_up();
+    if (n > 0 && ok && (ok = wait(&B.q_full[0], 0) && wait(&B.k_full[0], 0))) {
       fence_after();
       a_product(0);
     }
     for (int i = 0; i < n && ok; ++i) {
-      const int st = i % STAGES;
-      const uint8_t* stage = smem + st * L::STAGE;
-      const uint64_t vt = desc_mn(stage + 2 * L::K_BYTES, HALF);
-      if (WHOLE && i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
-        if (!(ok = wait(&B.full[(i + 1) % STAGES], (i + 1) / STAGES) && wait(&B.a_empty, i))) break;
+      const uint64_t vt = desc_mn(smem + L::V + i % VS * L::V_BYTES, HALF), kw = desc_mn(smem + L::KW, HALF);
+      if (i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
+        if (!(ok = wait(&B.q_full[(i + 1) % QS], (i + 1) / QS) && wait(&B.k_full[(i + 1) % KS], (i + 1) / KS) &&
+                   wait(&B.a_empty, i)))
+          break;
         fence_after();
         a_product(i + 1);
       }
-      if (!(ok = wait(&B.full[st], i / STAGES) && wait(&B.d_empty, i + 1))) break;
+      if (!(ok = wait(&B.v_full[i % VS], i / VS) && wait(&B.d_empty, i + 1))) break;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         if (!(ok = wait(&B.kw_full[hf], i))) break;
         fence_after();
         if (leader) {
-#pragma unroll
-          for (int term = 2; term >= 0; --term)  // the small ones first
-#pragma unroll
-            for (int s = 2 * hf; s < 2 * hf + 2; ++s)
-              mma_ss(COL_D, vt + 128 * s, desc_mn(smem + L::KW + term * L::K_BYTES, HALF) + 128 * s,
-                     idesc_bf16(128, DK, true, true), hf > 0 || term < 2 || s > 0);
+          add_products<DK>(COL_D, vt, kw, hf, hf == 0);
           commit(&B.kw_empty[hf]);
-          if (hf == 1) {
-            commit(&B.d_full);
-            if (!WHOLE) commit(&B.empty[st]);
-          }
+          if (hf == 1) commit(&B.d_full);
         }
         __syncwarp();
       }
       if (!ok) break;
-      if constexpr (WHOLE) {
-        if (!(ok = wait(&B.s_full, i) && wait(&B.o_empty, i + 1))) break;
-        fence_after();
-        if (leader) {
+      if (!(ok = wait(&B.s_full, i) && wait(&B.o_empty, i + 1))) break;
+      fence_after();
+      if (leader) {
+        const uint8_t* q = smem + L::Q + i % QS * L::K_BYTES;
 #pragma unroll
-          for (int term = 1; term >= 0; --term)
+        for (int term = 1; term >= 0; --term)
 #pragma unroll
-            for (int s = 0; s < DK / 16; ++s)
-              mma_ts(COL_X, COL_S + term * (DK / 2) + 8 * s, k_major(stage, s), idesc_bf16(128, 64, false, false),
-                     term < 1 || s > 0);
-          commit(&B.s_empty);
-        }
-        __syncwarp();
-        if (!(ok = wait(&B.p_full, i))) break;
-        fence_after();
-        if (leader) {
-#pragma unroll
-          for (int s = 0; s < C / 16; ++s)
-            mma_ss(COL_I, vt + 128 * s, desc_k(smem + L::P) + 2 * s, idesc_bf16(128, 64, true, false), s > 0);
-          commit(&B.o_full);
-          commit(&B.p_empty);
-          commit(&B.empty[st]);
-        }
-        __syncwarp();
+          for (int s = 0; s < DK / 16; ++s)
+            mma_ts(COL_X, COL_S + term * (DK / 2) + 8 * s, k_major(q, s), idesc_bf16(128, 64, false, false), term < 1 || s > 0);
+        commit(&B.s_empty);
+        commit(&B.q_empty[i % QS]);
       }
+      __syncwarp();
+      if (!(ok = wait(&B.p_full, i))) break;
+      fence_after();
+      if (leader) {
+#pragma unroll
+        for (int s = 0; s < C / 16; ++s)
+          mma_ss(COL_I, vt + 128 * s, desc_k(smem + L::P) + 2 * s, idesc_bf16(128, 64, true, false), s > 0);
+        commit(&B.o_full);
+        commit(&B.p_empty);
+        commit(&B.v_empty[i % VS]);
+      }
+      __syncwarp();
     }
     if (leader) {
       commit(&B.done);  // every product issued has finished
@@ -558,7 +750,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (warp == MMA_WARP) tmem_free(tmem);
 }
 
 // the states before the segments, in place of what the segments add: a thread a value
@@ -636,15 +828,17 @@ int run(const Args& A, cudaStream_t s) {
   const dim3 grid(unsigned(A.segments), unsigned(a.v_heads), unsigned(a.batch));
   constexpr int smem = Shape<DK>::BYTES;
   static_assert(smem <= 227 * 1024, "shared memory of a block");
-  if (int rc = raise_smem(reinterpret_cast<const void*>(chunk_kernel<DK, true>), smem, "linear attention smem attribute"))
+  if (int rc = raise_smem(reinterpret_cast<const void*>(chunk_kernel<DK>), smem, "linear attention smem attribute"))
     return rc;
   if (A.segments > 1) {
-    if (int rc = raise_smem(reinterpret_cast<const void*>(chunk_kernel<DK, false>), smem, "linear attention smem attribute"))
+    constexpr int add_smem = AddShape<DK>::BYTES;
+    static_assert(add_smem <= 227 * 1024, "shared memory of a block");
+    if (int rc = raise_smem(reinterpret_cast<const void*>(add_kernel<DK>), add_smem, "linear attention smem attribute"))
       return rc;
-    chunk_kernel<DK, false><<<dim3(grid.x - 1, grid.y, grid.z), THREADS, smem, s>>>(A, maps);
+    add_kernel<DK><<<dim3(grid.x - 1, grid.y, grid.z), THREADS, add_smem, s>>>(A, maps);
     scan_kernel<DK><<<dim3(unsigned(a.batch) * unsigned(a.v_heads), DK * 128 / 256), 256, 0, s>>>(A);
   }
-  chunk_kernel<DK, true><<<grid, THREADS, smem, s>>>(A, maps);
+  chunk_kernel<DK><<<grid, THREADS, smem, s>>>(A, maps);
   if (cudaError_t e = cudaGetLastError()) return cuda_failed(e, "linear attention launch");
   return SC_OK;
 }
