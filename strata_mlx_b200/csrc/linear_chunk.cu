@@ -15,7 +15,8 @@
 //   0-3    P from A                             4-7    the outputs, stored by TMA through a tile in shared memory
 //   8-15   the state (a lane a value dimension, half of k_dim each)
 //   16-19  w K, in halves of 32 tokens so that D's products run behind it; zeros over the values past a length
-//   20     one lane issues the products      21  the chunks' decays      22, 23  loads by TMA
+//   20     one lane issues A, X and I           21  the chunks' decays; loads of values
+//   22     loads of queries and keys            23  one lane issues D
 // Tensor memory: A, I, X, D and the two terms of S^T, 448 of 512 columns.
 //
 // One sequence's heads fill few SMs, so a long prompt is cut into segments: a first launch works out what each
@@ -44,7 +45,7 @@ constexpr int QS = 4, KS = 3, VS = 2;
 constexpr int RING = 4;      // chunks whose decays are held
 constexpr int HALF = C * 128;  // bytes of 64 columns of a chunk's rows
 constexpr int THREADS = 24 * 32;
-constexpr int OUT_WARP = 4, STATE_WARP = 8, KW_WARP = 16, MMA_WARP = 20, DECAY_WARP = 21, LOAD_WARP = 22, VALUE_WARP = 23;
+constexpr int OUT_WARP = 4, STATE_WARP = 8, KW_WARP = 16, MMA_WARP = 20, DECAY_WARP = 21, LOAD_WARP = 22, SUM_WARP = 23;
 // registers a thread: 80 at launch; the groups' shares add up to as many
 constexpr int P_REGS = 72, OUT_REGS = 72, STATE_REGS = 112, KW_REGS = 72, CONTROL_REGS = 40;
 static_assert(P_REGS + OUT_REGS + 2 * STATE_REGS + KW_REGS + CONTROL_REGS == 6 * 80, "a block's registers");
@@ -146,6 +147,18 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t& t0, uint32_t&
   t2 = bits_of(__floats2bfloat162_rn(x - lo_f(t1), y - hi_f(t1)));
 }
 
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {  // without waiting
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Waits, for a whole warp (all of its lanes go on, or none) and for one thread. Small in code, as there are many: the
 // warps' instructions have to fit the cache.
 struct Waits {
@@ -157,10 +170,23 @@ struct Waits {
     return false;
   }
   __device__ __forceinline__ bool operator()(uint64_t* bar, int phase) const {
-    const uint32_t parity = uint32_t(phase) & 1, start = uint32_t(clock());
+    const uint32_t parity = uint32_t(phase) & 1;
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const uint32_t start = uint32_t(clock());
     while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
       if (__any_sync(0xffffffffu, *bail || uint32_t(clock()) - start > 2000000000u)) return gave_up();
     return true;
+  }
+  // several barriers, their tests side by side: one test's latency where all are ready
+  __device__ __forceinline__ bool operator()(uint64_t* x, int px, uint64_t* y, int py) const {
+    const bool ready = mbar_test(x, uint32_t(px) & 1) & mbar_test(y, uint32_t(py) & 1);
+    if (__all_sync(0xffffffffu, ready)) return true;
+    return (*this)(x, px) && (*this)(y, py);
+  }
+  __device__ __forceinline__ bool operator()(uint64_t* x, int px, uint64_t* y, int py, uint64_t* z, int pz) const {
+    const bool ready = mbar_test(x, uint32_t(px) & 1) & mbar_test(y, uint32_t(py) & 1) & mbar_test(z, uint32_t(pz) & 1);
+    if (__all_sync(0xffffffffu, ready)) return true;
+    return (*this)(x, px) && (*this)(y, py) && (*this)(z, pz);
   }
   __device__ __forceinline__ bool alone(uint64_t* bar, int phase) const {
     const uint32_t parity = uint32_t(phase) & 1, start = uint32_t(clock());
@@ -261,8 +287,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
   if (warp < ADD_SUM_WARP) {
     for (int i = 0; i < n; ++i) {
       const int st = i % ADD_STAGES, m = len - chunk(i) * C;
-      if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.full[st], i / ADD_STAGES) || !wait(&B.kw_empty[i & 1], i / 2 + 1))
-        break;
+      if (!wait(&B.dec_full[i % RING], i / RING, &B.full[st], i / ADD_STAGES, &B.kw_empty[i & 1], i / 2 + 1)) break;
       const float* w = dec + i % RING * C;
       uint8_t* kw = smem + L::KW + (i & 1) * 3 * L::K_BYTES;
 #pragma unroll 2
@@ -350,7 +375,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
       for (int i = 0; i < n && ok; ++i) {
         const int st = i % ADD_STAGES, run = i / ADD_RUN;
         if (i % ADD_RUN == 0 && !(ok = wait(&B.d_empty[run & 1], run / 2 + 1))) break;
-        if (!(ok = wait(&B.full[st], i / ADD_STAGES) && wait(&B.kw_full[i & 1], i / 2))) break;
+        if (!(ok = wait(&B.full[st], i / ADD_STAGES, &B.kw_full[i & 1], i / 2))) break;
         fence_after();
         if (leader) {
           const uint64_t v = desc_mn(smem + st * L::STAGE + L::K_BYTES, HALF), kw = desc_mn(smem + L::KW + (i & 1) * 3 * L::K_BYTES, HALF);
@@ -391,13 +416,13 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   if (tid == 0) {
     for (int i = 0; i < QS; ++i) mbar_init(&B.q_full[i], 1), mbar_init(&B.q_empty[i], 1);
     for (int i = 0; i < KS; ++i) mbar_init(&B.k_full[i], 1), mbar_init(&B.k_empty[i], 4 + 1);
-    for (int i = 0; i < VS; ++i) mbar_init(&B.v_full[i], 1), mbar_init(&B.v_empty[i], 1);
+    for (int i = 0; i < VS; ++i) mbar_init(&B.v_full[i], 1), mbar_init(&B.v_empty[i], 2);
     for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], 20);
     mbar_init(&B.a_full, 1), mbar_init(&B.a_empty, 4), mbar_init(&B.p_full, 4), mbar_init(&B.p_empty, 1);
     mbar_init(&B.o_full, 1), mbar_init(&B.o_empty, 4);
     for (int i = 0; i < 2; ++i) mbar_init(&B.kw_full[i], 4), mbar_init(&B.kw_empty[i], 1);
     mbar_init(&B.d_full, 1), mbar_init(&B.d_empty, 8), mbar_init(&B.s_full, 8), mbar_init(&B.s_empty, 1);
-    mbar_init(&B.done, 1);
+    mbar_init(&B.done, 2);
     B.bail = 0;
     fence_mbar_init();
   }
@@ -420,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       const float shift = log2f(fabsf(a.scale));
       const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
       for (int i = 0; i < n; ++i) {
-        if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.a_full, i)) break;
+        if (!wait(&B.dec_full[i % RING], i / RING, &B.a_full, i)) break;
         fence_after();
         uint32_t r[32];
         ld_frag64(lanes + COL_A, r);
@@ -462,7 +487,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       // where this lane's rows of transposed fragments go: token (lane / 16) 8 + lane % 8 of 16, pieces of 8 values
       const int token = (lane >> 4) * 8 + (lane & 7), piece = 4 * (warp & 3) + ((lane >> 3) & 1);
       for (int i = 0; i < n; ++i) {
-        if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.o_full, i)) break;
+        if (!wait(&B.dec_full[i % RING], i / RING, &B.o_full, i)) break;
         fence_after();
         if (ot == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         out_sync();  // the tile's last store has read it
@@ -550,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     };
     if (n > 0) publish();
     for (int i = 0; i < n; ++i) {
-      if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.d_full, i)) break;
+      if (!wait(&B.dec_full[i % RING], i / RING, &B.d_full, i)) break;
       fence_after();
       const float d = dec[i % RING].a, one = dec[i % RING].one;
 #pragma unroll
@@ -582,7 +607,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     const int lt = tid - KW_WARP * 32;
     for (int i = 0; i < n; ++i) {
       const int m = len - (c0 + i) * C;
-      if (!wait(&B.dec_full[i % RING], i / RING) || !wait(&B.k_full[i % KS], i / KS)) break;
+      if (!wait(&B.dec_full[i % RING], i / RING, &B.k_full[i % KS], i / KS)) break;
       const uint8_t* k = smem + L::K + i % KS * L::K_BYTES;
       const float* w = dec[i % RING].w;
       if (m < C) {
@@ -611,7 +636,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     // ---- a chunk's decays: a lane tokens 2 lane and 2 lane + 1, sums from the front and from the back
     const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
     float2 next = two_decays(decay, a.decay_token, c0 * C, n ? len : 0);
-    for (int i = 0; i < n; ++i) {
+    auto decays = [&](int i) -> bool {
       const float g0 = next.x, g1 = next.y, pair = g0 + g1;
       if (i + 1 < n) next = two_decays(decay, a.decay_token, (c0 + i + 1) * C, len);
       float up = pair, down = pair;
@@ -627,7 +652,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       constexpr float LOG2E = 1.4426950408889634f;
       const float e0 = (before + g0) * LOG2E, e1 = up * LOG2E;
       Decays& D = dec[i % RING];
-      if (!wait(&B.dec_empty[i % RING], i / RING + 1)) break;
+      if (!wait(&B.dec_empty[i % RING], i / RING + 1)) return false;
       *reinterpret_cast<float2*>(&D.g2[2 * lane]) = make_float2(e0, e1);
       *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(exp2f(e0) * a.scale, exp2f(e1) * a.scale);
       *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(exp2f((after + g1) * LOG2E), exp2f(after * LOG2E));
@@ -636,7 +661,23 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         D.a = near ? expm1f(up) : expf(up), D.one = near ? 1.f : 0.f;
       }
       arrive(&B.dec_full[i % RING]);
+      return true;
+    };
+    const bool leader = elect_one();
+    int i = 0;  // the decays a chunk ahead of the values
+    for (bool ok = n == 0 || decays(0); ok && i < n; ++i) {
+      if (i + 1 < n && !decays(i + 1)) break;
+      if (!wait(&B.v_empty[i % VS], i / VS + 1)) break;
+      if (leader) {
+        mbar_arrive_expect_tx(&B.v_full[i % VS], (a.v_dim > 64 ? 2 : 1) * HALF);
+        for (int x = 0; x < a.v_dim; x += 64)
+          tma_load(smem + L::V + i % VS * L::V_BYTES + x / 64 * HALF, &maps.v, x, h, (c0 + i) * C, b, &B.v_full[i % VS]);
+      }
+      __syncwarp();
     }
+    if (leader)  // copies in flight land before the block may end
+      for (int k = max(0, i - VS); k < i; ++k) mbar_wait(&B.v_full[k % VS], uint32_t(k / VS) & 1, nullptr, 20000000LL);
+    __syncwarp();
   } else if (warp == LOAD_WARP) {
     // ---- keys and queries
     if (elect_one()) {
@@ -658,19 +699,30 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       for (int k = max(0, i - QS); k < i; ++k) mbar_wait(&B.q_full[k % QS], uint32_t(k / QS) & 1, nullptr, 20000000LL);
     }
     __syncwarp();
-  } else if (warp == VALUE_WARP) {
-    // ---- values
-    if (elect_one()) {
-      int i = 0;
-      for (; i < n; ++i) {
-        const int vs = i % VS;
-        if (!wait.alone(&B.v_empty[vs], i / VS + 1)) break;
-        mbar_arrive_expect_tx(&B.v_full[vs], (a.v_dim > 64 ? 2 : 1) * HALF);
-        for (int x = 0; x < a.v_dim; x += 64)
-          tma_load(smem + L::V + vs * L::V_BYTES + x / 64 * HALF, &maps.v, x, h, (c0 + i) * C, b, &B.v_full[vs]);
+  } else if (warp == SUM_WARP) {
+    // ---- D
+    const bool leader = elect_one();
+    const uint64_t kw = desc_mn(smem + L::KW, HALF);
+    for (int i = 0; i < n && tmem == 0; ++i) {
+      const uint64_t vt = desc_mn(smem + L::V + i % VS * L::V_BYTES, HALF);
+      if (!wait(&B.v_full[i % VS], i / VS, &B.d_empty, i + 1, &B.kw_full[0], i)) break;
+      fence_after();
+      if (leader) {
+        add_products<DK>(COL_D, vt, kw, 0, true);
+        commit(&B.kw_empty[0]);
       }
-      for (int k = max(0, i - VS); k < i; ++k) mbar_wait(&B.v_full[k % VS], uint32_t(k / VS) & 1, nullptr, 20000000LL);
+      __syncwarp();
+      if (!wait(&B.kw_full[1], i)) break;
+      fence_after();
+      if (leader) {
+        add_products<DK>(COL_D, vt, kw, 1, false);
+        commit(&B.d_full);
+        commit(&B.kw_empty[1]);
+        commit(&B.v_empty[i % VS]);
+      }
+      __syncwarp();
     }
+    if (leader) commit(&B.done);
     __syncwarp();
   } else if (warp == MMA_WARP) {
     // ---- the products. The whole warp follows the loop, so that what a product is given is uniform; one lane issues.
@@ -689,33 +741,19 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     };
     bool ok = tmem == 0;
     if (!ok) wait.gave_up();
-    if (n > 0 && ok && (ok = wait(&B.q_full[0], 0) && wait(&B.k_full[0], 0))) {
+    if (n > 0 && ok && (ok = wait(&B.q_full[0], 0, &B.k_full[0], 0))) {
       fence_after();
       a_product(0);
     }
     for (int i = 0; i < n && ok; ++i) {
-      const uint64_t vt = desc_mn(smem + L::V + i % VS * L::V_BYTES, HALF), kw = desc_mn(smem + L::KW, HALF);
+      const uint64_t vt = desc_mn(smem + L::V + i % VS * L::V_BYTES, HALF);
       if (i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
-        if (!(ok = wait(&B.q_full[(i + 1) % QS], (i + 1) / QS) && wait(&B.k_full[(i + 1) % KS], (i + 1) / KS) &&
-                   wait(&B.a_empty, i)))
-          break;
+        const int j = i + 1;
+        if (!(ok = wait(&B.q_full[j % QS], j / QS, &B.k_full[j % KS], j / KS, &B.a_empty, i))) break;
         fence_after();
-        a_product(i + 1);
+        a_product(j);
       }
-      if (!(ok = wait(&B.v_full[i % VS], i / VS) && wait(&B.d_empty, i + 1))) break;
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        if (!(ok = wait(&B.kw_full[hf], i))) break;
-        fence_after();
-        if (leader) {
-          add_products<DK>(COL_D, vt, kw, hf, hf == 0);
-          commit(&B.kw_empty[hf]);
-          if (hf == 1) commit(&B.d_full);
-        }
-        __syncwarp();
-      }
-      if (!ok) break;
-      if (!(ok = wait(&B.s_full, i) && wait(&B.o_empty, i + 1))) break;
+      if (!(ok = wait(&B.s_full, i, &B.o_empty, i + 1))) break;
       fence_after();
       if (leader) {
         const uint8_t* q = smem + L::Q + i % QS * L::K_BYTES;
@@ -728,7 +766,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         commit(&B.q_empty[i % QS]);
       }
       __syncwarp();
-      if (!(ok = wait(&B.p_full, i))) break;
+      if (!(ok = wait(&B.p_full, i, &B.v_full[i % VS], i / VS))) break;
+      if (len - (c0 + i) * C < C && !(ok = wait(&B.kw_full[0], i))) break;  // the last chunk's values are cleared
       fence_after();
       if (leader) {
 #pragma unroll
