@@ -147,51 +147,39 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t& t0, uint32_t&
   t2 = bits_of(__floats2bfloat162_rn(x - lo_f(t1), y - hi_f(t1)));
 }
 
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {  // without waiting
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
 // Waits, for a whole warp (all of its lanes go on, or none) and for one thread. Small in code, as there are many: the
 // warps' instructions have to fit the cache.
 struct Waits {
-  int* err;
-  volatile int* bail;
-  __device__ __forceinline__ bool gave_up() const {
-    record_error(err, SC_ERR_TIMEOUT);
+  volatile int* bail;  // the block's; whoever finds it set stops waiting, and a thread records the error at the end
+  __device__ __forceinline__ bool over(uint32_t start) const { return *bail || uint32_t(clock()) - start > 2000000000u; }
+  __device__ __forceinline__ bool stop() const {
     *bail = 1;
     return false;
   }
-  __device__ __forceinline__ bool operator()(uint64_t* bar, int phase) const {
-    const uint32_t parity = uint32_t(phase) & 1;
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  __device__ __forceinline__ bool operator()(uint64_t* x, int px) const {
     const uint32_t start = uint32_t(clock());
-    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
-      if (__any_sync(0xffffffffu, *bail || uint32_t(clock()) - start > 2000000000u)) return gave_up();
+    while (!__all_sync(0xffffffffu, mbar_try_wait(x, uint32_t(px) & 1)))
+      if (__any_sync(0xffffffffu, over(start))) return stop();
     return true;
   }
-  // several barriers, their tests side by side: one test's latency where all are ready
+  // several barriers side by side
   __device__ __forceinline__ bool operator()(uint64_t* x, int px, uint64_t* y, int py) const {
-    const bool ready = mbar_test(x, uint32_t(px) & 1) & mbar_test(y, uint32_t(py) & 1);
-    if (__all_sync(0xffffffffu, ready)) return true;
-    return (*this)(x, px) && (*this)(y, py);
+    const uint32_t start = uint32_t(clock());
+    while (!__all_sync(0xffffffffu, mbar_try_wait(x, uint32_t(px) & 1) & mbar_try_wait(y, uint32_t(py) & 1)))
+      if (__any_sync(0xffffffffu, over(start))) return stop();
+    return true;
   }
   __device__ __forceinline__ bool operator()(uint64_t* x, int px, uint64_t* y, int py, uint64_t* z, int pz) const {
-    const bool ready = mbar_test(x, uint32_t(px) & 1) & mbar_test(y, uint32_t(py) & 1) & mbar_test(z, uint32_t(pz) & 1);
-    if (__all_sync(0xffffffffu, ready)) return true;
-    return (*this)(x, px) && (*this)(y, py) && (*this)(z, pz);
+    const uint32_t start = uint32_t(clock());
+    while (!__all_sync(0xffffffffu, mbar_try_wait(x, uint32_t(px) & 1) & mbar_try_wait(y, uint32_t(py) & 1) &
+                                        mbar_try_wait(z, uint32_t(pz) & 1)))
+      if (__any_sync(0xffffffffu, over(start))) return stop();
+    return true;
   }
   __device__ __forceinline__ bool alone(uint64_t* bar, int phase) const {
-    const uint32_t parity = uint32_t(phase) & 1, start = uint32_t(clock());
-    while (!mbar_try_wait(bar, parity))
-      if (*bail || uint32_t(clock()) - start > 2000000000u) return gave_up();
+    const uint32_t start = uint32_t(clock());
+    while (!mbar_try_wait(bar, uint32_t(phase) & 1))
+      if (over(start)) return stop();
     return true;
   }
 };
@@ -224,12 +212,14 @@ __device__ __forceinline__ void split_piece(const uint8_t* k, float w, bool in, 
 
 // values past the length meet zeros of P and w K, which a NaN would spoil: zeros in their place, by `step` threads
 __device__ __forceinline__ void clear_values(uint8_t* v, int m, int thread, int step) {
+#pragma unroll 1
   for (int j = thread; j < 2 * HALF / 16; j += step)
     if ((j * 16 % HALF) / 128 >= m) *reinterpret_cast<uint4*>(v + 16 * j) = make_uint4(0, 0, 0, 0);
 }
 
 // the second half of the values is not loaded where there are 64 or fewer: zeros
 __device__ __forceinline__ void clear_halves(uint8_t* v, int n, int apart) {
+#pragma unroll 1
   for (int i = threadIdx.x; i < n * HALF / 16; i += THREADS)
     *reinterpret_cast<uint4*>(v + i / (HALF / 16) * apart + HALF + 16 * (i % (HALF / 16))) = make_uint4(0, 0, 0, 0);
   fence_async();
@@ -282,9 +272,10 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
   __syncthreads();
   fence_after();
   const uint32_t tmem = B.tmem;
-  const Waits wait{A.err, &B.bail};
+  const Waits wait{&B.bail};
   auto chunk = [&](int i) { return c0 + n - 1 - i; };  // the last first
   if (warp < ADD_SUM_WARP) {
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
       const int st = i % ADD_STAGES, m = len - chunk(i) * C;
       if (!wait(&B.dec_full[i % RING], i / RING, &B.full[st], i / ADD_STAGES, &B.kw_empty[i & 1], i / 2 + 1)) break;
@@ -310,6 +301,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
     float S[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) S[k] = 0.f;
+#pragma unroll 1
     for (int r = 0; r * ADD_RUN < n; ++r) {
       if (!wait(&B.d_full[r & 1], r / 2)) break;
       fence_after();
@@ -334,6 +326,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
       float later = 0.f;  // the decays of the chunks behind this one
       float2 next = n ? two_decays(decay, a.decay_token, chunk(0) * C, len) : make_float2(0.f, 0.f);
       bool ok = true;
+#pragma unroll 1
       for (int i = 0; i < n; ++i) {
         const float2 g = next;
         if (i + 1 < n) next = two_decays(decay, a.decay_token, chunk(i + 1) * C, len);
@@ -356,22 +349,27 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
       if (elect_one()) {
         const uint32_t bytes = uint32_t(L::K_BYTES + (a.v_dim > 64 ? 2 : 1) * HALF);
         int i = 0;
+#pragma unroll 1
         for (; i < n; ++i) {
           const int st = i % ADD_STAGES, t0 = chunk(i) * C;
           if (!wait.alone(&B.empty[st], i / ADD_STAGES + 1)) break;
           uint8_t* stage = smem + st * L::STAGE;
           mbar_arrive_expect_tx(&B.full[st], bytes);
+#pragma unroll 1
           for (int x = 0; x < DK; x += 64) tma_load(stage + x / 64 * HALF, &maps.k, x, hk, t0, b, &B.full[st]);
+#pragma unroll 1
           for (int x = 0; x < a.v_dim; x += 64) tma_load(stage + L::K_BYTES + x / 64 * HALF, &maps.v, x, h, t0, b, &B.full[st]);
         }
         // copies in flight land before the block may end
+#pragma unroll 1
         for (int k = max(0, i - ADD_STAGES); k < i; ++k)
           mbar_wait(&B.full[k % ADD_STAGES], uint32_t(k / ADD_STAGES) & 1, nullptr, 20000000LL);
       }
     } else if (warp == MMA_WARP) {
       const bool leader = elect_one();
       bool ok = tmem == 0;  // all 512 columns are this block's
-      if (!ok) wait.gave_up();
+      if (!ok) wait.stop();
+#pragma unroll 1
       for (int i = 0; i < n && ok; ++i) {
         const int st = i % ADD_STAGES, run = i / ADD_RUN;
         if (i % ADD_RUN == 0 && !(ok = wait(&B.d_empty[run & 1], run / 2 + 1))) break;
@@ -397,6 +395,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
   fence_before();
   __syncthreads();
   fence_after();
+  if (tid == 0 && B.bail) record_error(A.err, SC_ERR_TIMEOUT);
   if (warp == MMA_WARP) tmem_free(tmem);
 }
 
@@ -432,7 +431,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   __syncthreads();
   fence_after();
   const uint32_t tmem = B.tmem;
-  const Waits wait{A.err, &B.bail};
+  const Waits wait{&B.bail};
   const uint32_t quarter = uint32_t(warp & 3) * 32, lanes = tmem + (quarter << 16);
 
   if (warp < STATE_WARP) {
@@ -444,6 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       // the scale goes with the decays: 2^(G_i + log2 |scale| - G_j), its sign last
       const float shift = log2f(fabsf(a.scale));
       const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll 1
       for (int i = 0; i < n; ++i) {
         if (!wait(&B.dec_full[i % RING], i / RING, &B.a_full, i)) break;
         fence_after();
@@ -486,6 +486,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       uint8_t* tile = smem + L::OUT;
       // where this lane's rows of transposed fragments go: token (lane / 16) 8 + lane % 8 of 16, pieces of 8 values
       const int token = (lane >> 4) * 8 + (lane & 7), piece = 4 * (warp & 3) + ((lane >> 3) & 1);
+#pragma unroll 1
       for (int i = 0; i < n; ++i) {
         if (!wait(&B.dec_full[i % RING], i / RING, &B.o_full, i)) break;
         fence_after();
@@ -536,6 +537,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       }
       // zeros past the last chunk with tokens, 16 bytes at a time
       const int t1 = (c0 + n) * C, pieces = a.v_dim / 8, rows = max(0, min(a.tokens, c1 * C) - t1);
+#pragma unroll 1
       for (int e = ot; e < rows * pieces; e += 128)
         *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) +
                                   ((int64_t(b) * a.tokens + t1 + e / pieces) * a.v_heads + h) * a.v_dim + 8 * (e % pieces)) =
@@ -549,13 +551,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     const int dv = int(quarter) + lane, k0 = (warp - STATE_WARP) / 4 * N;
     float S[N];
     const int64_t head = int64_t(b) * a.v_heads + h;
-    const bool started = A.segments > 1;
-    const float* from = started ? A.parts + (head * A.segments + seg) * DK * 128 + dv
-                                : a.state_in + head * a.k_dim * a.v_dim + dv;
-    const int ld = started ? 128 : a.v_dim;
+    const bool started = A.segments > 1, there = started || (a.state_in && dv < a.v_dim);
+    const float* from = started ? A.parts + ((head * A.segments + seg) * DK + k0) * 128 + dv
+                                : a.state_in + (head * a.k_dim + k0) * a.v_dim + dv;
+    const int kd = started ? DK : a.k_dim, ld = started ? 128 : a.v_dim;
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      S[k] = started || (a.state_in && dv < a.v_dim && k0 + k < a.k_dim) ? from[int64_t(k0 + k) * ld] : 0.f;
+    for (int k = 0; k < N; ++k, from += ld) S[k] = there && k0 + k < kd ? *from : 0.f;
     auto publish = [&] {  // S^T as two terms, the A operand of X
 #pragma unroll
       for (int k = 0; k < N; k += 16) {
@@ -573,8 +574,13 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       fence_before();
       arrive(&B.s_full);
     };
-    if (n > 0) publish();
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
+      if (i > 0) {
+        if (!wait(&B.s_empty, i - 1)) break;
+        fence_after();
+      }
+      publish();
       if (!wait(&B.dec_full[i % RING], i / RING, &B.d_full, i)) break;
       fence_after();
       const float d = dec[i % RING].a, one = dec[i % RING].one;
@@ -589,22 +595,19 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       fence_before();
       arrive(&B.d_empty);
       arrive(&B.dec_empty[i % RING]);
-      if (i + 1 < n) {
-        if (!wait(&B.s_empty, i)) break;
-        fence_after();
-        publish();
-      }
     }
     if (seg == A.segments - 1) {
-      float* to = a.state_out + head * a.k_dim * a.v_dim + dv;
+      float* to = a.state_out + (head * a.k_dim + k0) * a.v_dim + dv;
+      const int kd = dv < a.v_dim ? a.k_dim - k0 : 0;
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (dv < a.v_dim && k0 + k < a.k_dim) to[int64_t(k0 + k) * a.v_dim] = S[k];
+      for (int k = 0; k < N; ++k, to += a.v_dim)
+        if (k < kd) *to = S[k];
     }
   } else if (warp < MMA_WARP) {
     // ---- w K
     fewer_registers<KW_REGS>();
     const int lt = tid - KW_WARP * 32;
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
       const int m = len - (c0 + i) * C;
       if (!wait(&B.dec_full[i % RING], i / RING, &B.k_full[i % KS], i / KS)) break;
@@ -664,38 +667,47 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       return true;
     };
     const bool leader = elect_one();
-    int i = 0;  // the decays a chunk ahead of the values
-    for (bool ok = n == 0 || decays(0); ok && i < n; ++i) {
+    int i = -1;  // the decays a chunk ahead of the values
+#pragma unroll 1
+    for (; i < n; ++i) {
       if (i + 1 < n && !decays(i + 1)) break;
+      if (i < 0) continue;
       if (!wait(&B.v_empty[i % VS], i / VS + 1)) break;
       if (leader) {
         mbar_arrive_expect_tx(&B.v_full[i % VS], (a.v_dim > 64 ? 2 : 1) * HALF);
+#pragma unroll 1
         for (int x = 0; x < a.v_dim; x += 64)
           tma_load(smem + L::V + i % VS * L::V_BYTES + x / 64 * HALF, &maps.v, x, h, (c0 + i) * C, b, &B.v_full[i % VS]);
       }
       __syncwarp();
     }
     if (leader)  // copies in flight land before the block may end
+#pragma unroll 1
       for (int k = max(0, i - VS); k < i; ++k) mbar_wait(&B.v_full[k % VS], uint32_t(k / VS) & 1, nullptr, 20000000LL);
     __syncwarp();
   } else if (warp == LOAD_WARP) {
     // ---- keys and queries
     if (elect_one()) {
       int i = 0;
+#pragma unroll 1
       for (; i < n; ++i) {
         const int t0 = (c0 + i) * C, ks = i % KS, qs = i % QS;
         if (!wait.alone(&B.k_empty[ks], i / KS + 1)) break;
         mbar_arrive_expect_tx(&B.k_full[ks], L::K_BYTES);
+#pragma unroll 1
         for (int x = 0; x < DK; x += 64) tma_load(smem + L::K + ks * L::K_BYTES + x / 64 * HALF, &maps.k, x, hk, t0, b, &B.k_full[ks]);
         if (!wait.alone(&B.q_empty[qs], i / QS + 1)) {
           mbar_wait(&B.k_full[ks], uint32_t(i / KS) & 1, nullptr, 20000000LL);
           break;
         }
         mbar_arrive_expect_tx(&B.q_full[qs], L::K_BYTES);
+#pragma unroll 1
         for (int x = 0; x < DK; x += 64) tma_load(smem + L::Q + qs * L::K_BYTES + x / 64 * HALF, &maps.q, x, hk, t0, b, &B.q_full[qs]);
       }
       // copies in flight land before the block may end
+#pragma unroll 1
       for (int k = max(0, i - KS); k < i; ++k) mbar_wait(&B.k_full[k % KS], uint32_t(k / KS) & 1, nullptr, 20000000LL);
+#pragma unroll 1
       for (int k = max(0, i - QS); k < i; ++k) mbar_wait(&B.q_full[k % QS], uint32_t(k / QS) & 1, nullptr, 20000000LL);
     }
     __syncwarp();
@@ -703,6 +715,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     // ---- D
     const bool leader = elect_one();
     const uint64_t kw = desc_mn(smem + L::KW, HALF);
+#pragma unroll 1
     for (int i = 0; i < n && tmem == 0; ++i) {
       const uint64_t vt = desc_mn(smem + L::V + i % VS * L::V_BYTES, HALF);
       if (!wait(&B.v_full[i % VS], i / VS, &B.d_empty, i + 1, &B.kw_full[0], i)) break;
@@ -740,11 +753,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       __syncwarp();
     };
     bool ok = tmem == 0;
-    if (!ok) wait.gave_up();
+    if (!ok) wait.stop();
     if (n > 0 && ok && (ok = wait(&B.q_full[0], 0, &B.k_full[0], 0))) {
       fence_after();
       a_product(0);
     }
+#pragma unroll 1
     for (int i = 0; i < n && ok; ++i) {
       const uint64_t vt = desc_mn(smem + L::V + i % VS * L::V_BYTES, HALF);
       if (i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
@@ -789,6 +803,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   fence_before();
   __syncthreads();
   fence_after();
+  if (tid == 0 && B.bail) record_error(A.err, SC_ERR_TIMEOUT);
   if (warp == MMA_WARP) tmem_free(tmem);
 }
 
