@@ -17,7 +17,7 @@
 //   16-19  w K, in halves of 32 tokens so that D's products run behind it; zeros over the values past a length
 //   20     one lane issues A, X and I           21  the chunks' decays; loads of values
 //   22     loads of queries and keys            23  one lane issues D
-// Tensor memory: A, I, X, D and the two terms of S^T, 448 of 512 columns.
+// Tensor memory: A, I, two of X, D and the two terms of S^T, all 512 columns.
 //
 // One sequence's heads fill few SMs, so a long prompt is cut into segments: a first launch works out what each
 // segment adds to the state, a second adds up the states before the segments, a third is the whole. The first takes a
@@ -57,7 +57,8 @@ constexpr int SMS = 148;
 constexpr float LEAST = -30.f;  // a token's decay below e^-30 is taken as e^-30: past it nothing is left in float32
 
 // tensor memory columns
-constexpr uint32_t COL_A = 0, COL_I = 64, COL_X = 128, COL_D = 192, COL_S = 320;
+constexpr uint32_t COL_A = 0, COL_I = 64, COL_D = 192, COL_S = 320;
+__device__ __forceinline__ uint32_t col_x(int i) { return i & 1 ? 448 : 128; }  // of chunk i: two, taken in turn
 
 struct Decays {
   float g2[C], eg[C], w[C];  // G_i log2(e), scale e^{G_i}, e^{G_63 - G_i}
@@ -498,7 +499,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         for (int q = 0; q < 4; ++q) {  // 16 value dimensions by 32 tokens at a time
           const int hf = q >> 1, j0 = 4 * (q & 1);
           uint32_t x[16], y[16];
-          ld_frag32(lanes + (uint32_t(16 * hf) << 16) + COL_X + 8 * j0, x);
+          ld_frag32(lanes + (uint32_t(16 * hf) << 16) + col_x(i) + 8 * j0, x);
           ld_frag32(lanes + (uint32_t(16 * hf) << 16) + COL_I + 8 * j0, y);
           wait_ld();
           if (q == 3) {
@@ -767,7 +768,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         fence_after();
         a_product(j);
       }
-      if (!(ok = wait(&B.s_full, i, &B.o_empty, i + 1))) break;
+      if (!(ok = wait(&B.s_full, i))) break;
       fence_after();
       if (leader) {
         const uint8_t* q = smem + L::Q + i % QS * L::K_BYTES;
@@ -775,12 +776,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         for (int term = 1; term >= 0; --term)
 #pragma unroll
           for (int s = 0; s < DK / 16; ++s)
-            mma_ts(COL_X, COL_S + term * (DK / 2) + 8 * s, k_major(q, s), idesc_bf16(128, 64, false, false), term < 1 || s > 0);
+            mma_ts(col_x(i), COL_S + term * (DK / 2) + 8 * s, k_major(q, s), idesc_bf16(128, 64, false, false), term < 1 || s > 0);
         commit(&B.s_empty);
         commit(&B.q_empty[i % QS]);
       }
       __syncwarp();
-      if (!(ok = wait(&B.p_full, i, &B.v_full[i % VS], i / VS))) break;
+      if (!(ok = wait(&B.p_full, i, &B.v_full[i % VS], i / VS, &B.o_empty, i + 1))) break;
       if (len - (c0 + i) * C < C && !(ok = wait(&B.kw_full[0], i))) break;  // the last chunk's values are cleared
       fence_after();
       if (leader) {
