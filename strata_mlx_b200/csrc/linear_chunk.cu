@@ -133,19 +133,38 @@ __device__ __forceinline__ float hi_f(uint32_t v) { return __uint_as_float(v & 0
 
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-// 2^x to 2^-22 of it, as P is rounded to eight bits
+// 2^x to 2^-22 of it, zero below 2^-126: P is rounded to eight bits, and a token's weight carries no further
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
+// e^x - 1 for x in [-ln 2, 0], by its series to x^10 / 10!: within 2^-29 of it
+__device__ __forceinline__ float expm1_near(float x) {
+  float y = 1.f / 3628800.f;
+  y = fmaf(y, x, 1.f / 362880.f);
+  y = fmaf(y, x, 1.f / 40320.f);
+  y = fmaf(y, x, 1.f / 5040.f);
+  y = fmaf(y, x, 1.f / 720.f);
+  y = fmaf(y, x, 1.f / 120.f);
+  y = fmaf(y, x, 1.f / 24.f);
+  y = fmaf(y, x, 1.f / 6.f);
+  y = fmaf(y, x, 0.5f);
+  return fmaf(y * x, x, x);
+}
+
+__device__ __forceinline__ float2 unpacked(uint32_t v) { return make_float2(lo_f(v), hi_f(v)); }
+__device__ __forceinline__ uint32_t rounded(float2 v) { return bits_of(__floats2bfloat162_rn(v.x, v.y)); }
+// two values less their bfloat16 roundings, exactly
+__device__ __forceinline__ float2 rest(float2 v, uint32_t r) { return __ffma2_rn(unpacked(r), make_float2(-1.f, -1.f), v); }
+
 // the three bfloat16 terms of two float32 values
-__device__ __forceinline__ void split3(float x, float y, uint32_t& t0, uint32_t& t1, uint32_t& t2) {
-  t0 = bits_of(__floats2bfloat162_rn(x, y));
-  x -= lo_f(t0), y -= hi_f(t0);
-  t1 = bits_of(__floats2bfloat162_rn(x, y));
-  t2 = bits_of(__floats2bfloat162_rn(x - lo_f(t1), y - hi_f(t1)));
+__device__ __forceinline__ void split3(float2 v, uint32_t& t0, uint32_t& t1, uint32_t& t2) {
+  t0 = rounded(v);
+  v = rest(v, t0);
+  t1 = rounded(v);
+  t2 = rounded(rest(v, t1));
 }
 
 // Waits, for a whole warp (all of its lanes go on, or none) and for one thread. Small in code, as there are many: the
@@ -201,11 +220,12 @@ __device__ __forceinline__ void tmem_free(uint32_t at) {
 __device__ __forceinline__ void split_piece(const uint8_t* k, float w, bool in, uint8_t* to, int term) {
   uint4 x = *reinterpret_cast<const uint4*>(k);
   if (!in) x = make_uint4(0, 0, 0, 0);
+  const float2 w2 = make_float2(w, w);
   uint4 t0, t1, t2;
-  split3(lo_f(x.x) * w, hi_f(x.x) * w, t0.x, t1.x, t2.x);
-  split3(lo_f(x.y) * w, hi_f(x.y) * w, t0.y, t1.y, t2.y);
-  split3(lo_f(x.z) * w, hi_f(x.z) * w, t0.z, t1.z, t2.z);
-  split3(lo_f(x.w) * w, hi_f(x.w) * w, t0.w, t1.w, t2.w);
+  split3(__fmul2_rn(unpacked(x.x), w2), t0.x, t1.x, t2.x);
+  split3(__fmul2_rn(unpacked(x.y), w2), t0.y, t1.y, t2.y);
+  split3(__fmul2_rn(unpacked(x.z), w2), t0.z, t1.z, t2.z);
+  split3(__fmul2_rn(unpacked(x.w), w2), t0.w, t1.w, t2.w);
   *reinterpret_cast<uint4*>(to) = t0;
   *reinterpret_cast<uint4*>(to + term) = t1;
   *reinterpret_cast<uint4*>(to + 2 * term) = t2;
@@ -226,15 +246,16 @@ __device__ __forceinline__ void clear_halves(uint8_t* v, int n, int apart) {
   fence_async();
 }
 
-// D += V^T (w K): the half `hf` of the tokens, the small terms first
+// D += V^T (w K): the half `hf` of the tokens, the small terms first. Here and below two to four products an iteration:
+// their issue keeps ahead of the tensor cores, and the code stays small.
 template <int DK>
 __device__ __forceinline__ void add_products(uint32_t d, uint64_t v, uint64_t kw, int hf, bool first) {
-#pragma unroll
-  for (int term = 2; term >= 0; --term)
-#pragma unroll
-    for (int s = 2 * hf; s < 2 * hf + 2; ++s)
-      mma_ss(d, v + 128 * s, kw + uint32_t(term * (DK / 64) * (HALF >> 4) + 128 * s), idesc_bf16(128, DK, true, true),
-             !first || term < 2 || s > 2 * hf);
+  v += 256 * hf, kw += 256 * hf + uint32_t(2 * (DK / 64) * (HALF >> 4));
+#pragma unroll 1
+  for (int term = 2; term >= 0; --term, kw -= uint32_t(DK / 64 * (HALF >> 4))) {
+    mma_ss(d, v, kw, idesc_bf16(128, DK, true, true), !first || term < 2);
+    mma_ss(d, v + 128, kw + 128, idesc_bf16(128, DK, true, true), true);
+  }
 }
 
 // a lane's two decays of a chunk: tokens 2 lane and 2 lane + 1 from t0 on
@@ -248,7 +269,8 @@ template <int DK>
 __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__ Args A, const __grid_constant__ Maps maps) {
   using L = AddShape<DK>;
   extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  // 1024-byte aligned, by an offset: through an integer the pointer would no longer be known to be shared memory's
+  uint8_t* smem = raw + (0u - smem_u32(raw) & 1023u);
   float* dec = reinterpret_cast<float*>(smem + L::DEC);  // (RING, C) weights
   AddBars& B = *reinterpret_cast<AddBars*>(smem + L::BARS);
   const sc_linear& a = A.a;
@@ -324,6 +346,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
     fewer_registers<CONTROL_REGS>();
     if (warp == DECAY_WARP) {
       const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
+      constexpr float LOG2E = 1.4426950408889634f;
       float later = 0.f;  // the decays of the chunks behind this one
       float2 next = n ? two_decays(decay, a.decay_token, chunk(0) * C, len) : make_float2(0.f, 0.f);
       bool ok = true;
@@ -341,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
         if (lane == 31) after = 0.f;
         after += later;
         if (!(ok = wait(&B.dec_empty[i % RING], i / RING + 1))) break;
-        *reinterpret_cast<float2*>(dec + i % RING * C + 2 * lane) = make_float2(expf(after + g.y), expf(after));
+        *reinterpret_cast<float2*>(dec + i % RING * C + 2 * lane) = make_float2(fast_exp2((after + g.y) * LOG2E), fast_exp2(after * LOG2E));
         later += __shfl_sync(0xffffffffu, down, 0);
         arrive(&B.dec_full[i % RING]);
       }
@@ -404,7 +427,8 @@ template <int DK>
 __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant__ Args A, const __grid_constant__ Maps maps) {
   using L = Shape<DK>;
   extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  // 1024-byte aligned, by an offset: through an integer the pointer would no longer be known to be shared memory's
+  uint8_t* smem = raw + (0u - smem_u32(raw) & 1023u);
   Decays* dec = reinterpret_cast<Decays*>(smem + L::DEC);
   Bars& B = *reinterpret_cast<Bars*>(smem + L::BARS);
   const sc_linear& a = A.a;
@@ -513,15 +537,17 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
             for (int e = 0; e < 2; ++e) {
               const int k = 4 * (j + e), col = 8 * (j0 + j + e) + 2 * t;
               const float2 s = *reinterpret_cast<const float2*>(eg + col);
-              float o[4];
+              float2 o[2];
 #pragma unroll
-              for (int r = 0; r < 4; ++r) o[r] = fmaf(r & 1 ? s.y : s.x, __uint_as_float(x[k + r]), __uint_as_float(y[k + r]));
+              for (int r = 0; r < 2; ++r)
+                o[r] = __ffma2_rn(s, make_float2(__uint_as_float(x[k + 2 * r]), __uint_as_float(x[k + 2 * r + 1])),
+                                  make_float2(__uint_as_float(y[k + 2 * r]), __uint_as_float(y[k + 2 * r + 1])));
               if (m < C) {  // zeros past the length
-                if (col >= m) o[0] = o[2] = 0.f;
-                if (col + 1 >= m) o[1] = o[3] = 0.f;
+                if (col >= m) o[0].x = o[1].x = 0.f;
+                if (col + 1 >= m) o[0].y = o[1].y = 0.f;
               }
-              f[2 * e] = bits_of(__floats2bfloat162_rn(o[0], o[1]));
-              f[2 * e + 1] = bits_of(__floats2bfloat162_rn(o[2], o[3]));
+              f[2 * e] = rounded(o[0]);
+              f[2 * e + 1] = rounded(o[1]);
             }
             const int row = 8 * (j0 + j) + token, pc = piece + 2 * hf;
             store_transposed(smem_u32(tile) + (pc >> 3) * HALF + row * 128 + (((pc & 7) ^ (row & 7)) << 4), f[0], f[1], f[2], f[3]);
@@ -550,23 +576,27 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     constexpr int N = DK / 2;
     more_registers<STATE_REGS>();
     const int dv = int(quarter) + lane, k0 = (warp - STATE_WARP) / 4 * N;
-    float S[N];
+    float2 S[N / 2];
     const int64_t head = int64_t(b) * a.v_heads + h;
     const bool started = A.segments > 1, there = started || (a.state_in && dv < a.v_dim);
     const float* from = started ? A.parts + ((head * A.segments + seg) * DK + k0) * 128 + dv
                                 : a.state_in + (head * a.k_dim + k0) * a.v_dim + dv;
     const int kd = started ? DK : a.k_dim, ld = started ? 128 : a.v_dim;
 #pragma unroll
-    for (int k = 0; k < N; ++k, from += ld) S[k] = there && k0 + k < kd ? *from : 0.f;
+    for (int k = 0; k < N / 2; ++k) {
+      S[k].x = there && k0 + 2 * k < kd ? *from : 0.f;
+      from += ld;
+      S[k].y = there && k0 + 2 * k + 1 < kd ? *from : 0.f;
+      from += ld;
+    }
     auto publish = [&] {  // S^T as two terms, the A operand of X
 #pragma unroll
       for (int k = 0; k < N; k += 16) {
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float x = S[k + 2 * e], y = S[k + 2 * e + 1];
-          hi[e] = bits_of(__floats2bfloat162_rn(x, y));
-          lo[e] = bits_of(__floats2bfloat162_rn(x - lo_f(hi[e]), y - hi_f(hi[e])));
+          hi[e] = rounded(S[k / 2 + e]);
+          lo[e] = rounded(rest(S[k / 2 + e], hi[e]));
         }
         st8(lanes + COL_S + (k0 + k) / 2, hi);
         st8(lanes + COL_S + DK / 2 + (k0 + k) / 2, lo);
@@ -584,14 +614,17 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       publish();
       if (!wait(&B.dec_full[i % RING], i / RING, &B.d_full, i)) break;
       fence_after();
-      const float d = dec[i % RING].a, one = dec[i % RING].one;
+      const float2 d = make_float2(dec[i % RING].a, dec[i % RING].a), one = make_float2(dec[i % RING].one, dec[i % RING].one);
 #pragma unroll
       for (int k = 0; k < N; k += 16) {
         uint32_t r[16];
         ld16(lanes + COL_D + k0 + k, r);
         wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) S[k + e] = fmaf(d, S[k + e], fmaf(one, S[k + e], __uint_as_float(r[e])));
+        for (int e = 0; e < 8; ++e) {
+          float2& x = S[k / 2 + e];
+          x = __ffma2_rn(d, x, __ffma2_rn(one, x, make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]))));
+        }
       }
       fence_before();
       arrive(&B.d_empty);
@@ -601,8 +634,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       float* to = a.state_out + (head * a.k_dim + k0) * a.v_dim + dv;
       const int kd = dv < a.v_dim ? a.k_dim - k0 : 0;
 #pragma unroll
-      for (int k = 0; k < N; ++k, to += a.v_dim)
-        if (k < kd) *to = S[k];
+      for (int k = 0; k < N / 2; ++k) {
+        if (2 * k < kd) *to = S[k].x;
+        to += a.v_dim;
+        if (2 * k + 1 < kd) *to = S[k].y;
+        to += a.v_dim;
+      }
     }
   } else if (warp < MMA_WARP) {
     // ---- w K
@@ -658,11 +695,11 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       Decays& D = dec[i % RING];
       if (!wait(&B.dec_empty[i % RING], i / RING + 1)) return false;
       *reinterpret_cast<float2*>(&D.g2[2 * lane]) = make_float2(e0, e1);
-      *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(exp2f(e0) * a.scale, exp2f(e1) * a.scale);
-      *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(exp2f((after + g1) * LOG2E), exp2f(after * LOG2E));
+      *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(fast_exp2(e0) * a.scale, fast_exp2(e1) * a.scale);
+      *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(fast_exp2((after + g1) * LOG2E), fast_exp2(after * LOG2E));
       if (lane == 31) {
         const bool near = up > -0.69314718f;
-        D.a = near ? expm1f(up) : expf(up), D.one = near ? 1.f : 0.f;
+        D.a = near ? expm1_near(up) : fast_exp2(e1), D.one = near ? 1.f : 0.f;
       }
       arrive(&B.dec_full[i % RING]);
       return true;
@@ -742,12 +779,14 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     // ---- the products. The whole warp follows the loop, so that what a product is given is uniform; one lane issues.
     // All 512 columns are this block's, so tensor memory starts at address 0.
     const bool leader = elect_one();
-    auto k_major = [&](const uint8_t* p, int s) { return desc_k(p) + uint32_t((s >> 2) * (HALF >> 4) + 2 * (s & 3)); };
     auto a_product = [&](int i) {
       const uint8_t *q = smem + L::Q + i % QS * L::K_BYTES, *k = smem + L::K + i % KS * L::K_BYTES;
       if (leader) {
+        uint64_t qd = desc_k(q), kd = desc_k(k);
+#pragma unroll 1
+        for (int x = 0; x < DK / 64; ++x, qd += HALF >> 4, kd += HALF >> 4)
 #pragma unroll
-        for (int s = 0; s < DK / 16; ++s) mma_ss(COL_A, k_major(q, s), k_major(k, s), idesc_bf16(64, 64, false, false), s > 0);
+          for (int s = 0; s < 4; ++s) mma_ss(COL_A, qd + 2 * s, kd + 2 * s, idesc_bf16(64, 64, false, false), x > 0 || s > 0);
         commit(&B.a_full);
         commit(&B.k_empty[i % KS]);
       }
@@ -771,12 +810,15 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       if (!(ok = wait(&B.s_full, i))) break;
       fence_after();
       if (leader) {
-        const uint8_t* q = smem + L::Q + i % QS * L::K_BYTES;
+        const uint64_t qd = desc_k(smem + L::Q + i % QS * L::K_BYTES);
+#pragma unroll 1
+        for (int e = 2 * (DK / 64) - 1; e >= 0; --e) {  // the rest, then the rounded state; 64 key dimensions each
+          const int x = e % (DK / 64);
 #pragma unroll
-        for (int term = 1; term >= 0; --term)
-#pragma unroll
-          for (int s = 0; s < DK / 16; ++s)
-            mma_ts(col_x(i), COL_S + term * (DK / 2) + 8 * s, k_major(q, s), idesc_bf16(128, 64, false, false), term < 1 || s > 0);
+          for (int s = 0; s < 4; ++s)
+            mma_ts(col_x(i), COL_S + 32 * e + 8 * s, qd + uint32_t(x * (HALF >> 4) + 2 * s), idesc_bf16(128, 64, false, false),
+                   e < 2 * (DK / 64) - 1 || s > 0);
+        }
         commit(&B.s_empty);
         commit(&B.q_empty[i % QS]);
       }
