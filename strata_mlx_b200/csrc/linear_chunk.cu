@@ -47,7 +47,7 @@ constexpr int HALF = C * 128;  // bytes of 64 columns of a chunk's rows
 constexpr int THREADS = 24 * 32;
 constexpr int OUT_WARP = 4, STATE_WARP = 8, KW_WARP = 16, MMA_WARP = 20, DECAY_WARP = 21, LOAD_WARP = 22, SUM_WARP = 23;
 // registers a thread: 80 at launch; the groups' shares add up to as many
-constexpr int P_REGS = 72, OUT_REGS = 72, STATE_REGS = 112, KW_REGS = 72, CONTROL_REGS = 40;
+constexpr int P_REGS = 64, OUT_REGS = 56, STATE_REGS = 120, KW_REGS = 72, CONTROL_REGS = 48;
 static_assert(P_REGS + OUT_REGS + 2 * STATE_REGS + KW_REGS + CONTROL_REGS == 6 * 80, "a block's registers");
 // the first launch's: 12 warps make w K, 8 add up D, 3 control
 constexpr int ADD_SUM_WARP = 12, ADD_STAGES = 4, ADD_RUN = 8;  // chunks whose D adds up in tensor memory
@@ -79,6 +79,10 @@ struct AddBars {
   uint32_t tmem;
   int bail;
 };
+
+// chunk i's place in a ring, and the phase of its barriers
+template <int N> __device__ __forceinline__ uint32_t slot(int i) { return uint32_t(i) % N; }
+template <int N> __device__ __forceinline__ int phase(int i) { return int(uint32_t(i) / N); }
 
 template <int DK>
 struct Shape {
@@ -300,9 +304,9 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
   if (warp < ADD_SUM_WARP) {
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
-      const int st = i % ADD_STAGES, m = len - chunk(i) * C;
-      if (!wait(&B.dec_full[i % RING], i / RING, &B.full[st], i / ADD_STAGES, &B.kw_empty[i & 1], i / 2 + 1)) break;
-      const float* w = dec + i % RING * C;
+      const int st = slot<ADD_STAGES>(i), m = len - chunk(i) * C;
+      if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.full[st], phase<ADD_STAGES>(i), &B.kw_empty[i & 1], i / 2 + 1)) break;
+      const float* w = dec + slot<RING>(i) * C;
       uint8_t* kw = smem + L::KW + (i & 1) * 3 * L::K_BYTES;
 #pragma unroll 2
       for (int j = tid; j < C * DK / 8; j += ADD_SUM_WARP * 32) {
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
       fence_async();
       arrive(&B.kw_full[i & 1]);
       arrive(&B.empty[st]);
-      arrive(&B.dec_empty[i % RING]);
+      arrive(&B.dec_empty[slot<RING>(i)]);
     }
   } else if (warp < MMA_WARP) {
     // ---- the sums of ADD_RUN chunks into one
@@ -363,10 +367,10 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
         float after = __shfl_down_sync(0xffffffffu, down, 1);
         if (lane == 31) after = 0.f;
         after += later;
-        if (!(ok = wait(&B.dec_empty[i % RING], i / RING + 1))) break;
-        *reinterpret_cast<float2*>(dec + i % RING * C + 2 * lane) = make_float2(fast_exp2((after + g.y) * LOG2E), fast_exp2(after * LOG2E));
+        if (!(ok = wait(&B.dec_empty[slot<RING>(i)], phase<RING>(i) + 1))) break;
+        *reinterpret_cast<float2*>(dec + slot<RING>(i) * C + 2 * lane) = make_float2(fast_exp2((after + g.y) * LOG2E), fast_exp2(after * LOG2E));
         later += __shfl_sync(0xffffffffu, down, 0);
-        arrive(&B.dec_full[i % RING]);
+        arrive(&B.dec_full[slot<RING>(i)]);
       }
       if (lane == 0) A.logs[(int64_t(b) * a.v_heads + h) * A.segments + seg] = later;
     } else if (warp == LOAD_WARP) {
@@ -375,8 +379,8 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
         int i = 0;
 #pragma unroll 1
         for (; i < n; ++i) {
-          const int st = i % ADD_STAGES, t0 = chunk(i) * C;
-          if (!wait.alone(&B.empty[st], i / ADD_STAGES + 1)) break;
+          const int st = slot<ADD_STAGES>(i), t0 = chunk(i) * C;
+          if (!wait.alone(&B.empty[st], phase<ADD_STAGES>(i) + 1)) break;
           uint8_t* stage = smem + st * L::STAGE;
           mbar_arrive_expect_tx(&B.full[st], bytes);
 #pragma unroll 1
@@ -387,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
         // copies in flight land before the block may end
 #pragma unroll 1
         for (int k = max(0, i - ADD_STAGES); k < i; ++k)
-          mbar_wait(&B.full[k % ADD_STAGES], uint32_t(k / ADD_STAGES) & 1, nullptr, 20000000LL);
+          mbar_wait(&B.full[slot<ADD_STAGES>(k)], uint32_t(phase<ADD_STAGES>(k)) & 1, nullptr, 20000000LL);
       }
     } else if (warp == MMA_WARP) {
       const bool leader = elect_one();
@@ -395,9 +399,9 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
       if (!ok) wait.stop();
 #pragma unroll 1
       for (int i = 0; i < n && ok; ++i) {
-        const int st = i % ADD_STAGES, run = i / ADD_RUN;
+        const int st = slot<ADD_STAGES>(i), run = i / ADD_RUN;
         if (i % ADD_RUN == 0 && !(ok = wait(&B.d_empty[run & 1], run / 2 + 1))) break;
-        if (!(ok = wait(&B.full[st], i / ADD_STAGES, &B.kw_full[i & 1], i / 2))) break;
+        if (!(ok = wait(&B.full[st], phase<ADD_STAGES>(i), &B.kw_full[i & 1], i / 2))) break;
         fence_after();
         if (leader) {
           const uint64_t v = desc_mn(smem + st * L::STAGE + L::K_BYTES, HALF), kw = desc_mn(smem + L::KW + (i & 1) * 3 * L::K_BYTES, HALF);
@@ -470,11 +474,11 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll 1
       for (int i = 0; i < n; ++i) {
-        if (!wait(&B.dec_full[i % RING], i / RING, &B.a_full, i)) break;
+        if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.a_full, i)) break;
         fence_after();
         uint32_t r[32];
         ld_frag64(lanes + COL_A, r);
-        const float* g2 = dec[i % RING].g2;
+        const float* g2 = dec[slot<RING>(i)].g2;
         const float ga = g2[r0] + shift, gb = g2[r0 + 8] + shift;
         wait_ld();
         fence_before();
@@ -494,7 +498,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
           }
           pk[2 * j] = bits_of(__floats2bfloat162_rn(x0, x1)) ^ sign, pk[2 * j + 1] = bits_of(__floats2bfloat162_rn(y0, y1)) ^ sign;
         }
-        arrive(&B.dec_empty[i % RING]);
+        arrive(&B.dec_empty[slot<RING>(i)]);
         if (!wait(&B.p_empty, i + 1)) break;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {  // r0 and r0 + 8 have one place in the swizzle
@@ -513,12 +517,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       const int token = (lane >> 4) * 8 + (lane & 7), piece = 4 * (warp & 3) + ((lane >> 3) & 1);
 #pragma unroll 1
       for (int i = 0; i < n; ++i) {
-        if (!wait(&B.dec_full[i % RING], i / RING, &B.o_full, i)) break;
+        if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.o_full, i)) break;
         fence_after();
         if (ot == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         out_sync();  // the tile's last store has read it
         const int t0 = (c0 + i) * C, m = len - t0;
-        const float* eg = dec[i % RING].eg;
+        const float* eg = dec[slot<RING>(i)].eg;
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {  // 16 value dimensions by 32 tokens at a time
           const int hf = q >> 1, j0 = 4 * (q & 1);
@@ -553,7 +557,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
             store_transposed(smem_u32(tile) + (pc >> 3) * HALF + row * 128 + (((pc & 7) ^ (row & 7)) << 4), f[0], f[1], f[2], f[3]);
           }
         }
-        arrive(&B.dec_empty[i % RING]);
+        arrive(&B.dec_empty[slot<RING>(i)]);
         fence_async();
         out_sync();
         if (ot == 0) {
@@ -612,9 +616,9 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         fence_after();
       }
       publish();
-      if (!wait(&B.dec_full[i % RING], i / RING, &B.d_full, i)) break;
+      if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.d_full, i)) break;
       fence_after();
-      const float2 d = make_float2(dec[i % RING].a, dec[i % RING].a), one = make_float2(dec[i % RING].one, dec[i % RING].one);
+      const float2 d = make_float2(dec[slot<RING>(i)].a, dec[slot<RING>(i)].a), one = make_float2(dec[slot<RING>(i)].one, dec[slot<RING>(i)].one);
 #pragma unroll
       for (int k = 0; k < N; k += 16) {
         uint32_t r[16];
@@ -628,7 +632,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       }
       fence_before();
       arrive(&B.d_empty);
-      arrive(&B.dec_empty[i % RING]);
+      arrive(&B.dec_empty[slot<RING>(i)]);
     }
     if (seg == A.segments - 1) {
       float* to = a.state_out + (head * a.k_dim + k0) * a.v_dim + dv;
@@ -648,12 +652,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
       const int m = len - (c0 + i) * C;
-      if (!wait(&B.dec_full[i % RING], i / RING, &B.k_full[i % KS], i / KS)) break;
-      const uint8_t* k = smem + L::K + i % KS * L::K_BYTES;
-      const float* w = dec[i % RING].w;
+      if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.k_full[slot<KS>(i)], phase<KS>(i))) break;
+      const uint8_t* k = smem + L::K + slot<KS>(i) * L::K_BYTES;
+      const float* w = dec[slot<RING>(i)].w;
       if (m < C) {
-        if (!wait(&B.v_full[i % VS], i / VS)) break;
-        clear_values(smem + L::V + i % VS * L::V_BYTES, m, lt, 128);
+        if (!wait(&B.v_full[slot<VS>(i)], phase<VS>(i))) break;
+        clear_values(smem + L::V + slot<VS>(i) * L::V_BYTES, m, lt, 128);
       }
       bool ok = true;
 #pragma unroll 1
@@ -668,8 +672,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         arrive(&B.kw_full[hf]);
       }
       if (!ok) break;
-      arrive(&B.k_empty[i % KS]);
-      arrive(&B.dec_empty[i % RING]);
+      arrive(&B.k_empty[slot<KS>(i)]);
+      arrive(&B.dec_empty[slot<RING>(i)]);
     }
   } else {
   fewer_registers<CONTROL_REGS>();
@@ -692,8 +696,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       if (lane == 31) after = 0.f;
       constexpr float LOG2E = 1.4426950408889634f;
       const float e0 = (before + g0) * LOG2E, e1 = up * LOG2E;
-      Decays& D = dec[i % RING];
-      if (!wait(&B.dec_empty[i % RING], i / RING + 1)) return false;
+      Decays& D = dec[slot<RING>(i)];
+      if (!wait(&B.dec_empty[slot<RING>(i)], phase<RING>(i) + 1)) return false;
       *reinterpret_cast<float2*>(&D.g2[2 * lane]) = make_float2(e0, e1);
       *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(fast_exp2(e0) * a.scale, fast_exp2(e1) * a.scale);
       *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(fast_exp2((after + g1) * LOG2E), fast_exp2(after * LOG2E));
@@ -701,7 +705,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         const bool near = up > -0.69314718f;
         D.a = near ? expm1_near(up) : fast_exp2(e1), D.one = near ? 1.f : 0.f;
       }
-      arrive(&B.dec_full[i % RING]);
+      arrive(&B.dec_full[slot<RING>(i)]);
       return true;
     };
     const bool leader = elect_one();
@@ -710,18 +714,18 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     for (; i < n; ++i) {
       if (i + 1 < n && !decays(i + 1)) break;
       if (i < 0) continue;
-      if (!wait(&B.v_empty[i % VS], i / VS + 1)) break;
+      if (!wait(&B.v_empty[slot<VS>(i)], phase<VS>(i) + 1)) break;
       if (leader) {
-        mbar_arrive_expect_tx(&B.v_full[i % VS], (a.v_dim > 64 ? 2 : 1) * HALF);
+        mbar_arrive_expect_tx(&B.v_full[slot<VS>(i)], (a.v_dim > 64 ? 2 : 1) * HALF);
 #pragma unroll 1
         for (int x = 0; x < a.v_dim; x += 64)
-          tma_load(smem + L::V + i % VS * L::V_BYTES + x / 64 * HALF, &maps.v, x, h, (c0 + i) * C, b, &B.v_full[i % VS]);
+          tma_load(smem + L::V + slot<VS>(i) * L::V_BYTES + x / 64 * HALF, &maps.v, x, h, (c0 + i) * C, b, &B.v_full[slot<VS>(i)]);
       }
       __syncwarp();
     }
     if (leader)  // copies in flight land before the block may end
 #pragma unroll 1
-      for (int k = max(0, i - VS); k < i; ++k) mbar_wait(&B.v_full[k % VS], uint32_t(k / VS) & 1, nullptr, 20000000LL);
+      for (int k = max(0, i - VS); k < i; ++k) mbar_wait(&B.v_full[slot<VS>(k)], uint32_t(phase<VS>(k)) & 1, nullptr, 20000000LL);
     __syncwarp();
   } else if (warp == LOAD_WARP) {
     // ---- keys and queries
@@ -729,13 +733,13 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       int i = 0;
 #pragma unroll 1
       for (; i < n; ++i) {
-        const int t0 = (c0 + i) * C, ks = i % KS, qs = i % QS;
-        if (!wait.alone(&B.k_empty[ks], i / KS + 1)) break;
+        const int t0 = (c0 + i) * C, ks = slot<KS>(i), qs = slot<QS>(i);
+        if (!wait.alone(&B.k_empty[ks], phase<KS>(i) + 1)) break;
         mbar_arrive_expect_tx(&B.k_full[ks], L::K_BYTES);
 #pragma unroll 1
         for (int x = 0; x < DK; x += 64) tma_load(smem + L::K + ks * L::K_BYTES + x / 64 * HALF, &maps.k, x, hk, t0, b, &B.k_full[ks]);
-        if (!wait.alone(&B.q_empty[qs], i / QS + 1)) {
-          mbar_wait(&B.k_full[ks], uint32_t(i / KS) & 1, nullptr, 20000000LL);
+        if (!wait.alone(&B.q_empty[qs], phase<QS>(i) + 1)) {
+          mbar_wait(&B.k_full[ks], uint32_t(phase<KS>(i)) & 1, nullptr, 20000000LL);
           break;
         }
         mbar_arrive_expect_tx(&B.q_full[qs], L::K_BYTES);
@@ -744,9 +748,9 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       }
       // copies in flight land before the block may end
 #pragma unroll 1
-      for (int k = max(0, i - KS); k < i; ++k) mbar_wait(&B.k_full[k % KS], uint32_t(k / KS) & 1, nullptr, 20000000LL);
+      for (int k = max(0, i - KS); k < i; ++k) mbar_wait(&B.k_full[slot<KS>(k)], uint32_t(phase<KS>(k)) & 1, nullptr, 20000000LL);
 #pragma unroll 1
-      for (int k = max(0, i - QS); k < i; ++k) mbar_wait(&B.q_full[k % QS], uint32_t(k / QS) & 1, nullptr, 20000000LL);
+      for (int k = max(0, i - QS); k < i; ++k) mbar_wait(&B.q_full[slot<QS>(k)], uint32_t(phase<QS>(k)) & 1, nullptr, 20000000LL);
     }
     __syncwarp();
   } else if (warp == SUM_WARP) {
@@ -755,8 +759,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     const uint64_t kw = desc_mn(smem + L::KW, HALF);
 #pragma unroll 1
     for (int i = 0; i < n && tmem == 0; ++i) {
-      const uint64_t vt = desc_mn(smem + L::V + i % VS * L::V_BYTES, HALF);
-      if (!wait(&B.v_full[i % VS], i / VS, &B.d_empty, i + 1, &B.kw_full[0], i)) break;
+      const uint64_t vt = desc_mn(smem + L::V + slot<VS>(i) * L::V_BYTES, HALF);
+      if (!wait(&B.v_full[slot<VS>(i)], phase<VS>(i), &B.d_empty, i + 1, &B.kw_full[0], i)) break;
       fence_after();
       if (leader) {
         add_products<DK>(COL_D, vt, kw, 0, true);
@@ -769,7 +773,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         add_products<DK>(COL_D, vt, kw, 1, false);
         commit(&B.d_full);
         commit(&B.kw_empty[1]);
-        commit(&B.v_empty[i % VS]);
+        commit(&B.v_empty[slot<VS>(i)]);
       }
       __syncwarp();
     }
@@ -780,7 +784,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     // All 512 columns are this block's, so tensor memory starts at address 0.
     const bool leader = elect_one();
     auto a_product = [&](int i) {
-      const uint8_t *q = smem + L::Q + i % QS * L::K_BYTES, *k = smem + L::K + i % KS * L::K_BYTES;
+      const uint8_t *q = smem + L::Q + slot<QS>(i) * L::K_BYTES, *k = smem + L::K + slot<KS>(i) * L::K_BYTES;
       if (leader) {
         uint64_t qd = desc_k(q), kd = desc_k(k);
 #pragma unroll 1
@@ -788,7 +792,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
 #pragma unroll
           for (int s = 0; s < 4; ++s) mma_ss(COL_A, qd + 2 * s, kd + 2 * s, idesc_bf16(64, 64, false, false), x > 0 || s > 0);
         commit(&B.a_full);
-        commit(&B.k_empty[i % KS]);
+        commit(&B.k_empty[slot<KS>(i)]);
       }
       __syncwarp();
     };
@@ -800,17 +804,17 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     }
 #pragma unroll 1
     for (int i = 0; i < n && ok; ++i) {
-      const uint64_t vt = desc_mn(smem + L::V + i % VS * L::V_BYTES, HALF);
+      const uint64_t vt = desc_mn(smem + L::V + slot<VS>(i) * L::V_BYTES, HALF);
       if (i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
         const int j = i + 1;
-        if (!(ok = wait(&B.q_full[j % QS], j / QS, &B.k_full[j % KS], j / KS, &B.a_empty, i))) break;
+        if (!(ok = wait(&B.q_full[slot<QS>(j)], phase<QS>(j), &B.k_full[slot<KS>(j)], phase<KS>(j), &B.a_empty, i))) break;
         fence_after();
         a_product(j);
       }
       if (!(ok = wait(&B.s_full, i))) break;
       fence_after();
       if (leader) {
-        const uint64_t qd = desc_k(smem + L::Q + i % QS * L::K_BYTES);
+        const uint64_t qd = desc_k(smem + L::Q + slot<QS>(i) * L::K_BYTES);
 #pragma unroll 1
         for (int e = 2 * (DK / 64) - 1; e >= 0; --e) {  // the rest, then the rounded state; 64 key dimensions each
           const int x = e % (DK / 64);
@@ -820,10 +824,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
                    e < 2 * (DK / 64) - 1 || s > 0);
         }
         commit(&B.s_empty);
-        commit(&B.q_empty[i % QS]);
+        commit(&B.q_empty[slot<QS>(i)]);
       }
       __syncwarp();
-      if (!(ok = wait(&B.p_full, i, &B.v_full[i % VS], i / VS, &B.o_empty, i + 1))) break;
+      if (!(ok = wait(&B.p_full, i, &B.v_full[slot<VS>(i)], phase<VS>(i), &B.o_empty, i + 1))) break;
       if (len - (c0 + i) * C < C && !(ok = wait(&B.kw_full[0], i))) break;  // the last chunk's values are cleared
       fence_after();
       if (leader) {
@@ -832,7 +836,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
           mma_ss(COL_I, vt + 128 * s, desc_k(smem + L::P) + 2 * s, idesc_bf16(128, 64, true, false), s > 0);
         commit(&B.o_full);
         commit(&B.p_empty);
-        commit(&B.v_empty[i % VS]);
+        commit(&B.v_empty[slot<VS>(i)]);
       }
       __syncwarp();
     }
