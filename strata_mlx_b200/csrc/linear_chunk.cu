@@ -282,6 +282,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
   const int seg = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / (a.v_heads / a.k_heads);
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.tokens) : a.tokens;
   const int c0 = seg * A.per, n = max(0, min(c0 + A.per, (len + C - 1) / C) - c0);
+  pdl_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < ADD_STAGES; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], ADD_SUM_WARP + 1);
     for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], ADD_SUM_WARP);
@@ -583,6 +584,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     float2 S[N / 2];
     const int64_t head = int64_t(b) * a.v_heads + h;
     const bool started = A.segments > 1, there = started || (a.state_in && dv < a.v_dim);
+    if (started) pdl_wait();  // for the states before the segments: only these warps read them
     const float* from = started ? A.parts + ((head * A.segments + seg) * DK + k0) * 128 + dv
                                 : a.state_in + (head * a.k_dim + k0) * a.v_dim + dv;
     const int kd = started ? DK : a.k_dim, ld = started ? 128 : a.v_dim;
@@ -858,6 +860,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
 template <int DK>
 __global__ void __launch_bounds__(256) scan_kernel(const Args A) {
   const sc_linear& a = A.a;
+  pdl_launch_dependents();
+  pdl_wait();
   const int64_t head = blockIdx.x;
   const int e = blockIdx.y * 256 + threadIdx.x, k = e / 128, dv = e % 128;
   float* part = A.parts + head * A.segments * DK * 128 + e;
@@ -937,9 +941,24 @@ int run(const Args& A, cudaStream_t s) {
     if (int rc = raise_smem(reinterpret_cast<const void*>(add_kernel<DK>), add_smem, "linear attention smem attribute"))
       return rc;
     add_kernel<DK><<<dim3(grid.x - 1, grid.y, grid.z), THREADS, add_smem, s>>>(A, maps);
-    scan_kernel<DK><<<dim3(unsigned(a.batch) * unsigned(a.v_heads), DK * 128 / 256), 256, 0, s>>>(A);
+    // the scan and the whole as programmatic dependents: their blocks start as the ones before leave their SMs
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(a.batch) * unsigned(a.v_heads), DK * 128 / 256);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, scan_kernel<DK>, A)) return cuda_failed(e, "linear attention scan launch");
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, chunk_kernel<DK>, A, maps)) return cuda_failed(e, "linear attention launch");
+  } else {
+    chunk_kernel<DK><<<grid, THREADS, smem, s>>>(A, maps);
   }
-  chunk_kernel<DK><<<grid, THREADS, smem, s>>>(A, maps);
   if (cudaError_t e = cudaGetLastError()) return cuda_failed(e, "linear attention launch");
   return SC_OK;
 }
