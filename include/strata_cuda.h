@@ -363,7 +363,8 @@ typedef struct sc_linear {
   float scale;
 } sc_linear;
 
-/* Prompts: any number of tokens, the state carried in float32. workspace: sc_linear_attention_workspace bytes. */
+/* Prompts: any number of tokens, the state carried in float32. workspace: sc_linear_attention_workspace bytes (NULL
+ * where that is 0). */
 SC_API int sc_linear_attention(const sc_linear* a, void* workspace, size_t workspace_bytes, int* err, void* stream);
 SC_API size_t sc_linear_attention_workspace(const sc_linear* a);
 

@@ -72,27 +72,31 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v)
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
   return __half22float2(*reinterpret_cast<__half2*>(&v));
 }
+// 2^x to 2^-22 of it, zero below 2^-126: a probability relative to a running maximum
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
 
 template <int N>
-__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* sh) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+__device__ __forceinline__ int block_sum(int v, int* sh) {
+  v = __reduce_add_sync(0xffffffffu, v);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
-  int64_t t = 0;
+  int t = 0;
 #pragma unroll
   for (int i = 0; i < N / 32; ++i) t += sh[i];
   __syncthreads();
   return t;
 }
-
 template <int N>
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& total) {  // inclusive
+__device__ __forceinline__ int block_scan(int v, int* sh, int& total) {  // inclusive
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, v, o);
+    const int y = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += y;
   }
   if (lane == 31) sh[warp] = v;
@@ -107,14 +111,17 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& t
   return v;
 }
 
-// The units' numbering: sequence after sequence, in each head after head. Block x of X takes units [x U / X,
-// (x + 1) U / X), so unit u is block ((u + 1) X - 1) / U's; X is at most U, so that every block up to X has a unit.
-template <int N>
-__device__ __forceinline__ int64_t units_before(const Args& A, int unit, int b, int64_t* sh, int* err) {
-  int64_t n = 0;
-  for (int i = threadIdx.x; i < b; i += N) n += (length_of(A.pages, i, err) + unit - 1) / unit;
-  return block_sum<N>(n, sh) * A.kv_heads;
-}
+// The units' numbering: sequence after sequence, in each head after head. X blocks (at most as many as there are
+// units, so that each has one) share U units as evenly as whole ones go: the first U % X blocks take one more.
+struct Split {
+  uint32_t each, more;  // U / X, U % X
+  __device__ __forceinline__ Split(uint32_t U, uint32_t X) : each(U / X), more(U % X) {}
+  __device__ __forceinline__ uint32_t start(uint32_t x) const { return x * each + min(x, more); }
+  __device__ __forceinline__ uint32_t block_of(uint32_t u) const {
+    const uint32_t longer = more * (each + 1);
+    return u < longer ? u / (each + 1) : more + (u - longer) / each;
+  }
+};
 
 template <typename T, int DP, int SUB>
 __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Args A) {
@@ -123,28 +130,32 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
   __shared__ uint4 s_q[KC][32];
   __shared__ __align__(16) float s_o[WARPS][HEADS][DP];
   __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS];
-  __shared__ int64_t s_sum[WARPS], s_before;
-  __shared__ int s_b;
+  __shared__ int s_sum[WARPS], s_before, s_b;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int ht = blockIdx.y;
-  const int64_t x = blockIdx.x;
+  const uint32_t x = blockIdx.x;
   pdl_launch_dependents();
   // the units in all, and the sequence that holds this block's first one (a single pass up to THREADS sequences)
-  int64_t U, to;
+  int U, to;
   const int first = tid < A.batch ? (length_of(A.pages, tid, A.err) + UNIT - 1) / UNIT : 0;
   if (A.batch == 1) {
     U = to = (length_of(A.pages, 0, nullptr) + UNIT - 1) / UNIT;
   } else {
     to = block_scan<THREADS>(first, s_sum, U);
-    if (A.batch > THREADS) U = units_before<THREADS>(A, UNIT, A.batch, s_sum, A.err);
+    if (A.batch > THREADS) {
+      int n = first;
+#pragma unroll 1
+      for (int i = tid + THREADS; i < A.batch; i += THREADS) n += (length_of(A.pages, i, A.err) + UNIT - 1) / UNIT;
+      U = block_sum<THREADS>(n, s_sum);
+    }
   }
   U *= A.kv_heads;
-  const int64_t X = min(int64_t(A.columns), U);
+  const uint32_t X = min(A.columns, U);
   if (x >= X) return;
-  int64_t u = x * U / X;
-  const int64_t u1 = (x + 1) * U / X;
-  int b = 0;
-  int64_t before = 0;
+  const Split split(U, X);
+  int u = split.start(x);
+  const int u1 = split.start(x + 1);
+  int b = 0, before = 0;
   if (A.batch > 1) {
     if (tid == 0) s_b = -1;
     __syncthreads();
@@ -154,10 +165,10 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
       __syncthreads();
       b0 += THREADS;
       if (s_b >= 0 || b0 >= A.batch) break;
-      int64_t total;
+      int total;
       if (tid == THREADS - 1) s_before = to;  // where the next sequences begin
       __syncthreads();
-      const int64_t from = s_before;
+      const int from = s_before;
       mine = b0 + tid < A.batch ? (length_of(A.pages, b0 + tid, nullptr) + UNIT - 1) / UNIT : 0;
       to = from + block_scan<THREADS>(mine, s_sum, total);
     }
@@ -167,8 +178,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
   int hk, ul;
   {
     const int n = (length_of(A.pages, b, nullptr) + UNIT - 1) / UNIT;
-    const int64_t in = u - before * A.kv_heads;
-    hk = int(in / n), ul = int(in % n);
+    const uint32_t in = u - before * A.kv_heads;
+    hk = in / n, ul = in % n;
   }
   const Pages& P = A.pages;
   const int mask = (1 << P.shift) - 1, chunks = A.dim / 8;
@@ -179,7 +190,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
       ++b, hk = 0, ul = 0;
       continue;
     }
-    const int ue = int(min(int64_t(n_units), ul + (u1 - u)));
+    const int ue = min(n_units, ul + (u1 - u));
     // ---- this warp's tiles
     const int end = min(len, ue * UNIT);
     int base = (ul * WARPS + warp) * TILE;
@@ -242,6 +253,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
     int id[IDS], next[IDS];
     load_ids(base, id);
     // the heads' queries, in the products' order
+#pragma unroll 1
     for (int i = tid; i < KC * 32; i += THREADS) {
       const int c = (i / 32) * 4 + (i & 3), h = (i & 31) >> 2;
       uint4 v = make_uint4(0, 0, 0, 0);
@@ -254,6 +266,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
     load_v(base, id);
     load_ids(base + UNIT, next);
     __syncthreads();
+#pragma unroll 1
     for (; base < end; base += UNIT) {
       float s[SUB][4], s2[SUB][4];  // two chains of products
 #pragma unroll
@@ -306,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
         }
         x0 = fmaxf(x0, m0), x1 = fmaxf(x1, m1);
         b0 = finite_or_0(x0), b1 = finite_or_0(x1);
-        const float c0 = exp2f(m0 - b0), c1 = exp2f(m1 - b1);
+        const float c0 = ex2(m0 - b0), c1 = ex2(m1 - b1);
         m0 = x0, m1 = x1;
         l0 *= c0, l1 *= c1;
 #pragma unroll
@@ -319,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
         uint32_t hi[2], lo[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float p0 = exp2f(s[i][2 * r] - b0), p1 = exp2f(s[i][2 * r + 1] - b1);
+          const float p0 = ex2(s[i][2 * r] - b0), p1 = ex2(s[i][2 * r + 1] - b1);
           l0 += p0, l1 += p1;
           const uint32_t h = pack2<T>(p0, p1);
           const float2 back = unpack2<T>(h);
@@ -355,7 +368,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
     float M0 = -INFINITY, M1 = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) M0 = fmaxf(M0, s_m[w][2 * t]), M1 = fmaxf(M1, s_m[w][2 * t + 1]);
-    const float c0 = exp2f(m0 - finite_or_0(M0)), c1 = exp2f(m1 - finite_or_0(M1));
+    const float c0 = ex2(m0 - finite_or_0(M0)), c1 = ex2(m1 - finite_or_0(M1));
 #pragma unroll
     for (int i = 0; i < VC; ++i) {
       float4* to = reinterpret_cast<float4*>(&s_o[warp][2 * t][64 * i + 8 * g]);
@@ -368,6 +381,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
     __syncthreads();
     const bool whole = ul == 0 && ue == n_units;
     const int64_t part = ((int64_t(ht) * A.columns + x) * 2 + (ul == 0)) * HEADS;  // 0: a head's later run, 1: its first
+#pragma unroll 1
     for (int e = tid; e < heads * (DP / 4); e += THREADS) {
       const int h = e / (DP / 4), d = 4 * (e % (DP / 4));
       float M = -INFINITY, L = 0.f;
@@ -377,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
       float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        L += s_l[w][h] * exp2f(s_m[w][h] - mb);
+        L += s_l[w][h] * ex2(s_m[w][h] - mb);
         const float4 v = *reinterpret_cast<const float4*>(&s_o[w][h][d]);
         r.x += v.x, r.y += v.y, r.z += v.z, r.w += v.w;
       }
@@ -402,28 +416,27 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Ar
 
 // The blocks that share the units of a sequence's heads: head hk's are first(hk) .. last(hk), none when n is 0.
 struct Share {
-  int64_t U, X, before, n;
-  __device__ int first(int hk) const { return int(((before + hk * n + 1) * X - 1) / U); }
-  __device__ int last(int hk) const { return int(((before + hk * n + n) * X - 1) / U); }
+  Split split;
+  int before, n;
+  __device__ __forceinline__ int first(int hk) const { return split.block_of(before + hk * n); }
+  __device__ __forceinline__ int last(int hk) const { return split.block_of(before + hk * n + n - 1); }
 };
 template <int N>
-__device__ __forceinline__ Share share_of(const Args& A, int unit, int b, int64_t* sh) {
-  Share s;
-  s.n = (length_of(A.pages, b, nullptr) + unit - 1) / unit;
-  if (A.batch == 1) {
-    s.U = s.n, s.before = 0;
-  } else {
-    int64_t all = 0, before = 0;
+__device__ __forceinline__ Share share_of(const Args& A, int unit, int b, int* sh) {
+  const int n = (length_of(A.pages, b, nullptr) + unit - 1) / unit;
+  int U = n, before = 0;
+  if (A.batch > 1) {
+    int all = 0;
+#pragma unroll 1
     for (int i = threadIdx.x; i < A.batch; i += N) {
-      const int64_t n = (length_of(A.pages, i, nullptr) + unit - 1) / unit;
-      all += n;
-      if (i < b) before += n;
+      const int k = (length_of(A.pages, i, nullptr) + unit - 1) / unit;
+      all += k;
+      if (i < b) before += k;
     }
-    s.U = block_sum<N>(all, sh), s.before = block_sum<N>(before, sh);
+    U = block_sum<N>(all, sh), before = block_sum<N>(before, sh);
   }
-  s.U *= A.kv_heads, s.before *= A.kv_heads;
-  s.X = min(int64_t(A.columns), s.U);
-  return s;
+  U = max(1, U * A.kv_heads);  // there may be none
+  return {Split(U, min(A.columns, U)), before * A.kv_heads, n};
 }
 
 // Blocks 0 .. batch x q_heads - 1: a query head's output from its partial results (zeros for an empty sequence). The
@@ -431,7 +444,7 @@ __device__ __forceinline__ Share share_of(const Args& A, int unit, int b, int64_
 template <typename T, int DP, int PACK>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int unit, int slot_blocks) {
   constexpr int LANES = DP / 4, GROUPS = JOIN_THREADS / LANES;  // threads of a row, and rows read side by side
-  __shared__ int64_t sh[JOIN_THREADS / 32];
+  __shared__ int sh[JOIN_THREADS / 32];
   __shared__ __align__(16) float s_o[GROUPS][DP];
   __shared__ float2 s_gml[GROUPS];
   extern __shared__ float2 s_ml[];  // of every query head (weights)
@@ -445,6 +458,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int un
     const int first = s.n ? s.first(hk) : 0, last = s.n ? s.last(hk) : 0;
     pdl_wait();
     if (s.n == 0) {
+#pragma unroll 1
       for (int d = tid; d < A.dim; d += JOIN_THREADS) out[d] = from_f32<T>(0.f);
       return;
     }
@@ -454,6 +468,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int un
     const int64_t base = int64_t(ht) * A.columns * 2 * HEADS + hr;
     float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
     for (int x0 = first + row; x0 <= last; x0 += 4 * GROUPS) {
       float2 ml[4];
       float4 v[4];
@@ -469,12 +484,12 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int un
         }
       }
       const float top = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), M), mb = finite_or_0(top);
-      const float c = exp2f(M - mb);
+      const float c = ex2(M - mb);
       M = top;
       L *= c, o.x *= c, o.y *= c, o.z *= c, o.w *= c;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float e = exp2f(ml[i].x - mb);
+        const float e = ex2(ml[i].x - mb);
         L += ml[i].y * e;
         o.x += v[i].x * e, o.y += v[i].y * e, o.z += v[i].z * e, o.w += v[i].w * e;
       }
@@ -491,7 +506,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int un
 #pragma unroll
       for (int i = 0; i < GROUPS; ++i) {
         const float4 v = *reinterpret_cast<const float4*>(&s_o[i][d]);
-        const float e = exp2f(s_gml[i].x - mb);
+        const float e = ex2(s_gml[i].x - mb);
         L += s_gml[i].y * e;
         o.x += v.x * e, o.y += v.y * e, o.z += v.z * e, o.w += v.w * e;
       }
@@ -536,6 +551,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int un
   load(0);
   const float old = live ? A.weight[b * A.weight_row + s] : 0.f;
   // s_ml: (tiles, PACK) the heads' maxima and the inverses of their sums, zeros for heads that there are not
+#pragma unroll 1
   for (int i = tid; i < tiles * PACK; i += JOIN_THREADS) {
     const int hk = i / PACK / A.head_tiles, ht = i / PACK % A.head_tiles, hh = ht * HEADS + i % PACK;
     float2 ml = make_float2(0.f, 0.f);
@@ -546,11 +562,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int un
       } else {
         const int64_t base = int64_t(ht) * A.columns * 2 * HEADS + i % PACK;
         float M = -INFINITY, L = 0.f;
-#pragma unroll 8
+#pragma unroll 2
         for (int k = first; k <= last; ++k) {
           const float2 v = A.part_ml[base + (int64_t(k) * 2 + (k == first)) * HEADS];
           const float top = fmaxf(M, v.x), mb = finite_or_0(top);
-          L = L * exp2f(M - mb) + v.y * exp2f(v.x - mb);
+          L = L * ex2(M - mb) + v.y * ex2(v.x - mb);
           M = top;
         }
         ml = make_float2(finite_or_0(M), L);
@@ -568,7 +584,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int un
 #pragma unroll
         for (int h = 0; h < PACK; ++h) {
           const float2 ml = s_ml[(t0 + i) * PACK + h];
-          if (ml.y != 0.f) sum += exp2f(x[i][h] - ml.x) * ml.y;
+          if (ml.y != 0.f) sum += ex2(x[i][h] - ml.x) * ml.y;
         }
     t0 += AHEAD;
     if (t0 >= tiles) break;
@@ -654,7 +670,7 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int slot_blocks = kv->weight ? int(ceil_div(A.slots, da::JOIN_THREADS)) : 0;
   const int64_t join_blocks = int64_t(kv->batch) * (q_heads + slot_blocks);
-  if (join_blocks > INT32_MAX) return SC_ERR_SHAPE;
+  if (join_blocks > INT32_MAX || int64_t(kv->batch) * kv->kv_heads * ceil_div(A.slots, l.unit) > INT32_MAX) return SC_ERR_SHAPE;
   auto run = [&](auto t, auto dp, auto sub) -> int {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value, SUB = decltype(sub)::value;

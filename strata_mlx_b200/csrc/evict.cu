@@ -29,7 +29,7 @@ constexpr int MAX_CLUSTER = 8;
 constexpr int STRETCH = 128 * WARPS;  // a block's slots are a multiple
 constexpr int PER_BLOCK = 2 * STRETCH;  // slots of a block before the cluster grows
 constexpr int MOST = 50 * 1024;   // slots a block can hold the keys of (200 KB); past 8 such blocks keys are made anew
-constexpr int FETCH = 16;         // weights and positions a thread loads at a time
+constexpr int FETCH = 8;          // weights and positions a thread loads at a time
 constexpr int MOVE_WARPS = 8;
 constexpr uint32_t KEPT = 0xffffffffu;
 
@@ -88,44 +88,39 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const Args A) {
     if (blocks > 1) cluster.sync();
     else __syncthreads();
   };
-  // weights and positions, FETCH a thread at a time; those below the budget are copied at once (the evicted among
-  // them are overwritten when their slots are filled)
-  auto fetch = [&](auto f) {
-    for (int i0 = tid; i0 < mine; i0 += FETCH * THREADS) {
-      float x[FETCH];
-      int32_t p[FETCH];
+  const int64_t from = int64_t(A.seen[b]) - A.recent;
+  auto is_safe = [&](int32_t p) { return p < A.sinks || p >= from; };
+  for (int i = tid; i < 2 * BINS; i += THREADS) s_hist[0][i] = 0;
+  // ---- weights and positions, FETCH a thread at a time; those below the budget are copied at once (the evicted among
+  // them are overwritten when their slots are filled). Keys; how many slots are kept by their place, and the least and
+  // largest of the other keys.
+  int safes = 0;
+  uint32_t lo = KEPT, hi = 0;
+#pragma unroll 1
+  for (int i0 = tid; i0 < mine; i0 += FETCH * THREADS) {
+    float x[FETCH];
+    int32_t p[FETCH];
 #pragma unroll
-      for (int u = 0; u < FETCH; ++u)
-        if (i0 + u * THREADS < mine) x[u] = w[s0 + i0 + u * THREADS], p[u] = pos[s0 + i0 + u * THREADS];
+    for (int u = 0; u < FETCH; ++u)
+      if (i0 + u * THREADS < mine) x[u] = w[s0 + i0 + u * THREADS], p[u] = pos[s0 + i0 + u * THREADS];
 #pragma unroll
-      for (int u = 0; u < FETCH; ++u) {
-        const int i = i0 + u * THREADS;
-        if (i < mine) {
-          if (s0 + i < keep) wo[s0 + i] = x[u], po[s0 + i] = p[u];
-          f(i, x[u], p[u]);
-        }
+    for (int u = 0; u < FETCH; ++u) {
+      const int i = i0 + u * THREADS;
+      if (i < mine) {
+        if (s0 + i < keep) wo[s0 + i] = x[u], po[s0 + i] = p[u];
+        const bool safe = is_safe(p[u]);
+        const uint32_t k = safe ? KEPT : order_of(x[u]);
+        safes += safe;
+        if (!safe) lo = min(lo, k), hi = max(hi, k);
+        if constexpr (HELD) s_key[i] = k;
       }
     }
-  };
+  }
   if (n <= keep) {
-    fetch([](int, float, int32_t) {});
     sync();  // lengths_out may be the lengths themselves
     if (rank == 0 && tid == 0) A.count[b] = 0, A.lengths_out[b] = n;
     return;
   }
-  const int64_t from = int64_t(A.seen[b]) - A.recent;
-  auto is_safe = [&](int32_t p) { return p < A.sinks || p >= from; };
-  for (int i = tid; i < 2 * BINS; i += THREADS) s_hist[0][i] = 0;
-  // ---- keys; how many slots are kept by their place, and the least and largest of the other keys
-  int safes = 0;
-  uint32_t lo = KEPT, hi = 0;
-  fetch([&](int i, float x, int32_t p) {
-    const bool safe = is_safe(p);
-    const uint32_t k = safe ? KEPT : order_of(x);
-    safes += safe;
-    if (!safe) lo = min(lo, k), hi = max(hi, k);
-    if constexpr (HELD) s_key[i] = k;
-  });
   if constexpr (HELD) {  // a step's end holds no slot's key
     const int end = (mine + 127) / 128 * 128;
     for (int i = mine + tid; i < end; i += THREADS) s_key[i] = 0;

@@ -172,15 +172,16 @@ static bool chunked(const sc_linear& a) { return a.tokens > la::FEW && lc::takes
 
 extern "C" size_t sc_linear_attention_workspace(const sc_linear* a) {
   if (la::check(a) || a->batch == 0) return 0;
-  return chunked(*a) ? lc::workspace(*a) : 16;
+  return chunked(*a) ? lc::workspace(*a) : 0;
 }
 
 extern "C" int sc_linear_attention(const sc_linear* a, void* workspace, size_t workspace_bytes, int* err, void* stream) {
   if (int rc = la::check(a)) return rc;
   if (a->batch == 0) return SC_OK;
-  if (!workspace) return SC_ERR_ARG;
+  const size_t need = sc_linear_attention_workspace(a);
+  if (need && !workspace) return SC_ERR_ARG;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return SC_ERR_ALIGN;
-  if (workspace_bytes < sc_linear_attention_workspace(a)) return SC_ERR_WORKSPACE;
+  if (workspace_bytes < need) return SC_ERR_WORKSPACE;
   if (chunked(*a)) return lc::launch(*a, workspace, err, static_cast<cudaStream_t>(stream));
   return la::launch(*a, stream);
 }

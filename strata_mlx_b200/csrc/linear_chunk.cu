@@ -903,7 +903,7 @@ inline size_t parts_bytes(const sc_linear& a, int segments) {
   return segments > 1 ? size_t(a.batch) * a.v_heads * segments * (size_t(dk) * 128 + 4) * 4 : 0;
 }
 
-size_t workspace(const sc_linear& a) { return parts_bytes(a, segments_of(a)) + 16; }
+size_t workspace(const sc_linear& a) { return parts_bytes(a, segments_of(a)); }
 
 // a tensor of (batch, tokens, heads, dim) as a map; the strides of axes of one entry are not looked at
 inline int map_of(CUtensorMap* m, const void* p, int dim, int heads, int tokens, int batch, int64_t head, int64_t token, int64_t row) {

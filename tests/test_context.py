@@ -106,10 +106,12 @@ def test_linear_attention_refusals(change, code):
 
 def test_linear_attention_workspace_and_the_step_form():
     lib = _lib.load()
-    A = linear(tokens=4096)
+    A = linear(tokens=4096, q_token=128, k_token=128, v_token=256, q_row=1 << 20, k_row=1 << 20, v_row=1 << 20)
     n = lib.sc_linear_attention_workspace(ctypes.addressof(A))
     assert n > 0 and lib.sc_linear_attention(ctypes.addressof(A), FAKE, n - 1, None, None) == -7
     assert lib.sc_linear_attention(ctypes.addressof(A), None, n, None, None) == -5
+    assert lib.sc_linear_attention(ctypes.addressof(A), FAKE + 8, n, None, None) == -4
+    assert lib.sc_linear_attention_workspace(ctypes.addressof(linear(tokens=8))) == 0  # the recurrence needs none
     assert lib.sc_linear_attention_step(ctypes.addressof(A), None) == -2  # one token a sequence
     assert lib.sc_linear_attention_step(ctypes.addressof(linear(lengths=FAKE)), None) == -2
     assert lib.sc_linear_attention_step(ctypes.addressof(linear(batch=0)), None) == 0
