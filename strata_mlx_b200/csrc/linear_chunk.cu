@@ -50,7 +50,7 @@ constexpr int OUT_WARP = 4, STATE_WARP = 8, KW_WARP = 16, MMA_WARP = 20, DECAY_W
 constexpr int P_REGS = 64, OUT_REGS = 56, STATE_REGS = 120, KW_REGS = 72, CONTROL_REGS = 48;
 static_assert(P_REGS + OUT_REGS + 2 * STATE_REGS + KW_REGS + CONTROL_REGS == 6 * 80, "a block's registers");
 // the first launch's: 12 warps make w K, 8 add up D, 3 control
-constexpr int ADD_SUM_WARP = 12, ADD_STAGES = 4, ADD_RUN = 8;  // chunks whose D adds up in tensor memory
+constexpr int ADD_SUM_WARP = 12, ADD_KW_WARPS = 6, ADD_STAGES = 4, ADD_RUN = 8;  // chunks whose D adds up in tensor memory
 constexpr int SUM_REGS = 96;
 static_assert(3 * 80 + 2 * SUM_REGS + CONTROL_REGS <= 6 * 80, "a block's registers");
 constexpr int SMS = 148;
@@ -171,6 +171,36 @@ __device__ __forceinline__ void split3(float2 v, uint32_t& t0, uint32_t& t1, uin
   t2 = rounded(rest(v, t1));
 }
 
+// tries of several barriers at once, so that their latencies overlap
+__device__ __forceinline__ bool try_wait2(uint64_t* x, uint32_t px, uint64_t* y, uint32_t py) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "and.pred p, p, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(x)), "r"(px & 1), "r"(smem_u32(y)), "r"(py & 1)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool try_wait3(uint64_t* x, uint32_t px, uint64_t* y, uint32_t py, uint64_t* z, uint32_t pz) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q, r;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n\t"
+      "and.pred p, p, q;\n\t"
+      "and.pred p, p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(x)), "r"(px & 1), "r"(smem_u32(y)), "r"(py & 1), "r"(smem_u32(z)), "r"(pz & 1)
+      : "memory");
+  return ok != 0;
+}
+
 // Waits, for a whole warp (all of its lanes go on, or none) and for one thread. Small in code, as there are many: the
 // warps' instructions have to fit the cache.
 struct Waits {
@@ -189,14 +219,13 @@ struct Waits {
   // several barriers side by side
   __device__ __forceinline__ bool operator()(uint64_t* x, int px, uint64_t* y, int py) const {
     const uint32_t start = uint32_t(clock());
-    while (!__all_sync(0xffffffffu, mbar_try_wait(x, uint32_t(px) & 1) & mbar_try_wait(y, uint32_t(py) & 1)))
+    while (!__all_sync(0xffffffffu, try_wait2(x, px, y, py)))
       if (__any_sync(0xffffffffu, over(start))) return stop();
     return true;
   }
   __device__ __forceinline__ bool operator()(uint64_t* x, int px, uint64_t* y, int py, uint64_t* z, int pz) const {
     const uint32_t start = uint32_t(clock());
-    while (!__all_sync(0xffffffffu, mbar_try_wait(x, uint32_t(px) & 1) & mbar_try_wait(y, uint32_t(py) & 1) &
-                                        mbar_try_wait(z, uint32_t(pz) & 1)))
+    while (!__all_sync(0xffffffffu, try_wait3(x, px, y, py, z, pz)))
       if (__any_sync(0xffffffffu, over(start))) return stop();
     return true;
   }
@@ -284,10 +313,10 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
   const int c0 = seg * A.per, n = max(0, min(c0 + A.per, (len + C - 1) / C) - c0);
   pdl_launch_dependents();
   if (tid == 0) {
-    for (int i = 0; i < ADD_STAGES; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], ADD_SUM_WARP + 1);
-    for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], ADD_SUM_WARP);
+    for (int i = 0; i < ADD_STAGES; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], ADD_KW_WARPS + 1);
+    for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], ADD_KW_WARPS);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&B.kw_full[i], ADD_SUM_WARP), mbar_init(&B.kw_empty[i], 1);
+      mbar_init(&B.kw_full[i], ADD_KW_WARPS), mbar_init(&B.kw_empty[i], 1);
       mbar_init(&B.d_full[i], 1), mbar_init(&B.d_empty[i], 8);
     }
     mbar_init(&B.done, 1);
@@ -303,18 +332,21 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
   const Waits wait{&B.bail};
   auto chunk = [&](int i) { return c0 + n - 1 - i; };  // the last first
   if (warp < ADD_SUM_WARP) {
+    // ---- w K, two groups of warps taking the chunks in turn: one's waits pass while the other computes
+    constexpr int GROUP = ADD_KW_WARPS * 32;
+    const int gt = tid % GROUP;
 #pragma unroll 1
-    for (int i = 0; i < n; ++i) {
+    for (int i = tid / GROUP; i < n; i += 2) {
       const int st = slot<ADD_STAGES>(i), m = len - chunk(i) * C;
       if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.full[st], phase<ADD_STAGES>(i), &B.kw_empty[i & 1], i / 2 + 1)) break;
       const float* w = dec + slot<RING>(i) * C;
       uint8_t* kw = smem + L::KW + (i & 1) * 3 * L::K_BYTES;
 #pragma unroll 2
-      for (int j = tid; j < C * DK / 8; j += ADD_SUM_WARP * 32) {
+      for (int j = gt; j < C * DK / 8; j += GROUP) {
         const int r = (j * 16 % HALF) / 128;
         split_piece(smem + st * L::STAGE + 16 * j, w[r], r < m, kw + 16 * j, L::K_BYTES);
       }
-      if (m < C) clear_values(smem + st * L::STAGE + L::K_BYTES, m, tid, ADD_SUM_WARP * 32);
+      if (m < C) clear_values(smem + st * L::STAGE + L::K_BYTES, m, gt, GROUP);
       fence_async();
       arrive(&B.kw_full[i & 1]);
       arrive(&B.empty[st]);
