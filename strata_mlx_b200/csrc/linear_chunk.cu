@@ -3,10 +3,11 @@
 //   out_i = scale ( e^{G_i} q_i S + sum_{j <= i} e^{G_i - G_j} (q_i . k_j) v_j )
 //   S'    = e^{G_63} S + sum_j e^{G_63 - G_j} k_j v_j^T
 // four products a chunk, with the state transposed so that value dimensions are the products' 128 rows:
-//   A = Q K^T             (64 x 64)     -> P: times e^{G_i - G_j}, zero above the diagonal, rounded to bfloat16
-//   I = V^T P^T           (128 x 64)    the chunk's own part of the outputs
-//   X = S^T Q^T           (128 x 64)    the state's part; S^T from tensor memory as two bfloat16 terms (its rounding
-//                                       and the rest), so that of the outputs only P and the result are rounded
+//   A = Q K^T             (64 x 64)     -> P: times e^{G_i - G_j}, zero above the diagonal
+//   I = V^T P^T           (128 x 64)    the chunk's own part of the outputs; P as two bfloat16 terms, its rounding and
+//                                       what that left (one term alone made the outputs' error 1.4 times their rounding)
+//   X = S^T Q^T           (128 x 64)    the state's part; S^T from tensor memory as two terms too, so that of the
+//                                       outputs only the result is rounded
 //   D = V^T (w K)         (128 x k_dim) what the chunk adds; w_j k_j as three bfloat16 terms, exact to 2^-24
 // The state stays in float32 registers: S = a S + D. A decay a near 1 enters as S + (a - 1) S, as its own rounding
 // would be repeated every chunk.
@@ -41,7 +42,7 @@ using namespace tc;
 constexpr int C = 64;        // tokens of a chunk
 // chunks of queries, keys and values held: scores are made a chunk ahead and a chunk's queries are needed until its
 // last products, keys until w K is made, values for the chunk's own products only
-constexpr int QS = 4, KS = 3, VS = 2;
+constexpr int QS = 3, KS = 3, VS = 2;
 constexpr int RING = 4;      // chunks whose decays are held
 constexpr int HALF = C * 128;  // bytes of 64 columns of a chunk's rows
 constexpr int THREADS = 24 * 32;
@@ -88,7 +89,7 @@ template <int DK>
 struct Shape {
   static constexpr int K_BYTES = DK / 64 * HALF, V_BYTES = 2 * HALF;
   static constexpr int Q = 0, K = Q + QS * K_BYTES, V = K + KS * K_BYTES, KW = V + VS * V_BYTES, P = KW + 3 * K_BYTES;
-  static constexpr int OUT = P + HALF, DEC = OUT + V_BYTES, BARS = DEC + RING * int(sizeof(Decays));
+  static constexpr int OUT = P + 2 * HALF, DEC = OUT + V_BYTES, BARS = DEC + RING * int(sizeof(Decays));
   static constexpr int BYTES = BARS + int(sizeof(Bars)) + 1024;  // and to align the start
 };
 template <int DK>
@@ -516,10 +517,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         wait_ld();
         fence_before();
         arrive(&B.a_empty);
-        uint32_t pk[16];
+        uint32_t pk[16], lo[16];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          pk[2 * j] = pk[2 * j + 1] = 0;
+          pk[2 * j] = pk[2 * j + 1] = lo[2 * j] = lo[2 * j + 1] = 0;
           if (8 * j > 16 * warp + 15) continue;  // above the diagonal
           const float2 gj = *reinterpret_cast<const float2*>(g2 + 8 * j + 2 * t);
           const int col = 8 * j + 2 * t;
@@ -529,14 +530,20 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
             x0 = col <= r0 ? x0 : 0.f, x1 = col + 1 <= r0 ? x1 : 0.f;
             y0 = col <= r0 + 8 ? y0 : 0.f, y1 = col + 1 <= r0 + 8 ? y1 : 0.f;
           }
-          pk[2 * j] = bits_of(__floats2bfloat162_rn(x0, x1)) ^ sign, pk[2 * j + 1] = bits_of(__floats2bfloat162_rn(y0, y1)) ^ sign;
+          const float2 x = make_float2(x0, x1), y = make_float2(y0, y1);
+          pk[2 * j] = rounded(x), pk[2 * j + 1] = rounded(y);
+          lo[2 * j] = rounded(rest(x, pk[2 * j])) ^ sign, lo[2 * j + 1] = rounded(rest(y, pk[2 * j + 1])) ^ sign;
+          pk[2 * j] ^= sign, pk[2 * j + 1] ^= sign;
         }
         arrive(&B.dec_empty[slot<RING>(i)]);
         if (!wait(&B.p_empty, i + 1)) break;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {  // r0 and r0 + 8 have one place in the swizzle
-          *reinterpret_cast<uint32_t*>(p + r0 * 128 + ((j ^ g) << 4) + 4 * t) = pk[2 * j];
-          *reinterpret_cast<uint32_t*>(p + (r0 + 8) * 128 + ((j ^ g) << 4) + 4 * t) = pk[2 * j + 1];
+          uint8_t* to = p + r0 * 128 + ((j ^ g) << 4) + 4 * t;
+          *reinterpret_cast<uint32_t*>(to) = pk[2 * j];
+          *reinterpret_cast<uint32_t*>(to + 8 * 128) = pk[2 * j + 1];
+          *reinterpret_cast<uint32_t*>(to + HALF) = lo[2 * j];
+          *reinterpret_cast<uint32_t*>(to + HALF + 8 * 128) = lo[2 * j + 1];
         }
         fence_async();
         arrive(&B.p_full);
@@ -865,9 +872,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       if (len - (c0 + i) * C < C && !(ok = wait(&B.kw_full[0], i))) break;  // the last chunk's values are cleared
       fence_after();
       if (leader) {
+        uint64_t pd = desc_k(smem + L::P + HALF);
+#pragma unroll 1
+        for (int term = 1; term >= 0; --term, pd -= HALF >> 4)  // the rest, then the rounded
 #pragma unroll
-        for (int s = 0; s < C / 16; ++s)
-          mma_ss(COL_I, vt + 128 * s, desc_k(smem + L::P) + 2 * s, idesc_bf16(128, 64, true, false), s > 0);
+          for (int s = 0; s < C / 16; ++s)
+            mma_ss(COL_I, vt + 128 * s, pd + 2 * s, idesc_bf16(128, 64, true, false), term < 1 || s > 0);
         commit(&B.o_full);
         commit(&B.p_empty);
         commit(&B.v_empty[slot<VS>(i)]);
