@@ -30,7 +30,7 @@ namespace da {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int HEADS = 8;       // query heads of a block: the products' N
-constexpr int BLOCKS_PER_SM = 2;
+constexpr int blocks_per_sm(int dp) { return dp == 256 ? 2 : 3; }
 constexpr int SMS = 148;
 constexpr float SLACK = 8.f;   // log2 by which a score may pass the running maximum
 constexpr int JOIN_THREADS = 256;
@@ -124,7 +124,7 @@ struct Split {
 };
 
 template <typename T, int DP, int SUB>
-__global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attend_kernel(const Args A) {
+__global__ void __launch_bounds__(THREADS, blocks_per_sm(DP)) attend_kernel(const Args A) {
   constexpr int KC = DP / 32, VC = DP / 64, TILE = 16 * SUB, UNIT = WARPS * TILE;
   constexpr int IDS = (TILE + 31) / 32;
   __shared__ uint4 s_q[KC][32];
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args A, int un
 
 // dimensions as the kernels are built for them, and the slots of a warp's tile: 16 KB of keys and values at each
 inline int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-inline int tile_of(int dp) { return dp == 64 ? 64 : dp == 128 ? 32 : 16; }
+inline int tile_of(int dp) { return dp == 64 ? 32 : 16; }
 
 struct Layout {
   int dp, unit, head_tiles, columns, pack;
@@ -612,7 +612,7 @@ inline Layout layout(const sc_kv_pages& c, int q_heads) {
   l.head_tiles = (group + HEADS - 1) / HEADS;
   for (l.pack = 1; l.pack < std::min(group, HEADS); l.pack *= 2) {}
   const int64_t slots = int64_t(c.max_pages) * c.page, units = int64_t(c.batch) * c.kv_heads * ceil_div(slots, l.unit);
-  l.columns = int(std::max<int64_t>(1, std::min<int64_t>(units, BLOCKS_PER_SM * SMS / l.head_tiles)));
+  l.columns = int(std::max<int64_t>(1, std::min<int64_t>(units, blocks_per_sm(l.dp) * SMS / l.head_tiles)));
   const size_t parts = size_t(l.head_tiles) * l.columns * 2 * HEADS;
   auto take = [&](size_t n) {
     const size_t at = l.bytes;
@@ -695,8 +695,8 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
   };
   auto typed = [&](auto t) -> int {
     using std::integral_constant;
-    if (l.dp == 64) return run(t, integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    if (l.dp == 128) return run(t, integral_constant<int, 128>{}, integral_constant<int, 2>{});
+    if (l.dp == 64) return run(t, integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    if (l.dp == 128) return run(t, integral_constant<int, 128>{}, integral_constant<int, 1>{});
     return run(t, integral_constant<int, 256>{}, integral_constant<int, 1>{});
   };
   return kv->dtype == SC_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
