@@ -28,9 +28,13 @@
 namespace sc {
 namespace da {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int HEADS = 8;       // query heads of a block: the products' N
-constexpr int blocks_per_sm(int dp) { return dp == 256 ? 2 : 3; }
+// Warps of a block and blocks of an SM, as many as the registers of a warp's tile leave room for. Heads of 256: one
+// block, as two of half as many warps write twice the partial results (one sequence of 8192: 16.1 us against 12.6).
+// Smaller heads: three, as fewer and larger ones leave more of the memory idle where runs end and start (a ragged batch:
+// 148 us with one block of 12 warps, 132 with two of 6 or three of 4; short sequences 10.0, 8.4 and 8.0).
+constexpr int warps_of(int dp) { return dp == 256 ? 8 : 4; }
+constexpr int blocks_per_sm(int dp) { return dp == 256 ? 1 : 3; }
 constexpr int SMS = 148;
 constexpr float SLACK = 8.f;   // log2 by which a score may pass the running maximum
 constexpr int JOIN_THREADS = 256;
@@ -124,11 +128,13 @@ struct Split {
 };
 
 template <typename T, int DP, int SUB>
-__global__ void __launch_bounds__(THREADS, blocks_per_sm(DP)) attend_kernel(const Args A) {
+__global__ void __launch_bounds__(warps_of(DP) * 32, blocks_per_sm(DP)) attend_kernel(const Args A) {
+  constexpr int WARPS = warps_of(DP), THREADS = WARPS * 32;
   constexpr int KC = DP / 32, VC = DP / 64, TILE = 16 * SUB, UNIT = WARPS * TILE;
   constexpr int IDS = (TILE + 31) / 32;
   __shared__ uint4 s_q[KC][32];
-  __shared__ __align__(16) float s_o[WARPS][HEADS][DP];
+  extern __shared__ __align__(16) float s_dyn[];
+  auto s_o = reinterpret_cast<float (*)[HEADS][DP]>(s_dyn);  // [WARPS]
   __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS];
   __shared__ int s_sum[WARPS], s_before, s_b;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -608,11 +614,11 @@ inline Layout layout(const sc_kv_pages& c, int q_heads) {
   Layout l{};
   const int group = q_heads / c.kv_heads;
   l.dp = padded(c.head_dim);
-  l.unit = WARPS * tile_of(l.dp);
+  l.unit = warps_of(l.dp) * tile_of(l.dp);
   l.head_tiles = (group + HEADS - 1) / HEADS;
   for (l.pack = 1; l.pack < std::min(group, HEADS); l.pack *= 2) {}
   const int64_t slots = int64_t(c.max_pages) * c.page, units = int64_t(c.batch) * c.kv_heads * ceil_div(slots, l.unit);
-  l.columns = int(std::max<int64_t>(1, std::min<int64_t>(units, blocks_per_sm(l.dp) * SMS / l.head_tiles)));
+  l.columns = int(std::max<int64_t>(1, std::min<int64_t>(units, std::max(1, blocks_per_sm(l.dp) * SMS / l.head_tiles))));
   const size_t parts = size_t(l.head_tiles) * l.columns * 2 * HEADS;
   auto take = [&](size_t n) {
     const size_t at = l.bytes;
@@ -674,7 +680,10 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
   auto run = [&](auto t, auto dp, auto sub) -> int {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value, SUB = decltype(sub)::value;
-    da::attend_kernel<T, DP, SUB><<<dim3(unsigned(l.columns), unsigned(l.head_tiles)), da::THREADS, 0, s>>>(A);
+    constexpr int warps = da::warps_of(DP), smem = warps * da::HEADS * DP * 4;
+    const auto attend = da::attend_kernel<T, DP, SUB>;
+    if (int rc = raise_smem(reinterpret_cast<const void*>(attend), smem, "decode attention smem attribute")) return rc;
+    attend<<<dim3(unsigned(l.columns), unsigned(l.head_tiles)), warps * 32, smem, s>>>(A);
     // programmatic dependent launch: the joining blocks are placed as the attention's leave
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(join_blocks));
