@@ -7,6 +7,9 @@ router, top-k and combine around them) rebuilt for the B200.
                              memory over NVLink (peer stores), or NCCL all-gather + all-reduce
     strata_mlx_b200.paged    experts within a device-memory budget, read from the GGUF file as routes ask
                              (strata_mlx/paged.py)
+    strata_mlx_b200.context  what a decoder keeps of its context: attention over a batch's paged cache, eviction by
+                             attention weight, linear attention with a decay
+    strata_mlx_b200.hybrid   a small decoder on those operators
     include/strata_cuda.h    the C ABI of libstrata_cuda.so underneath
 
 The package is importable without a GPU; the kernels need one (sm_100a).

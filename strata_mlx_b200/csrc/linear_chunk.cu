@@ -717,179 +717,179 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       arrive(&B.dec_empty[slot<RING>(i)]);
     }
   } else {
-  fewer_registers<CONTROL_REGS>();
-  if (warp == DECAY_WARP) {
-    // ---- a chunk's decays: a lane tokens 2 lane and 2 lane + 1, sums from the front and from the back
-    const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
-    float2 next = two_decays(decay, a.decay_token, c0 * C, n ? len : 0);
-    auto decays = [&](int i) -> bool {
-      const float g0 = next.x, g1 = next.y, pair = g0 + g1;
-      if (i + 1 < n) next = two_decays(decay, a.decay_token, (c0 + i + 1) * C, len);
-      float up = pair, down = pair;
+    fewer_registers<CONTROL_REGS>();
+    if (warp == DECAY_WARP) {
+      // ---- a chunk's decays: a lane tokens 2 lane and 2 lane + 1, sums from the front and from the back
+      const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
+      float2 next = two_decays(decay, a.decay_token, c0 * C, n ? len : 0);
+      auto decays = [&](int i) -> bool {
+        const float g0 = next.x, g1 = next.y, pair = g0 + g1;
+        if (i + 1 < n) next = two_decays(decay, a.decay_token, (c0 + i + 1) * C, len);
+        float up = pair, down = pair;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const float x = __shfl_up_sync(0xffffffffu, up, o), y = __shfl_down_sync(0xffffffffu, down, o);
-        if (lane >= o) up += x;
-        if (lane + o < 32) down += y;
-      }
-      float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
-      if (lane == 0) before = 0.f;
-      if (lane == 31) after = 0.f;
-      constexpr float LOG2E = 1.4426950408889634f;
-      const float e0 = (before + g0) * LOG2E, e1 = up * LOG2E;
-      Decays& D = dec[slot<RING>(i)];
-      if (!wait(&B.dec_empty[slot<RING>(i)], phase<RING>(i) + 1)) return false;
-      *reinterpret_cast<float2*>(&D.g2[2 * lane]) = make_float2(e0, e1);
-      *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(fast_exp2(e0) * a.scale, fast_exp2(e1) * a.scale);
-      *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(fast_exp2((after + g1) * LOG2E), fast_exp2(after * LOG2E));
-      if (lane == 31) {
-        const bool near = up > -0.69314718f;
-        D.a = near ? expm1_near(up) : fast_exp2(e1), D.one = near ? 1.f : 0.f;
-      }
-      arrive(&B.dec_full[slot<RING>(i)]);
-      return true;
-    };
-    const bool leader = elect_one();
-    int i = -1;  // the decays a chunk ahead of the values
-#pragma unroll 1
-    for (; i < n; ++i) {
-      if (i + 1 < n && !decays(i + 1)) break;
-      if (i < 0) continue;
-      if (!wait(&B.v_empty[slot<VS>(i)], phase<VS>(i) + 1)) break;
-      if (leader) {
-        mbar_arrive_expect_tx(&B.v_full[slot<VS>(i)], (a.v_dim > 64 ? 2 : 1) * HALF);
-#pragma unroll 1
-        for (int x = 0; x < a.v_dim; x += 64)
-          tma_load(smem + L::V + slot<VS>(i) * L::V_BYTES + x / 64 * HALF, &maps.v, x, h, (c0 + i) * C, b, &B.v_full[slot<VS>(i)]);
-      }
-      __syncwarp();
-    }
-    if (leader)  // copies in flight land before the block may end
-#pragma unroll 1
-      for (int k = max(0, i - VS); k < i; ++k) mbar_wait(&B.v_full[slot<VS>(k)], uint32_t(phase<VS>(k)) & 1, nullptr, 20000000LL);
-    __syncwarp();
-  } else if (warp == LOAD_WARP) {
-    // ---- keys and queries
-    if (elect_one()) {
-      int i = 0;
+        for (int o = 1; o < 32; o <<= 1) {
+          const float x = __shfl_up_sync(0xffffffffu, up, o), y = __shfl_down_sync(0xffffffffu, down, o);
+          if (lane >= o) up += x;
+          if (lane + o < 32) down += y;
+        }
+        float before = __shfl_up_sync(0xffffffffu, up, 1), after = __shfl_down_sync(0xffffffffu, down, 1);
+        if (lane == 0) before = 0.f;
+        if (lane == 31) after = 0.f;
+        constexpr float LOG2E = 1.4426950408889634f;
+        const float e0 = (before + g0) * LOG2E, e1 = up * LOG2E;
+        Decays& D = dec[slot<RING>(i)];
+        if (!wait(&B.dec_empty[slot<RING>(i)], phase<RING>(i) + 1)) return false;
+        *reinterpret_cast<float2*>(&D.g2[2 * lane]) = make_float2(e0, e1);
+        *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(fast_exp2(e0) * a.scale, fast_exp2(e1) * a.scale);
+        *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(fast_exp2((after + g1) * LOG2E), fast_exp2(after * LOG2E));
+        if (lane == 31) {
+          const bool near = up > -0.69314718f;
+          D.a = near ? expm1_near(up) : fast_exp2(e1), D.one = near ? 1.f : 0.f;
+        }
+        arrive(&B.dec_full[slot<RING>(i)]);
+        return true;
+      };
+      const bool leader = elect_one();
+      int i = -1;  // the decays a chunk ahead of the values
 #pragma unroll 1
       for (; i < n; ++i) {
-        const int t0 = (c0 + i) * C, ks = slot<KS>(i), qs = slot<QS>(i);
-        if (!wait.alone(&B.k_empty[ks], phase<KS>(i) + 1)) break;
-        mbar_arrive_expect_tx(&B.k_full[ks], L::K_BYTES);
+        if (i + 1 < n && !decays(i + 1)) break;
+        if (i < 0) continue;
+        if (!wait(&B.v_empty[slot<VS>(i)], phase<VS>(i) + 1)) break;
+        if (leader) {
+          mbar_arrive_expect_tx(&B.v_full[slot<VS>(i)], (a.v_dim > 64 ? 2 : 1) * HALF);
 #pragma unroll 1
-        for (int x = 0; x < DK; x += 64) tma_load(smem + L::K + ks * L::K_BYTES + x / 64 * HALF, &maps.k, x, hk, t0, b, &B.k_full[ks]);
-        if (!wait.alone(&B.q_empty[qs], phase<QS>(i) + 1)) {
-          mbar_wait(&B.k_full[ks], uint32_t(phase<KS>(i)) & 1, nullptr, 20000000LL);
-          break;
+          for (int x = 0; x < a.v_dim; x += 64)
+            tma_load(smem + L::V + slot<VS>(i) * L::V_BYTES + x / 64 * HALF, &maps.v, x, h, (c0 + i) * C, b, &B.v_full[slot<VS>(i)]);
         }
-        mbar_arrive_expect_tx(&B.q_full[qs], L::K_BYTES);
-#pragma unroll 1
-        for (int x = 0; x < DK; x += 64) tma_load(smem + L::Q + qs * L::K_BYTES + x / 64 * HALF, &maps.q, x, hk, t0, b, &B.q_full[qs]);
+        __syncwarp();
       }
-      // copies in flight land before the block may end
+      if (leader)  // copies in flight land before the block may end
 #pragma unroll 1
-      for (int k = max(0, i - KS); k < i; ++k) mbar_wait(&B.k_full[slot<KS>(k)], uint32_t(phase<KS>(k)) & 1, nullptr, 20000000LL);
+        for (int k = max(0, i - VS); k < i; ++k) mbar_wait(&B.v_full[slot<VS>(k)], uint32_t(phase<VS>(k)) & 1, nullptr, 20000000LL);
+      __syncwarp();
+    } else if (warp == LOAD_WARP) {
+      // ---- keys and queries
+      if (elect_one()) {
+        int i = 0;
 #pragma unroll 1
-      for (int k = max(0, i - QS); k < i; ++k) mbar_wait(&B.q_full[slot<QS>(k)], uint32_t(phase<QS>(k)) & 1, nullptr, 20000000LL);
-    }
-    __syncwarp();
-  } else if (warp == SUM_WARP) {
-    // ---- D
-    const bool leader = elect_one();
-    const uint64_t kw = desc_mn(smem + L::KW, HALF);
+        for (; i < n; ++i) {
+          const int t0 = (c0 + i) * C, ks = slot<KS>(i), qs = slot<QS>(i);
+          if (!wait.alone(&B.k_empty[ks], phase<KS>(i) + 1)) break;
+          mbar_arrive_expect_tx(&B.k_full[ks], L::K_BYTES);
 #pragma unroll 1
-    for (int i = 0; i < n && tmem == 0; ++i) {
-      const uint64_t vt = desc_mn(smem + L::V + slot<VS>(i) * L::V_BYTES, HALF);
-      if (!wait(&B.v_full[slot<VS>(i)], phase<VS>(i), &B.d_empty, i + 1, &B.kw_full[0], i)) break;
-      fence_after();
-      if (leader) {
-        add_products<DK>(COL_D, vt, kw, 0, true);
-        commit(&B.kw_empty[0]);
+          for (int x = 0; x < DK; x += 64) tma_load(smem + L::K + ks * L::K_BYTES + x / 64 * HALF, &maps.k, x, hk, t0, b, &B.k_full[ks]);
+          if (!wait.alone(&B.q_empty[qs], phase<QS>(i) + 1)) {
+            mbar_wait(&B.k_full[ks], uint32_t(phase<KS>(i)) & 1, nullptr, 20000000LL);
+            break;
+          }
+          mbar_arrive_expect_tx(&B.q_full[qs], L::K_BYTES);
+#pragma unroll 1
+          for (int x = 0; x < DK; x += 64) tma_load(smem + L::Q + qs * L::K_BYTES + x / 64 * HALF, &maps.q, x, hk, t0, b, &B.q_full[qs]);
+        }
+        // copies in flight land before the block may end
+#pragma unroll 1
+        for (int k = max(0, i - KS); k < i; ++k) mbar_wait(&B.k_full[slot<KS>(k)], uint32_t(phase<KS>(k)) & 1, nullptr, 20000000LL);
+#pragma unroll 1
+        for (int k = max(0, i - QS); k < i; ++k) mbar_wait(&B.q_full[slot<QS>(k)], uint32_t(phase<QS>(k)) & 1, nullptr, 20000000LL);
       }
       __syncwarp();
-      if (!wait(&B.kw_full[1], i)) break;
-      fence_after();
-      if (leader) {
-        add_products<DK>(COL_D, vt, kw, 1, false);
-        commit(&B.d_full);
-        commit(&B.kw_empty[1]);
-        commit(&B.v_empty[slot<VS>(i)]);
-      }
-      __syncwarp();
-    }
-    if (leader) commit(&B.done);
-    __syncwarp();
-  } else if (warp == MMA_WARP) {
-    // ---- the products. The whole warp follows the loop, so that what a product is given is uniform; one lane issues.
-    // All 512 columns are this block's, so tensor memory starts at address 0.
-    const bool leader = elect_one();
-    auto a_product = [&](int i) {
-      const uint8_t *q = smem + L::Q + slot<QS>(i) * L::K_BYTES, *k = smem + L::K + slot<KS>(i) * L::K_BYTES;
-      if (leader) {
-        uint64_t qd = desc_k(q), kd = desc_k(k);
+    } else if (warp == SUM_WARP) {
+      // ---- D
+      const bool leader = elect_one();
+      const uint64_t kw = desc_mn(smem + L::KW, HALF);
 #pragma unroll 1
-        for (int x = 0; x < DK / 64; ++x, qd += HALF >> 4, kd += HALF >> 4)
-#pragma unroll
-          for (int s = 0; s < 4; ++s) mma_ss(COL_A, qd + 2 * s, kd + 2 * s, idesc_bf16(64, 64, false, false), x > 0 || s > 0);
-        commit(&B.a_full);
-        commit(&B.k_empty[slot<KS>(i)]);
-      }
-      __syncwarp();
-    };
-    bool ok = tmem == 0;
-    if (!ok) wait.stop();
-    if (n > 0 && ok && (ok = wait(&B.q_full[0], 0, &B.k_full[0], 0))) {
-      fence_after();
-      a_product(0);
-    }
-#pragma unroll 1
-    for (int i = 0; i < n && ok; ++i) {
-      const uint64_t vt = desc_mn(smem + L::V + slot<VS>(i) * L::V_BYTES, HALF);
-      if (i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
-        const int j = i + 1;
-        if (!(ok = wait(&B.q_full[slot<QS>(j)], phase<QS>(j), &B.k_full[slot<KS>(j)], phase<KS>(j), &B.a_empty, i))) break;
+      for (int i = 0; i < n && tmem == 0; ++i) {
+        const uint64_t vt = desc_mn(smem + L::V + slot<VS>(i) * L::V_BYTES, HALF);
+        if (!wait(&B.v_full[slot<VS>(i)], phase<VS>(i), &B.d_empty, i + 1, &B.kw_full[0], i)) break;
         fence_after();
-        a_product(j);
-      }
-      if (!(ok = wait(&B.s_full, i))) break;
-      fence_after();
-      if (leader) {
-        const uint64_t qd = desc_k(smem + L::Q + slot<QS>(i) * L::K_BYTES);
-#pragma unroll 1
-        for (int e = 2 * (DK / 64) - 1; e >= 0; --e) {  // the rest, then the rounded state; 64 key dimensions each
-          const int x = e % (DK / 64);
-#pragma unroll
-          for (int s = 0; s < 4; ++s)
-            mma_ts(col_x(i), COL_S + 32 * e + 8 * s, qd + uint32_t(x * (HALF >> 4) + 2 * s), idesc_bf16(128, 64, false, false),
-                   e < 2 * (DK / 64) - 1 || s > 0);
+        if (leader) {
+          add_products<DK>(COL_D, vt, kw, 0, true);
+          commit(&B.kw_empty[0]);
         }
-        commit(&B.s_empty);
-        commit(&B.q_empty[slot<QS>(i)]);
+        __syncwarp();
+        if (!wait(&B.kw_full[1], i)) break;
+        fence_after();
+        if (leader) {
+          add_products<DK>(COL_D, vt, kw, 1, false);
+          commit(&B.d_full);
+          commit(&B.kw_empty[1]);
+          commit(&B.v_empty[slot<VS>(i)]);
+        }
+        __syncwarp();
       }
+      if (leader) commit(&B.done);
       __syncwarp();
-      if (!(ok = wait(&B.p_full, i, &B.v_full[slot<VS>(i)], phase<VS>(i), &B.o_empty, i + 1))) break;
-      if (len - (c0 + i) * C < C && !(ok = wait(&B.kw_full[0], i))) break;  // the last chunk's values are cleared
-      fence_after();
-      if (leader) {
-        uint64_t pd = desc_k(smem + L::P + HALF);
+    } else if (warp == MMA_WARP) {
+      // ---- the products. The whole warp follows the loop, so that what a product is given is uniform; one lane issues.
+      // All 512 columns are this block's, so tensor memory starts at address 0.
+      const bool leader = elect_one();
+      auto a_product = [&](int i) {
+        const uint8_t *q = smem + L::Q + slot<QS>(i) * L::K_BYTES, *k = smem + L::K + slot<KS>(i) * L::K_BYTES;
+        if (leader) {
+          uint64_t qd = desc_k(q), kd = desc_k(k);
 #pragma unroll 1
-        for (int term = 1; term >= 0; --term, pd -= HALF >> 4)  // the rest, then the rounded
+          for (int x = 0; x < DK / 64; ++x, qd += HALF >> 4, kd += HALF >> 4)
 #pragma unroll
-          for (int s = 0; s < C / 16; ++s)
-            mma_ss(COL_I, vt + 128 * s, pd + 2 * s, idesc_bf16(128, 64, true, false), term < 1 || s > 0);
-        commit(&B.o_full);
-        commit(&B.p_empty);
-        commit(&B.v_empty[slot<VS>(i)]);
+            for (int s = 0; s < 4; ++s) mma_ss(COL_A, qd + 2 * s, kd + 2 * s, idesc_bf16(64, 64, false, false), x > 0 || s > 0);
+          commit(&B.a_full);
+          commit(&B.k_empty[slot<KS>(i)]);
+        }
+        __syncwarp();
+      };
+      bool ok = tmem == 0;
+      if (!ok) wait.stop();
+      if (n > 0 && ok && (ok = wait(&B.q_full[0], 0, &B.k_full[0], 0))) {
+        fence_after();
+        a_product(0);
+      }
+#pragma unroll 1
+      for (int i = 0; i < n && ok; ++i) {
+        const uint64_t vt = desc_mn(smem + L::V + slot<VS>(i) * L::V_BYTES, HALF);
+        if (i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
+          const int j = i + 1;
+          if (!(ok = wait(&B.q_full[slot<QS>(j)], phase<QS>(j), &B.k_full[slot<KS>(j)], phase<KS>(j), &B.a_empty, i))) break;
+          fence_after();
+          a_product(j);
+        }
+        if (!(ok = wait(&B.s_full, i))) break;
+        fence_after();
+        if (leader) {
+          const uint64_t qd = desc_k(smem + L::Q + slot<QS>(i) * L::K_BYTES);
+#pragma unroll 1
+          for (int e = 2 * (DK / 64) - 1; e >= 0; --e) {  // the rest, then the rounded state; 64 key dimensions each
+            const int x = e % (DK / 64);
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              mma_ts(col_x(i), COL_S + 32 * e + 8 * s, qd + uint32_t(x * (HALF >> 4) + 2 * s), idesc_bf16(128, 64, false, false),
+                     e < 2 * (DK / 64) - 1 || s > 0);
+          }
+          commit(&B.s_empty);
+          commit(&B.q_empty[slot<QS>(i)]);
+        }
+        __syncwarp();
+        if (!(ok = wait(&B.p_full, i, &B.v_full[slot<VS>(i)], phase<VS>(i), &B.o_empty, i + 1))) break;
+        if (len - (c0 + i) * C < C && !(ok = wait(&B.kw_full[0], i))) break;  // the last chunk's values are cleared
+        fence_after();
+        if (leader) {
+          uint64_t pd = desc_k(smem + L::P + HALF);
+#pragma unroll 1
+          for (int term = 1; term >= 0; --term, pd -= HALF >> 4)  // the rest, then the rounded
+#pragma unroll
+            for (int s = 0; s < C / 16; ++s)
+              mma_ss(COL_I, vt + 128 * s, pd + 2 * s, idesc_bf16(128, 64, true, false), term < 1 || s > 0);
+          commit(&B.o_full);
+          commit(&B.p_empty);
+          commit(&B.v_empty[slot<VS>(i)]);
+        }
+        __syncwarp();
+      }
+      if (leader) {
+        commit(&B.done);  // every product issued has finished
+        mbar_wait(&B.done, 0, nullptr, 20000000LL);
       }
       __syncwarp();
     }
-    if (leader) {
-      commit(&B.done);  // every product issued has finished
-      mbar_wait(&B.done, 0, nullptr, 20000000LL);
-    }
-    __syncwarp();
-  }
   }
   fence_before();
   __syncthreads();

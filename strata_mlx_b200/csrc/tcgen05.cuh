@@ -71,14 +71,7 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 columns of this thread's lane (a warp reads the 32 lanes of its quarter); wait_ld before the registers are used
-__device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : SC_R8(r, 0), SC_R8(r, 8), SC_R8(r, 16), SC_R8(r, 24)
-      : "r"(addr));
-}
+// 16 columns of this thread's lane (a warp reads the 32 lanes of its quarter); wait_ld before the registers are used
 __device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
@@ -106,13 +99,6 @@ __device__ __forceinline__ void ld_frag32(uint32_t addr, uint32_t (&r)[16]) {
 __device__ __forceinline__ void st8(uint32_t addr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), SC_W8(r, 0)
                : "memory");
-}
-__device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};" ::"r"(addr),
-      SC_W8(r, 0), SC_W8(r, 8)
-      : "memory");
 }
 #undef SC_R8
 #undef SC_W8
