@@ -44,6 +44,7 @@ constexpr int C = 64;        // tokens of a chunk
 // last products, keys until w K is made, values for the chunk's own products only
 constexpr int QS = 3, KS = 3, VS = 2;
 constexpr int RING = 4;      // chunks whose decays are held
+constexpr int AHEAD = 8;     // and those whose decays are fetched ahead
 constexpr int HALF = C * 128;  // bytes of 64 columns of a chunk's rows
 constexpr int THREADS = 24 * 32;
 constexpr int OUT_WARP = 4, STATE_WARP = 8, KW_WARP = 16, MMA_WARP = 20, DECAY_WARP = 21, LOAD_WARP = 22, SUM_WARP = 23;
@@ -52,6 +53,7 @@ constexpr int P_REGS = 64, OUT_REGS = 56, STATE_REGS = 120, KW_REGS = 72, CONTRO
 static_assert(P_REGS + OUT_REGS + 2 * STATE_REGS + KW_REGS + CONTROL_REGS == 6 * 80, "a block's registers");
 // the first launch's: 12 warps make w K, 8 add up D, 3 control
 constexpr int ADD_SUM_WARP = 12, ADD_KW_WARPS = 6, ADD_STAGES = 4, ADD_RUN = 8;  // chunks whose D adds up in tensor memory
+constexpr int ADD_RING = 6, ADD_AHEAD = 3;  // chunks whose decays, then weights are held, and of them those fetched ahead
 constexpr int SUM_REGS = 96;
 static_assert(3 * 80 + 2 * SUM_REGS + CONTROL_REGS <= 6 * 80, "a block's registers");
 constexpr int SMS = 148;
@@ -75,7 +77,7 @@ struct Bars {
 };
 
 struct AddBars {
-  uint64_t full[ADD_STAGES], empty[ADD_STAGES], dec_full[RING], dec_empty[RING], kw_full[2], kw_empty[2], d_full[2],
+  uint64_t full[ADD_STAGES], empty[ADD_STAGES], dec_full[ADD_RING], dec_empty[ADD_RING], kw_full[2], kw_empty[2], d_full[2],
       d_empty[2], done;
   uint32_t tmem;
   int bail;
@@ -89,13 +91,14 @@ template <int DK>
 struct Shape {
   static constexpr int K_BYTES = DK / 64 * HALF, V_BYTES = 2 * HALF;
   static constexpr int Q = 0, K = Q + QS * K_BYTES, V = K + KS * K_BYTES, KW = V + VS * V_BYTES, P = KW + 3 * K_BYTES;
-  static constexpr int OUT = P + 2 * HALF, DEC = OUT + V_BYTES, BARS = DEC + RING * int(sizeof(Decays));
+  static constexpr int OUT = P + 2 * HALF, DEC = OUT + V_BYTES, RAW = DEC + RING * int(sizeof(Decays));
+  static constexpr int BARS = RAW + AHEAD * C * 4;
   static constexpr int BYTES = BARS + int(sizeof(Bars)) + 1024;  // and to align the start
 };
 template <int DK>
 struct AddShape {
   static constexpr int K_BYTES = DK / 64 * HALF, V_BYTES = 2 * HALF, STAGE = K_BYTES + V_BYTES;
-  static constexpr int KW = ADD_STAGES * STAGE, DEC = KW + 2 * 3 * K_BYTES, BARS = DEC + RING * C * 4;
+  static constexpr int KW = ADD_STAGES * STAGE, DEC = KW + 2 * 3 * K_BYTES, BARS = DEC + ADD_RING * C * 4;
   static constexpr int BYTES = BARS + int(sizeof(AddBars)) + 1024;
 };
 
@@ -292,10 +295,26 @@ __device__ __forceinline__ void add_products(uint32_t d, uint64_t v, uint64_t kw
   }
 }
 
-// a lane's two decays of a chunk: tokens 2 lane and 2 lane + 1 from t0 on
-__device__ __forceinline__ float2 two_decays(const float* decay, int64_t token, int t0, int len) {
-  const int t = t0 + 2 * (threadIdx.x & 31);
-  return make_float2(t < len ? fmaxf(decay[t * token], LEAST) : 0.f, t + 1 < len ? fmaxf(decay[(t + 1) * token], LEAST) : 0.f);
+// A chunk's decays on their way to shared memory, a lane tokens 2 lane and 2 lane + 1 from t0 on; zeros past the length.
+// Several chunks' are under way: with one, its trip to memory (2,000 cycles under load) was what a chunk took.
+__device__ __forceinline__ void fetch_decays(float* place, const float* decay, int64_t token, int t0, int len) {
+  const int lane = threadIdx.x & 31, t = t0 + 2 * lane;
+  const uint32_t to = smem_u32(place + 2 * lane);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const bool in = t + e < len;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4 * e), "l"(decay + (in ? (t + e) * token : 0)),
+                 "r"(in ? 4 : 0)
+                 : "memory");
+  }
+}
+__device__ __forceinline__ void close_fetch() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// those of the oldest chunk under way, `Behind` chunks being behind it
+template <int Behind>
+__device__ __forceinline__ float2 fetched(const float* place) {
+  asm volatile("cp.async.wait_group %0;" ::"n"(Behind) : "memory");
+  const float2 g = *reinterpret_cast<const float2*>(place + 2 * (threadIdx.x & 31));
+  return make_float2(fmaxf(g.x, LEAST), fmaxf(g.y, LEAST));
 }
 
 // What a segment adds to the state, and its decay.
@@ -305,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
   extern __shared__ uint8_t raw[];
   // 1024-byte aligned, by an offset: through an integer the pointer would no longer be known to be shared memory's
   uint8_t* smem = raw + (0u - smem_u32(raw) & 1023u);
-  float* dec = reinterpret_cast<float*>(smem + L::DEC);  // (RING, C) weights
+  float* dec = reinterpret_cast<float*>(smem + L::DEC);  // (ADD_RING, C) decays, then weights
   AddBars& B = *reinterpret_cast<AddBars*>(smem + L::BARS);
   const sc_linear& a = A.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -315,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
   pdl_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < ADD_STAGES; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], ADD_KW_WARPS + 1);
-    for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], ADD_KW_WARPS);
+    for (int i = 0; i < ADD_RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], ADD_KW_WARPS);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&B.kw_full[i], ADD_KW_WARPS), mbar_init(&B.kw_empty[i], 1);
       mbar_init(&B.d_full[i], 1), mbar_init(&B.d_empty[i], 8);
@@ -339,8 +358,8 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
 #pragma unroll 1
     for (int i = tid / GROUP; i < n; i += 2) {
       const int st = slot<ADD_STAGES>(i), m = len - chunk(i) * C;
-      if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.full[st], phase<ADD_STAGES>(i), &B.kw_empty[i & 1], i / 2 + 1)) break;
-      const float* w = dec + slot<RING>(i) * C;
+      if (!wait(&B.dec_full[slot<ADD_RING>(i)], phase<ADD_RING>(i), &B.full[st], phase<ADD_STAGES>(i), &B.kw_empty[i & 1], i / 2 + 1)) break;
+      const float* w = dec + slot<ADD_RING>(i) * C;
       uint8_t* kw = smem + L::KW + (i & 1) * 3 * L::K_BYTES;
 #pragma unroll 2
       for (int j = gt; j < C * DK / 8; j += GROUP) {
@@ -351,7 +370,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
       fence_async();
       arrive(&B.kw_full[i & 1]);
       arrive(&B.empty[st]);
-      arrive(&B.dec_empty[slot<RING>(i)]);
+      arrive(&B.dec_empty[slot<ADD_RING>(i)]);
     }
   } else if (warp < MMA_WARP) {
     // ---- the sums of ADD_RUN chunks into one
@@ -386,12 +405,20 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
       const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
       constexpr float LOG2E = 1.4426950408889634f;
       float later = 0.f;  // the decays of the chunks behind this one
-      float2 next = n ? two_decays(decay, a.decay_token, chunk(0) * C, len) : make_float2(0.f, 0.f);
-      bool ok = true;
+#pragma unroll 1
+      for (int i = 0; i < ADD_AHEAD; ++i) {
+        if (i < n) fetch_decays(dec + i * C, decay, a.decay_token, chunk(i) * C, len);
+        close_fetch();
+      }
 #pragma unroll 1
       for (int i = 0; i < n; ++i) {
-        const float2 g = next;
-        if (i + 1 < n) next = two_decays(decay, a.decay_token, chunk(i + 1) * C, len);
+        const int j = i + ADD_AHEAD;
+        if (j < n) {
+          if (!wait(&B.dec_empty[slot<ADD_RING>(j)], phase<ADD_RING>(j) + 1)) break;
+          fetch_decays(dec + slot<ADD_RING>(j) * C, decay, a.decay_token, chunk(j) * C, len);
+        }
+        close_fetch();
+        const float2 g = fetched<ADD_AHEAD>(dec + slot<ADD_RING>(i) * C);
         float down = g.x + g.y;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -401,11 +428,11 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
         float after = __shfl_down_sync(0xffffffffu, down, 1);
         if (lane == 31) after = 0.f;
         after += later;
-        if (!(ok = wait(&B.dec_empty[slot<RING>(i)], phase<RING>(i) + 1))) break;
-        *reinterpret_cast<float2*>(dec + slot<RING>(i) * C + 2 * lane) = make_float2(fast_exp2((after + g.y) * LOG2E), fast_exp2(after * LOG2E));
+        *reinterpret_cast<float2*>(dec + slot<ADD_RING>(i) * C + 2 * lane) = make_float2(fast_exp2((after + g.y) * LOG2E), fast_exp2(after * LOG2E));
         later += __shfl_sync(0xffffffffu, down, 0);
-        arrive(&B.dec_full[slot<RING>(i)]);
+        arrive(&B.dec_full[slot<ADD_RING>(i)]);
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       if (lane == 0) A.logs[(int64_t(b) * a.v_heads + h) * A.segments + seg] = later;
     } else if (warp == LOAD_WARP) {
       if (elect_one()) {
@@ -721,10 +748,17 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     if (warp == DECAY_WARP) {
       // ---- a chunk's decays: a lane tokens 2 lane and 2 lane + 1, sums from the front and from the back
       const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
-      float2 next = two_decays(decay, a.decay_token, c0 * C, n ? len : 0);
+      float* got = reinterpret_cast<float*>(smem + L::RAW);
+#pragma unroll 1
+      for (int i = 0; i < AHEAD; ++i) {
+        if (i < n) fetch_decays(got + i * C, decay, a.decay_token, (c0 + i) * C, len);
+        close_fetch();
+      }
       auto decays = [&](int i) -> bool {
-        const float g0 = next.x, g1 = next.y, pair = g0 + g1;
-        if (i + 1 < n) next = two_decays(decay, a.decay_token, (c0 + i + 1) * C, len);
+        const float2 g = fetched<AHEAD - 1>(got + slot<AHEAD>(i) * C);
+        const float g0 = g.x, g1 = g.y, pair = g0 + g1;
+        if (i + AHEAD < n) fetch_decays(got + slot<AHEAD>(i) * C, decay, a.decay_token, (c0 + i + AHEAD) * C, len);
+        close_fetch();
         float up = pair, down = pair;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -764,6 +798,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         }
         __syncwarp();
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       if (leader)  // copies in flight land before the block may end
 #pragma unroll 1
         for (int k = max(0, i - VS); k < i; ++k) mbar_wait(&B.v_full[slot<VS>(k)], uint32_t(phase<VS>(k)) & 1, nullptr, 20000000LL);

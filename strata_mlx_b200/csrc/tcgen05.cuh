@@ -100,6 +100,15 @@ __device__ __forceinline__ void st8(uint32_t addr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), SC_W8(r, 0)
                : "memory");
 }
+// 16 lanes by 32 columns, from fragments of 8 x 8 pairs: thread (g, t) gives, for column 4 j + t, row g in r[2j] and row
+// g + 8 in r[2j + 1]
+__device__ __forceinline__ void st_frag32(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(addr),
+      SC_W8(r, 0), SC_W8(r, 8)
+      : "memory");
+}
 #undef SC_R8
 #undef SC_W8
 
