@@ -24,8 +24,12 @@
 // segment adds to the state, a second adds up the states before the segments, a third is the whole. The first takes a
 // segment's chunks from the last to the first, the weights w running on from chunk to chunk, so that D of eight chunks
 // adds up in tensor memory and no state is carried between them.
-// What bounds it: a chunk's loads and stores are 64 KB at 128 dimensions (1.5 us of an SM's share of the measured
-// copy), its products about 1,800 tensor cycles, and its conversions about 7,000 warp instructions.
+// What bounds it at 128 dimensions, a chunk: 64 KB of loads and stores (1.5 us of an SM's share of the measured copy),
+// 1,792 tensor cycles (A, of 64 rows, runs at half rate), 9,400 warp instructions (2,350 cycles of issue), and the chain
+// state -> its terms -> X -> state, which sets the pace: 3,500 cycles where a block is alone, 3,900 with all SMs at work.
+// A loop's code counts twice: 24 warps in eight roles share the instruction cache, and what does not fit is fetched
+// again every chunk (kernel of 116 KB: 282 us for 32768 tokens of 16 heads, 70 KB: 195, 61 KB: 184). So loops are rolled, an
+// operation stands in one place, and both halves of P run through the same code.
 // Every wait is bounded; one that gives up records SC_ERR_TIMEOUT and the block winds down.
 #include <algorithm>
 #include <type_traits>
@@ -69,7 +73,7 @@ struct Decays {
 };
 
 struct Bars {
-  uint64_t q_full[QS], q_empty[QS], k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], dec_full[RING], dec_empty[RING];
+  uint64_t qk_full[2][KS], qk_empty[2][KS], v_full[VS], v_empty[VS], dec_full[RING], dec_empty[RING];
   uint64_t a_full, a_empty, p_full, p_empty, o_full, o_empty, kw_full[2], kw_empty[2], d_full, d_empty, s_full, s_empty,
       done;
   uint32_t tmem;
@@ -503,8 +507,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
   const int c0 = seg * A.per, all = (a.tokens + C - 1) / C, c1 = min(all, c0 + A.per);
   const int n = max(0, min(c1, (len + C - 1) / C) - c0);  // this segment's chunks with tokens
   if (tid == 0) {
-    for (int i = 0; i < QS; ++i) mbar_init(&B.q_full[i], 1), mbar_init(&B.q_empty[i], 1);
-    for (int i = 0; i < KS; ++i) mbar_init(&B.k_full[i], 1), mbar_init(&B.k_empty[i], 4 + 1);
+    for (int i = 0; i < QS; ++i) mbar_init(&B.qk_full[0][i], 1), mbar_init(&B.qk_empty[0][i], 1);
+    for (int i = 0; i < KS; ++i) mbar_init(&B.qk_full[1][i], 1), mbar_init(&B.qk_empty[1][i], 4 + 1);
     for (int i = 0; i < VS; ++i) mbar_init(&B.v_full[i], 1), mbar_init(&B.v_empty[i], 2);
     for (int i = 0; i < RING; ++i) mbar_init(&B.dec_full[i], 1), mbar_init(&B.dec_empty[i], 20);
     mbar_init(&B.a_full, 1), mbar_init(&B.a_empty, 4), mbar_init(&B.p_full, 4), mbar_init(&B.p_empty, 1);
@@ -537,41 +541,47 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       for (int i = 0; i < n; ++i) {
         if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.a_full, i)) break;
         fence_after();
-        uint32_t r[32];
-        ld_frag64(lanes + COL_A, r);
         const float* g2 = dec[slot<RING>(i)].g2;
         const float ga = g2[r0] + shift, gb = g2[r0 + 8] + shift;
-        wait_ld();
-        fence_before();
-        arrive(&B.a_empty);
-        uint32_t pk[16], lo[16];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          pk[2 * j] = pk[2 * j + 1] = lo[2 * j] = lo[2 * j + 1] = 0;
-          if (8 * j > 16 * warp + 15) continue;  // above the diagonal
-          const float2 gj = *reinterpret_cast<const float2*>(g2 + 8 * j + 2 * t);
-          const int col = 8 * j + 2 * t;
-          float x0 = __uint_as_float(r[4 * j]) * fast_exp2(ga - gj.x), x1 = __uint_as_float(r[4 * j + 1]) * fast_exp2(ga - gj.y);
-          float y0 = __uint_as_float(r[4 * j + 2]) * fast_exp2(gb - gj.x), y1 = __uint_as_float(r[4 * j + 3]) * fast_exp2(gb - gj.y);
-          if (8 * j + 7 > 16 * warp) {  // on it
-            x0 = col <= r0 ? x0 : 0.f, x1 = col + 1 <= r0 ? x1 : 0.f;
-            y0 = col <= r0 + 8 ? y0 : 0.f, y1 = col + 1 <= r0 + 8 ? y1 : 0.f;
+        bool ok = true;
+#pragma unroll 1
+        for (int c = 0; c < C; c += 32) {  // half the columns
+          uint32_t r[16], pk[8], lo[8];
+          ld_frag32(lanes + COL_A + c, r);
+          wait_ld();
+          if (c > 0) {
+            fence_before();
+            arrive(&B.a_empty);
           }
-          const float2 x = make_float2(x0, x1), y = make_float2(y0, y1);
-          pk[2 * j] = rounded(x), pk[2 * j + 1] = rounded(y);
-          lo[2 * j] = rounded(rest(x, pk[2 * j])) ^ sign, lo[2 * j + 1] = rounded(rest(y, pk[2 * j + 1])) ^ sign;
-          pk[2 * j] ^= sign, pk[2 * j + 1] ^= sign;
-        }
-        arrive(&B.dec_empty[slot<RING>(i)]);
-        if (!wait(&B.p_empty, i + 1)) break;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {  // r0 and r0 + 8 have one place in the swizzle
-          uint8_t* to = p + r0 * 128 + ((j ^ g) << 4) + 4 * t;
-          *reinterpret_cast<uint32_t*>(to) = pk[2 * j];
-          *reinterpret_cast<uint32_t*>(to + 8 * 128) = pk[2 * j + 1];
-          *reinterpret_cast<uint32_t*>(to + HALF) = lo[2 * j];
-          *reinterpret_cast<uint32_t*>(to + HALF + 8 * 128) = lo[2 * j + 1];
+          for (int j = 0; j < 4; ++j) {
+            const int col = c + 8 * j + 2 * t;
+            pk[2 * j] = pk[2 * j + 1] = lo[2 * j] = lo[2 * j + 1] = 0;
+            if (c + 8 * j > 16 * warp + 15) continue;  // above the diagonal
+            const float2 gj = *reinterpret_cast<const float2*>(g2 + col);
+            float x0 = __uint_as_float(r[4 * j]) * fast_exp2(ga - gj.x), x1 = __uint_as_float(r[4 * j + 1]) * fast_exp2(ga - gj.y);
+            float y0 = __uint_as_float(r[4 * j + 2]) * fast_exp2(gb - gj.x), y1 = __uint_as_float(r[4 * j + 3]) * fast_exp2(gb - gj.y);
+            if (c + 8 * j + 7 > 16 * warp) {  // on it
+              x0 = col <= r0 ? x0 : 0.f, x1 = col + 1 <= r0 ? x1 : 0.f;
+              y0 = col <= r0 + 8 ? y0 : 0.f, y1 = col + 1 <= r0 + 8 ? y1 : 0.f;
+            }
+            const float2 x = make_float2(x0, x1), y = make_float2(y0, y1);
+            pk[2 * j] = rounded(x), pk[2 * j + 1] = rounded(y);
+            lo[2 * j] = rounded(rest(x, pk[2 * j])) ^ sign, lo[2 * j + 1] = rounded(rest(y, pk[2 * j + 1])) ^ sign;
+            pk[2 * j] ^= sign, pk[2 * j + 1] ^= sign;
+          }
+          if (c == 0 && !(ok = wait(&B.p_empty, i + 1))) break;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {  // r0 and r0 + 8 have one place in the swizzle
+            uint8_t* to = p + r0 * 128 + ((c / 8 + j ^ g) << 4) + 4 * t;
+            *reinterpret_cast<uint32_t*>(to) = pk[2 * j];
+            *reinterpret_cast<uint32_t*>(to + 8 * 128) = pk[2 * j + 1];
+            *reinterpret_cast<uint32_t*>(to + HALF) = lo[2 * j];
+            *reinterpret_cast<uint32_t*>(to + HALF + 8 * 128) = lo[2 * j + 1];
+          }
         }
+        if (!ok) break;
+        arrive(&B.dec_empty[slot<RING>(i)]);
         fence_async();
         arrive(&B.p_full);
       }
@@ -661,29 +671,32 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       S[k].y = there && k0 + 2 * k + 1 < kd ? *from : 0.f;
       from += ld;
     }
-    auto publish = [&] {  // S^T as two terms, the A operand of X
+    // S^T as two terms, the A operand of X. The first 16 are made while the last X still reads the old ones (one prompt
+    // of 32768 tokens of 16 heads: 183.7 us, with none 185.4, with half of them 184.4)
+    auto terms = [&](int k, uint32_t (&hi)[8], uint32_t (&lo)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        hi[e] = rounded(S[k / 2 + e]);
+        lo[e] = rounded(rest(S[k / 2 + e], hi[e]));
+      }
+    };
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      uint32_t hi[8], lo[8];
+      terms(0, hi, lo);
+      if (i > 0) {
+        if (!wait(&B.s_empty, i - 1)) break;
+        fence_after();
+      }
 #pragma unroll
       for (int k = 0; k < N; k += 16) {
-        uint32_t hi[8], lo[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          hi[e] = rounded(S[k / 2 + e]);
-          lo[e] = rounded(rest(S[k / 2 + e], hi[e]));
-        }
+        if (k > 0) terms(k, hi, lo);
         st8(lanes + COL_S + (k0 + k) / 2, hi);
         st8(lanes + COL_S + DK / 2 + (k0 + k) / 2, lo);
       }
       wait_st();
       fence_before();
       arrive(&B.s_full);
-    };
-#pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      if (i > 0) {
-        if (!wait(&B.s_empty, i - 1)) break;
-        fence_after();
-      }
-      publish();
       if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.d_full, i)) break;
       fence_after();
       const float2 d = make_float2(dec[slot<RING>(i)].a, dec[slot<RING>(i)].a), one = make_float2(dec[slot<RING>(i)].one, dec[slot<RING>(i)].one);
@@ -720,7 +733,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
       const int m = len - (c0 + i) * C;
-      if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.k_full[slot<KS>(i)], phase<KS>(i))) break;
+      if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.qk_full[1][slot<KS>(i)], phase<KS>(i))) break;
       const uint8_t* k = smem + L::K + slot<KS>(i) * L::K_BYTES;
       const float* w = dec[slot<RING>(i)].w;
       if (m < C) {
@@ -731,7 +744,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
 #pragma unroll 1
       for (int hf = 0; hf < 2; ++hf) {
         if (!(ok = wait(&B.kw_empty[hf], i + 1))) break;
-#pragma unroll 2
+#pragma unroll 1
         for (int j = lt; j < C / 2 * DK / 8; j += 128) {
           const int r = C / 2 * hf + j / 8 % (C / 2), at = j / (C / 2 * 8) * HALF + r * 128 + j % 8 * 16;
           split_piece(k + at, w[r], r < m, smem + L::KW + at, L::K_BYTES);
@@ -740,7 +753,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         arrive(&B.kw_full[hf]);
       }
       if (!ok) break;
-      arrive(&B.k_empty[slot<KS>(i)]);
+      arrive(&B.qk_empty[1][slot<KS>(i)]);
       arrive(&B.dec_empty[slot<RING>(i)]);
     }
   } else {
@@ -806,27 +819,21 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     } else if (warp == LOAD_WARP) {
       // ---- keys and queries
       if (elect_one()) {
-        int i = 0;
+        static_assert(QS == KS && L::K == L::Q + QS * L::K_BYTES, "queries' and keys' places");
+        int e = 0;
 #pragma unroll 1
-        for (; i < n; ++i) {
-          const int t0 = (c0 + i) * C, ks = slot<KS>(i), qs = slot<QS>(i);
-          if (!wait.alone(&B.k_empty[ks], phase<KS>(i) + 1)) break;
-          mbar_arrive_expect_tx(&B.k_full[ks], L::K_BYTES);
+        for (; e < 2 * n; ++e) {  // by turns
+          const int i = e >> 1, of = 1 - (e & 1), st = slot<KS>(i);
+          if (!wait.alone(&B.qk_empty[of][st], phase<KS>(i) + 1)) break;
+          mbar_arrive_expect_tx(&B.qk_full[of][st], L::K_BYTES);
 #pragma unroll 1
-          for (int x = 0; x < DK; x += 64) tma_load(smem + L::K + ks * L::K_BYTES + x / 64 * HALF, &maps.k, x, hk, t0, b, &B.k_full[ks]);
-          if (!wait.alone(&B.q_empty[qs], phase<QS>(i) + 1)) {
-            mbar_wait(&B.k_full[ks], uint32_t(phase<KS>(i)) & 1, nullptr, 20000000LL);
-            break;
-          }
-          mbar_arrive_expect_tx(&B.q_full[qs], L::K_BYTES);
-#pragma unroll 1
-          for (int x = 0; x < DK; x += 64) tma_load(smem + L::Q + qs * L::K_BYTES + x / 64 * HALF, &maps.q, x, hk, t0, b, &B.q_full[qs]);
+          for (int x = 0; x < DK; x += 64)
+            tma_load(smem + L::Q + (of * QS + st) * L::K_BYTES + x / 64 * HALF, of ? &maps.k : &maps.q, x, hk, (c0 + i) * C, b, &B.qk_full[of][st]);
         }
         // copies in flight land before the block may end
 #pragma unroll 1
-        for (int k = max(0, i - KS); k < i; ++k) mbar_wait(&B.k_full[slot<KS>(k)], uint32_t(phase<KS>(k)) & 1, nullptr, 20000000LL);
-#pragma unroll 1
-        for (int k = max(0, i - QS); k < i; ++k) mbar_wait(&B.q_full[slot<QS>(k)], uint32_t(phase<QS>(k)) & 1, nullptr, 20000000LL);
+        for (int k = max(0, e - 2 * KS); k < e; ++k)
+          mbar_wait(&B.qk_full[1 - (k & 1)][slot<KS>(k >> 1)], uint32_t(phase<KS>(k >> 1)) & 1, nullptr, 20000000LL);
       }
       __syncwarp();
     } else if (warp == SUM_WARP) {
@@ -836,22 +843,22 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
 #pragma unroll 1
       for (int i = 0; i < n && tmem == 0; ++i) {
         const uint64_t vt = desc_mn(smem + L::V + slot<VS>(i) * L::V_BYTES, HALF);
-        if (!wait(&B.v_full[slot<VS>(i)], phase<VS>(i), &B.d_empty, i + 1, &B.kw_full[0], i)) break;
-        fence_after();
-        if (leader) {
-          add_products<DK>(COL_D, vt, kw, 0, true);
-          commit(&B.kw_empty[0]);
+        bool ok = true;
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {
+          if (!(ok = wait(&B.v_full[slot<VS>(i)], phase<VS>(i), &B.d_empty, i + 1, &B.kw_full[hf], i))) break;
+          fence_after();
+          if (leader) {
+            add_products<DK>(COL_D, vt, kw, hf, hf == 0);
+            commit(&B.kw_empty[hf]);
+            if (hf > 0) {
+              commit(&B.d_full);
+              commit(&B.v_empty[slot<VS>(i)]);
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        if (!wait(&B.kw_full[1], i)) break;
-        fence_after();
-        if (leader) {
-          add_products<DK>(COL_D, vt, kw, 1, false);
-          commit(&B.d_full);
-          commit(&B.kw_empty[1]);
-          commit(&B.v_empty[slot<VS>(i)]);
-        }
-        __syncwarp();
+        if (!ok) break;
       }
       if (leader) commit(&B.done);
       __syncwarp();
@@ -868,41 +875,40 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
 #pragma unroll
             for (int s = 0; s < 4; ++s) mma_ss(COL_A, qd + 2 * s, kd + 2 * s, idesc_bf16(64, 64, false, false), x > 0 || s > 0);
           commit(&B.a_full);
-          commit(&B.k_empty[slot<KS>(i)]);
+          commit(&B.qk_empty[1][slot<KS>(i)]);
         }
         __syncwarp();
       };
       bool ok = tmem == 0;
       if (!ok) wait.stop();
-      if (n > 0 && ok && (ok = wait(&B.q_full[0], 0, &B.k_full[0], 0))) {
-        fence_after();
-        a_product(0);
-      }
 #pragma unroll 1
-      for (int i = 0; i < n && ok; ++i) {
+      for (int i = -1; i < n && ok; ++i) {
         const uint64_t vt = desc_mn(smem + L::V + slot<VS>(i) * L::V_BYTES, HALF);
         if (i + 1 < n) {  // ahead: P of the next chunk is made while this chunk's products run
           const int j = i + 1;
-          if (!(ok = wait(&B.q_full[slot<QS>(j)], phase<QS>(j), &B.k_full[slot<KS>(j)], phase<KS>(j), &B.a_empty, i))) break;
+          if (!(ok = wait(&B.qk_full[0][slot<QS>(j)], phase<QS>(j), &B.qk_full[1][slot<KS>(j)], phase<KS>(j), &B.a_empty, i))) break;
           fence_after();
           a_product(j);
         }
-        if (!(ok = wait(&B.s_full, i))) break;
-        fence_after();
-        if (leader) {
-          const uint64_t qd = desc_k(smem + L::Q + slot<QS>(i) * L::K_BYTES);
+        if (i >= 0) {
+          if (!(ok = wait(&B.s_full, i))) break;
+          fence_after();
+          if (leader) {
+            const uint64_t qd = desc_k(smem + L::Q + slot<QS>(i) * L::K_BYTES);
 #pragma unroll 1
-          for (int e = 2 * (DK / 64) - 1; e >= 0; --e) {  // the rest, then the rounded state; 64 key dimensions each
-            const int x = e % (DK / 64);
+            for (int e = 2 * (DK / 64) - 1; e >= 0; --e) {  // the rest, then the rounded state; 64 key dimensions each
+              const int x = e % (DK / 64);
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-              mma_ts(col_x(i), COL_S + 32 * e + 8 * s, qd + uint32_t(x * (HALF >> 4) + 2 * s), idesc_bf16(128, 64, false, false),
-                     e < 2 * (DK / 64) - 1 || s > 0);
+              for (int s = 0; s < 4; ++s)
+                mma_ts(col_x(i), COL_S + 32 * e + 8 * s, qd + uint32_t(x * (HALF >> 4) + 2 * s), idesc_bf16(128, 64, false, false),
+                       e < 2 * (DK / 64) - 1 || s > 0);
+            }
+            commit(&B.s_empty);
+            commit(&B.qk_empty[0][slot<QS>(i)]);
           }
-          commit(&B.s_empty);
-          commit(&B.q_empty[slot<QS>(i)]);
+          __syncwarp();
         }
-        __syncwarp();
+        if (i < 0) continue;
         if (!(ok = wait(&B.p_full, i, &B.v_full[slot<VS>(i)], phase<VS>(i), &B.o_empty, i + 1))) break;
         if (len - (c0 + i) * C < C && !(ok = wait(&B.kw_full[0], i))) break;  // the last chunk's values are cleared
         fence_after();

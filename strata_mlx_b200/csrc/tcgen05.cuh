@@ -79,16 +79,8 @@ __device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
       : SC_R8(r, 0), SC_R8(r, 8)
       : "r"(addr));
 }
-// 16 lanes by 64 columns, as accumulator fragments: thread (g, t) = (lane / 4, lane % 4) gets, for columns 8 j + 2t and
+// 16 lanes by 32 columns, as accumulator fragments: thread (g, t) = (lane / 4, lane % 4) gets, for columns 8 j + 2t and
 // + 1, row g in r[4j], r[4j + 1] and row g + 8 in r[4j + 2], r[4j + 3]
-__device__ __forceinline__ void ld_frag64(uint32_t addr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : SC_R8(r, 0), SC_R8(r, 8), SC_R8(r, 16), SC_R8(r, 24)
-      : "r"(addr));
-}
-// the same, 32 columns
 __device__ __forceinline__ void ld_frag32(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
@@ -99,15 +91,6 @@ __device__ __forceinline__ void ld_frag32(uint32_t addr, uint32_t (&r)[16]) {
 __device__ __forceinline__ void st8(uint32_t addr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), SC_W8(r, 0)
                : "memory");
-}
-// 16 lanes by 32 columns, from fragments of 8 x 8 pairs: thread (g, t) gives, for column 4 j + t, row g in r[2j] and row
-// g + 8 in r[2j + 1]
-__device__ __forceinline__ void st_frag32(uint32_t addr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};" ::"r"(addr),
-      SC_W8(r, 0), SC_W8(r, 8)
-      : "memory");
 }
 #undef SC_R8
 #undef SC_W8
