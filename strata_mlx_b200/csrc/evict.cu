@@ -4,13 +4,15 @@
 //                unsigned integer of the same order, the largest integer where its place keeps it; keys stay in shared
 //                memory. The key of the last slot that stays is found digit by digit below the bits that all keys
 //                share: a histogram of 512 digits a round in every block, summed over the cluster through distributed
-//                shared memory, until so few keys are left that they are ranked one against another. Then each warp counts and lists, in slot order, the holes (evicted slots below the
-//                budget) and the movers (kept slots past it): as many of one as of the other. Latency bounds it: a
-//                round is two barriers and a walk over the histogram.
+//                shared memory, until so few keys are left that they are ranked one against another. Then each warp
+//                counts and lists, in slot order, the holes (evicted slots below the budget) and the movers (kept
+//                slots past it): as many of one as of the other. Latency bounds it: a round is two barriers and a
+//                walk over the histogram (8 sequences of 131072 slots 25 us; with histograms of 2048 digits, of which
+//                every block reads 8 KB of each other's, 36).
 //   move_kernel  mover i's keys, values, weight and position into hole i. Sources lie at or past the budget and
 //                destinations below it, so no row is read that another warp writes, and the order is free. Bandwidth
 //                bounds it: a warp fetches the list entries and page ids of its rows at once and keeps four 16-byte
-//                words a lane in flight.
+//                words a lane in flight (8 sequences of 131072 slots to 32768: 132 us, the measured copy's rate).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -27,7 +29,6 @@ constexpr int BITS = 9, BINS = 1 << BITS;  // a digit a thread
 constexpr int FEW = 256;          // keys that are ranked one against another
 constexpr int MAX_CLUSTER = 8;
 constexpr int STRETCH = 128 * WARPS;  // a block's slots are a multiple
-constexpr int PER_BLOCK = 2 * STRETCH;  // slots of a block before the cluster grows
 constexpr int MOST = 50 * 1024;   // slots a block can hold the keys of (200 KB); past 8 such blocks keys are made anew
 constexpr int FETCH = 8;          // weights and positions a thread loads at a time
 constexpr int MOVE_WARPS = 8;
@@ -413,8 +414,11 @@ extern "C" int sc_evict(const sc_kv_pages* kv, const int32_t* seen, int keep, in
   A.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t slots = int64_t(kv->max_pages) * kv->page;
+  // One block up to two stretches of slots, where a cluster's barriers cost more than they share out (one sequence of
+  // 2304: 10.4 us, with two blocks 11.5; 64 of 4096: 32.9 and 34.0); past that a stretch a block (one of 8192: four
+  // blocks 14.4, one 16.5, eight 14.6; four of 32768: eight 26.1, four 28.7).
   int cluster = 1;
-  while (cluster < ev::MAX_CLUSTER && slots > int64_t(cluster) * ev::PER_BLOCK) cluster *= 2;
+  while (cluster < ev::MAX_CLUSTER && slots > int64_t(cluster > 1 ? cluster : 2) * ev::STRETCH) cluster *= 2;
   const int64_t hold = ceil_div(ceil_div(slots, cluster), ev::STRETCH) * ev::STRETCH;
   const bool held = hold <= ev::MOST;
   const int smem = held ? int(hold) * 4 : 0;

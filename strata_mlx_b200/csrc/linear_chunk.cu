@@ -966,16 +966,18 @@ __global__ void __launch_bounds__(256) scan_kernel(const Args A) {
 }
 
 // The segments that cost least, in chunks' time of an SM: waves of blocks times a segment's chunks (and about three
-// to start and end a block), the first launch's at three fifths, and the scan over the segments' states.
+// to start and end a block), the first launch's at three fifths, and the scan over the segments' states. Measured with 16
+// heads of one sequence: 512 tokens 18.8 us in four segments, 21.0 in one; 1024 20.4 in eight, 36.3 in one; 32768 174 in
+// nine, 355 in four, 192 in 18 (a second wave). 96 heads of 1536 tokens: 53 in one, 82 in two.
 inline int segments_of(const sc_linear& a) {
   const int64_t heads = int64_t(a.batch) * a.v_heads;
   const int chunks = int(ceil_div(a.tokens, C));
   int best = 1;
   double least = 1e30;
-  for (int s = 1; s <= std::max(1, std::min(chunks / 4, SMS)); ++s) {
+  for (int s = 1; s <= std::max(1, std::min(chunks / 2, SMS)); ++s) {
     const double per = double(ceil_div(chunks, s)) + 3;
     double cost = double(ceil_div(heads * s, SMS)) * per;
-    if (s > 1) cost += 0.6 * double(ceil_div(heads * (s - 1), SMS)) * per + 2 + 0.02 * double(heads * s);
+    if (s > 1) cost += 0.6 * double(ceil_div(heads * (s - 1), SMS)) * per + 1 + 0.02 * double(heads * s);
     if (cost < least) least = cost, best = s;
   }
   return best;
