@@ -237,7 +237,8 @@ EVICT = [  # lengths, keep, sinks, recent, kv_heads, head_dim, page, type
     ([100], 60, 4, 10, 2, 256, 16, BF), ([0, 1, 2, 3, 50], 2, 0, 0, 1, 64, 16, HF), ([500, 20, 300], 100, 4, 30, 3, 80, 8, BF),
     ([1000, 1024, 1025], 1000, 4, 996, 2, 64, 32, HF), ([5000, 1], 1234, 1, 0, 8, 8, 16, BF),
     ([40, 39], 0, 0, 0, 1, 64, 16, BF), ([33, 70], 200, 4, 10, 1, 64, 16, BF), ([140000, 9, 70001], 20011, 4, 128, 1, 8, 64, BF),
-    ([2304], 2048, 4, 256, 2, 256, 16, BF), ([4096] * 3, 1, 1, 0, 1, 16, 1, HF)]
+    ([2304], 2048, 4, 256, 2, 256, 16, BF), ([4096] * 3, 1, 1, 0, 1, 16, 1, HF),
+    ([8191, 30, 4097], 3001, 4, 500, 2, 64, 16, BF), ([10001, 16000], 9999, 0, 1, 1, 32, 16, HF)]
 
 
 @pytest.mark.parametrize("weights", ["spread", "equal", "odd"])
@@ -452,6 +453,14 @@ def test_linear_attention_of_ragged_prompts(cuda, lengths, dtype):
         assert (out[b, m:] == 0).all()
         if m == 0:
             assert torch.equal(state[b], args[4][b])
+
+
+def test_linear_attention_of_long_ragged_prompts(cuda):
+    lengths = [1100, 0, 513, 64]  # in several segments, most of them short or empty
+    args = make(4, 1100, 2, 2, 128, 128, BF, lengths=lengths)
+    out, state = context.linear_attention(*args[:4], state=args[4], lengths=args[5])
+    check_linear(clean(args), out, state)
+    assert all((out[b, m:] == 0).all() for b, m in enumerate(lengths)) and torch.equal(state[1], args[4][1])
 
 
 def test_linear_attention_of_views_and_nothing(cuda):
