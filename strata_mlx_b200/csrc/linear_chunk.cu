@@ -25,7 +25,7 @@
 // segment's chunks from the last to the first, the weights w running on from chunk to chunk, so that D of eight chunks
 // adds up in tensor memory and no state is carried between them.
 // What bounds it at 128 dimensions, a chunk: 64 KB of loads and stores (1.5 us of an SM's share of the measured copy),
-// 1,792 tensor cycles (A, of 64 rows, runs at half rate), 9,400 warp instructions (2,350 cycles of issue), and the chain
+// 1,792 tensor cycles (A, of 64 rows, runs at half rate), 9,600 warp instructions (2,400 cycles of issue), and the chain
 // state -> its terms -> X -> state, which sets the pace: 3,500 cycles where a block is alone, 3,900 with all SMs at work.
 // A loop's code counts twice: 24 warps in eight roles share the instruction cache, and what does not fit is fetched
 // again every chunk (kernel of 116 KB: 282 us for 32768 tokens of 16 heads, 70 KB: 195, 61 KB: 184). So loops are rolled, an
