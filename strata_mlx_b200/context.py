@@ -226,7 +226,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: t
     """A prompt (or a chunk of one) through linear attention: S_t = exp(decay_t) S_{t-1} + k_t v_t^T, out_t = scale
     q_t S_t. q, k (batch, tokens, k_heads, k_dim), v (batch, tokens, v_heads, v_dim): value head h reads key head
     h // (v_heads / k_heads); k_dim and v_dim multiples of 8 up to 128. decay (batch, tokens, v_heads) float32
-    logarithms, of any strides (a fixed decay a head is an expanded view). state (batch, v_heads, k_dim, v_dim)
+    logarithms of either sign, of any strides (a fixed decay a head is an expanded view). state (batch, v_heads, k_dim, v_dim)
     float32, zeros when None, is left as it was. lengths (batch,) int32: tokens past a sequence's length are not read,
     their outputs zeros. scale defaults to k_dim ** -0.5. Returns (out of v's shape, the state after the last token)."""
     q, k, v, sizes, index = _linear(q, k, v, decay, state, 4)

@@ -9,8 +9,8 @@
 //   X = S^T Q^T           (128 x 64)    the state's part; S^T from tensor memory as two terms too, so that of the
 //                                       outputs only the result is rounded
 //   D = V^T (w K)         (128 x k_dim) what the chunk adds; w_j k_j as three bfloat16 terms, exact to 2^-24
-// The state stays in float32 registers: S = a S + D. A decay a near 1 enters as S + (a - 1) S, as its own rounding
-// would be repeated every chunk.
+// The state stays in float32 registers: S = a S + D. A decay a near 1 (between a half and two) enters as S + (a - 1) S,
+// as its own rounding would be repeated every chunk.
 //
 // A block per (segment of the tokens, value head, sequence); 24 warps in six groups, each with its share of registers:
 //   0-3    P from A                             4-7    the outputs, stored by TMA through a tile in shared memory
@@ -152,7 +152,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
-// e^x - 1 for x in [-ln 2, 0], by its series to x^10 / 10!: within 2^-29 of it
+// e^x - 1 for x in [-ln 2, ln 2], by its series to x^10 / 10!: within 2^-28 of it
 __device__ __forceinline__ float expm1_near(float x) {
   float y = 1.f / 3628800.f;
   y = fmaf(y, x, 1.f / 362880.f);
@@ -790,8 +790,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(fast_exp2(e0) * a.scale, fast_exp2(e1) * a.scale);
         *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(fast_exp2((after + g1) * LOG2E), fast_exp2(after * LOG2E));
         if (lane == 31) {
-          const bool near = up > -0.69314718f;
-          D.a = near ? expm1_near(up) : fast_exp2(e1), D.one = near ? 1.f : 0.f;
+          const bool near = fabsf(up) < 0.69314718f;  // past it, growth included, a itself
+          D.a = near ? expm1_near(up) : expf(up), D.one = near ? 1.f : 0.f;
         }
         arrive(&B.dec_full[slot<RING>(i)]);
         return true;
