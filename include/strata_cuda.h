@@ -344,7 +344,8 @@ SC_API size_t sc_evict_workspace(const sc_kv_pages* kv, int keep);
  *   S_t = exp(decay_t) S_{t-1} + k_t v_t^T,   out_t = scale q_t S_t.
  * q, k (batch, tokens, k_heads, k_dim), v (batch, tokens, v_heads, v_dim), bfloat16 or float16, the last axis
  * adjacent; value head h reads key head h / (v_heads / k_heads). decay (batch, tokens, v_heads) float32 logarithms
- * (0 keeps, above 0 grows, -inf forgets), any strides, 0 among them. state_in (batch, v_heads, k_dim, v_dim) float32 contiguous, or
+ * (0 keeps, above 0 grows, below -104 forgets all; a NaN makes the outputs from its token on and the state NaN), any
+ * strides, 0 among them. state_in (batch, v_heads, k_dim, v_dim) float32 contiguous, or
  * NULL for zeros; state_out the same shape (may be state_in). lengths (batch) on the device, or NULL: tokens past a
  * sequence's length are not read and their outputs are zeros. out (batch, tokens, v_heads, v_dim) contiguous, of q's
  * type. k_dim and v_dim multiples of 8, at most 128. Strides of q, k, v multiples of 8, pointers 16-byte aligned. */

@@ -61,15 +61,19 @@ constexpr int ADD_RING = 6, ADD_AHEAD = 3;  // chunks whose decays, then weights
 constexpr int SUM_REGS = 96;
 static_assert(3 * 80 + 2 * SUM_REGS + CONTROL_REGS <= 6 * 80, "a block's registers");
 constexpr int SMS = 148;
-constexpr float LEAST = -30.f;  // a token's decay below e^-30 is taken as e^-30: past it nothing is left in float32
+constexpr float LEAST = -104.f;  // a token whose decay is below this is a reset: e^-104 is zero in float32
 
 // tensor memory columns
 constexpr uint32_t COL_A = 0, COL_I = 64, COL_D = 192, COL_S = 320;
 __device__ __forceinline__ uint32_t col_x(int i) { return i & 1 ? 448 : 128; }  // of chunk i: two, taken in turn
 
+// Resets count as 0 in the sums G, so that the other tokens' differences stay exact and finite; what a reset parts is set
+// to zero beside them: P by from[i], the scale e^{G_i} behind the first, the weights before the last, the chunk's a.
 struct Decays {
   float g2[C], eg[C], w[C];  // G_i log2(e), scale e^{G_i}, e^{G_63 - G_i}
   float a, one;              // the chunk's decay as S' = a S + one S + D
+  uint32_t resets, unused;   // whether the chunk has any
+  uint8_t from[C];           // where it has: the first token that token i sees, its own or the last reset's at or before i
 };
 
 struct Bars {
@@ -317,8 +321,15 @@ __device__ __forceinline__ void close_fetch() { asm volatile("cp.async.commit_gr
 template <int Behind>
 __device__ __forceinline__ float2 fetched(const float* place) {
   asm volatile("cp.async.wait_group %0;" ::"n"(Behind) : "memory");
-  const float2 g = *reinterpret_cast<const float2*>(place + 2 * (threadIdx.x & 31));
-  return make_float2(fmaxf(g.x, LEAST), fmaxf(g.y, LEAST));
+  return *reinterpret_cast<const float2*>(place + 2 * (threadIdx.x & 31));
+}
+// Takes the resets out of a lane's two decays; which lanes had one at their first token, and at their second. (A NaN is
+// none: it goes into the sums.)
+__device__ __forceinline__ uint2 take_resets(float2& g) {
+  const bool x = g.x < LEAST, y = g.y < LEAST;
+  if (x) g.x = 0.f;
+  if (y) g.y = 0.f;
+  return make_uint2(__ballot_sync(0xffffffffu, x), __ballot_sync(0xffffffffu, y));
 }
 
 // What a segment adds to the state, and its decay.
@@ -409,6 +420,7 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
       const float* decay = a.decay + b * a.decay_row + h * a.decay_head;
       constexpr float LOG2E = 1.4426950408889634f;
       float later = 0.f;  // the decays of the chunks behind this one
+      bool cut = false;   // and whether they hold a reset
 #pragma unroll 1
       for (int i = 0; i < ADD_AHEAD; ++i) {
         if (i < n) fetch_decays(dec + i * C, decay, a.decay_token, chunk(i) * C, len);
@@ -422,7 +434,8 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
           fetch_decays(dec + slot<ADD_RING>(j) * C, decay, a.decay_token, chunk(j) * C, len);
         }
         close_fetch();
-        const float2 g = fetched<ADD_AHEAD>(dec + slot<ADD_RING>(i) * C);
+        float2 g = fetched<ADD_AHEAD>(dec + slot<ADD_RING>(i) * C);
+        const uint2 reset = take_resets(g);
         float down = g.x + g.y;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -432,12 +445,19 @@ __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__
         float after = __shfl_down_sync(0xffffffffu, down, 1);
         if (lane == 31) after = 0.f;
         after += later;
-        *reinterpret_cast<float2*>(dec + slot<ADD_RING>(i) * C + 2 * lane) = make_float2(fast_exp2((after + g.y) * LOG2E), fast_exp2(after * LOG2E));
+        float2 w = make_float2(fast_exp2((after + g.y) * LOG2E), fast_exp2(after * LOG2E));
+        if (cut || (reset.x | reset.y)) {  // nothing of what came before a reset, unless it is NaN
+          const uint32_t behind = ~0u << lane;
+          if (cut || (reset.x & (behind << 1)) || (reset.y & behind)) w.x = 0.f * (after + g.y);
+          if (cut || ((reset.x | reset.y) & (behind << 1))) w.y = 0.f * after;
+          cut = true;
+        }
+        *reinterpret_cast<float2*>(dec + slot<ADD_RING>(i) * C + 2 * lane) = w;
         later += __shfl_sync(0xffffffffu, down, 0);
         arrive(&B.dec_full[slot<ADD_RING>(i)]);
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
-      if (lane == 0) A.logs[(int64_t(b) * a.v_heads + h) * A.segments + seg] = later;
+      if (lane == 0) A.logs[(int64_t(b) * a.v_heads + h) * A.segments + seg] = cut ? later * 0.f - INFINITY : later;
     } else if (warp == LOAD_WARP) {
       if (elect_one()) {
         const uint32_t bytes = uint32_t(L::K_BYTES + (a.v_dim > 64 ? 2 : 1) * HALF);
@@ -543,6 +563,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         fence_after();
         const float* g2 = dec[slot<RING>(i)].g2;
         const float ga = g2[r0] + shift, gb = g2[r0 + 8] + shift;
+        const bool cut = dec[slot<RING>(i)].resets != 0;
         bool ok = true;
 #pragma unroll 1
         for (int c = 0; c < C; c += 32) {  // half the columns
@@ -564,6 +585,11 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
             if (c + 8 * j + 7 > 16 * warp) {  // on it
               x0 = col <= r0 ? x0 : 0.f, x1 = col + 1 <= r0 ? x1 : 0.f;
               y0 = col <= r0 + 8 ? y0 : 0.f, y1 = col + 1 <= r0 + 8 ? y1 : 0.f;
+            }
+            if (cut) {  // what a reset parts
+              const int fa = dec[slot<RING>(i)].from[r0], fb = dec[slot<RING>(i)].from[r0 + 8];
+              x0 = col >= fa ? x0 : 0.f, x1 = col + 1 >= fa ? x1 : 0.f;
+              y0 = col >= fb ? y0 : 0.f, y1 = col + 1 >= fb ? y1 : 0.f;
             }
             const float2 x = make_float2(x0, x1), y = make_float2(y0, y1);
             pk[2 * j] = rounded(x), pk[2 * j + 1] = rounded(y);
@@ -768,7 +794,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         close_fetch();
       }
       auto decays = [&](int i) -> bool {
-        const float2 g = fetched<AHEAD - 1>(got + slot<AHEAD>(i) * C);
+        float2 g = fetched<AHEAD - 1>(got + slot<AHEAD>(i) * C);
+        const uint2 reset = take_resets(g);
         const float g0 = g.x, g1 = g.y, pair = g0 + g1;
         if (i + AHEAD < n) fetch_decays(got + slot<AHEAD>(i) * C, decay, a.decay_token, (c0 + i + AHEAD) * C, len);
         close_fetch();
@@ -786,12 +813,27 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
         const float e0 = (before + g0) * LOG2E, e1 = up * LOG2E;
         Decays& D = dec[slot<RING>(i)];
         if (!wait(&B.dec_empty[slot<RING>(i)], phase<RING>(i) + 1)) return false;
+        float2 eg = make_float2(fast_exp2(e0) * a.scale, fast_exp2(e1) * a.scale);
+        float2 w = make_float2(fast_exp2((after + g1) * LOG2E), fast_exp2(after * LOG2E));
+        const bool cut = (reset.x | reset.y) != 0;
+        if (cut) {  // zeros across a reset, unless a NaN is in the sum
+          const uint32_t behind = ~0u << lane, upto = ~(behind << 1), x = reset.x & upto, y = reset.y & ~behind;
+          const uint32_t y1 = reset.y & upto;
+          // tokens 2 lane and 2 lane + 1: the last reset at or before them (an empty mask gives -2 or -1)
+          D.from[2 * lane] = uint8_t(max(0, max(62 - 2 * __clz(x), 63 - 2 * __clz(y))));
+          D.from[2 * lane + 1] = uint8_t(max(0, max(62 - 2 * __clz(x), 63 - 2 * __clz(y1))));
+          if (x | y) eg.x = 0.f * e0;
+          if (x | y1) eg.y = 0.f * e1;
+          if ((reset.x & (behind << 1)) | (reset.y & behind)) w.x = 0.f * (after + g1);
+          if ((reset.x | reset.y) & (behind << 1)) w.y = 0.f * after;
+        }
         *reinterpret_cast<float2*>(&D.g2[2 * lane]) = make_float2(e0, e1);
-        *reinterpret_cast<float2*>(&D.eg[2 * lane]) = make_float2(fast_exp2(e0) * a.scale, fast_exp2(e1) * a.scale);
-        *reinterpret_cast<float2*>(&D.w[2 * lane]) = make_float2(fast_exp2((after + g1) * LOG2E), fast_exp2(after * LOG2E));
+        *reinterpret_cast<float2*>(&D.eg[2 * lane]) = eg;
+        *reinterpret_cast<float2*>(&D.w[2 * lane]) = w;
         if (lane == 31) {
           const bool near = fabsf(up) < 0.69314718f;  // past it, growth included, a itself
-          D.a = near ? expm1_near(up) : expf(up), D.one = near ? 1.f : 0.f;
+          D.a = cut ? 0.f * up : near ? expm1_near(up) : expf(up), D.one = near && !cut ? 1.f : 0.f;
+          D.resets = cut;
         }
         arrive(&B.dec_full[slot<RING>(i)]);
         return true;

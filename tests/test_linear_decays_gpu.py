@@ -5,7 +5,8 @@ Tolerances (u: the type's unit roundoff, e = 2^-23; OA, A: outputs and state of 
   outputs  u |o| for their own rounding; what enters the products does so to u^2 (two terms of the type), the exponents
            and sums to (D + 200 + G) e, G the largest sum of |decay| over two chunks (128 tokens)
   state    (D + 200 + G) e A + 3 u^3 A
-Both plus what float32 does not hold: 1e-30 (products of exponentials below 2^-126 are zero)."""
+Both plus what float32 does not hold: 1e-30 (products of exponentials below 2^-126 are zero), and outputs half of their
+type's least value (2^-25 in float16)."""
 
 import pytest
 import torch
@@ -16,6 +17,7 @@ pytestmark = pytest.mark.gpu
 
 BF, HF = torch.bfloat16, torch.float16
 U = {BF: 2.0 ** -8, HF: 2.0 ** -11}
+LEAST = {BF: 2.0 ** -134, HF: 2.0 ** -25}
 E = 2.0 ** -23
 INF, NAN = float("inf"), float("nan")
 
@@ -45,10 +47,12 @@ def check(q, k, v, g, S, scale=None):
     u, d = U[q.dtype], q.shape[-1]
     G = 128 * g.nan_to_num(0.0, posinf=0.0, neginf=0.0).clamp(min=-104.0).abs().amax().item()
     e = (d + 200 + G) * E
-    for got, want, tol in ((out, O, u * O.abs() + (u * u + e) * OA + 1e-30), (state, F, (e + 3 * u ** 3) * A + 1e-30)):
+    past = O.abs() > torch.finfo(q.dtype).max  # outputs past the type's range are its infinities
+    assert torch.equal(out.isinf(), past) and torch.equal(out[past] > 0, O[past] > 0)
+    out_tol = u * O.abs() + (u * u + e) * OA + 1e-30 + LEAST[q.dtype]
+    for got, want, tol, skip in ((out, O, out_tol, past), (state, F, (e + 3 * u ** 3) * A + 1e-30, False)):
         assert torch.equal(got.isnan(), want.isnan())
-        err = torch.where(want.isnan(), 0.0, (got.double() - want).abs())
-        ratio = torch.where(want.isnan(), 0.0, err / tol)
+        ratio = torch.where(want.isnan() | skip, 0.0, (got.double() - want).abs() / tol)
         assert (ratio <= 1).all(), ratio.max().item()
     _lib.check_device_errors()
     return out, state
@@ -63,7 +67,8 @@ def make(n, t, hk, hv, dk, dv, dtype, seed=0, stated=True):
     return q, k, v, r, S
 
 
-SHAPES = [(1, 40, 1, 2, 64, 64, BF), (1, 200, 1, 2, 128, 128, BF), (2, 1100, 1, 1, 128, 64, BF), (1, 150, 2, 2, 64, 48, HF)]
+SHAPES = [(1, 40, 1, 2, 64, 64, BF), (1, 200, 1, 2, 128, 128, BF), (2, 1100, 1, 1, 128, 64, BF),
+          (1, 150, 2, 2, 64, 48, HF)]
 
 
 @pytest.mark.parametrize("rate", [0.01, 0.05])
@@ -83,3 +88,66 @@ def test_growth_of_tenths_a_token(cuda):
     """A chunk's sum of 6.4 and a prompt's of 30: e^30."""
     q, k, v, r, S = make(1, 300, 1, 1, 128, 128, BF)
     check(q, k, v, torch.full_like(r, 0.1), S)
+
+
+LONG = [(1, 64, 1, 2, 64, 64, BF), *SHAPES[1:]]
+LOWEST = torch.finfo(torch.float32).min
+
+
+@pytest.mark.parametrize("value", [-INF, LOWEST, -105.0])
+@pytest.mark.parametrize("where", ["chunk's ends", "often", "every token", "the first", "the last"])
+@pytest.mark.parametrize("n, t, hk, hv, dk, dv, dtype", LONG)
+def test_resets_forget(cuda, n, t, hk, hv, dk, dv, dtype, where, value):
+    """A decay of -inf, or one whose exponential is zero in float32: nothing of an earlier token or of a state twelve
+    orders larger is left."""
+    q, k, v, r, S = make(n, t, hk, hv, dk, dv, dtype)
+    at = torch.arange(t, device="cuda")
+    hit = {"chunk's ends": (at % 64 == 63) | (at % 128 == 0), "often": r > 0.95, "every token": r >= 0,
+           "the first": at == 0, "the last": at == t - 1}[where]
+    hit = hit if hit.dim() == 3 else hit[:, None].expand_as(r)
+    check(q, k, v, torch.where(hit, value, -0.02 * r), S * 1e12)
+
+
+@pytest.mark.parametrize("n, t, hk, hv, dk, dv, dtype", LONG)
+@pytest.mark.parametrize("last", [0, 5, 63, 64, 149])
+def test_nothing_is_left_where_nothing_is_added(cuda, n, t, hk, hv, dk, dv, dtype, last):
+    """Behind the last reset the keys are zero: so are the outputs and the state, exactly."""
+    last = min(last, t - 1)
+    q, k, v, r, S = make(n, t, hk, hv, dk, dv, dtype)
+    k[:, last:] = 0
+    g = -0.1 * r
+    g[:, last] = -INF
+    out, state = check(q, k, v, g, S)
+    assert (out[:, last:] == 0).all() and (state == 0).all()
+
+
+@pytest.mark.parametrize("n, t, hk, hv, dk, dv, dtype", LONG)
+def test_strong_decays_are_their_exponentials(cuda, n, t, hk, hv, dk, dv, dtype):
+    """e^-31 to e^-80, with nothing added behind them that would cover what they leave."""
+    q, k, v, r, S = make(n, t, hk, hv, dk, dv, dtype)
+    k[:, 20:] = 0
+    g = -0.001 * r
+    g[:, 30] = -31.0 - 49.0 * r[:, 30]
+    check(q, k, v, g, S)
+    q, k, v, r, S = make(n, t, hk, hv, dk, dv, dtype, seed=1)
+    check(q, k, v, torch.where(r > 0.9, -100.0 * r, -0.01 * r), S)
+
+
+@pytest.mark.parametrize("at", [0, 1, 40, 63, 64, 100, 149])
+@pytest.mark.parametrize("resets", ["none", "before", "after", "around"])
+@pytest.mark.parametrize("stated", [False, True])
+@pytest.mark.parametrize("n, t, hk, hv, dk, dv, dtype", LONG)
+def test_a_broken_gate_shows(cuda, n, t, hk, hv, dk, dv, dtype, at, resets, stated):
+    """A NaN decay of one head: NaN in every output of the head from its token on and in the state, though resets follow
+    (0 times NaN); the tokens before it and the other heads are as they were."""
+    at = min(at, t - 1)
+    q, k, v, r, S = make(n, t, hk, hv, dk, dv, dtype, stated=stated)
+    g = -0.05 * r
+    if resets in ("before", "around"):
+        g[:, max(0, at - 3)] = -INF
+    if resets in ("after", "around"):
+        g[:, min(t - 1, at + 2)] = -INF
+    g[0, at, hv - 1] = NAN
+    out, state = check(q, k, v, g, S)
+    assert out[0, at:, hv - 1].isnan().all() and state[0, hv - 1].isnan().all()
+    assert not out[0, :at].isnan().any() and not out[0, :, : hv - 1].isnan().any()
