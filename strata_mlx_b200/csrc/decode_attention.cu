@@ -18,7 +18,10 @@
 // The softmax is online: scores are taken relative to a running maximum a head, moved only when a score passes it by
 // 2^8 (a vote a tile instead of a reduction; float32 holds the larger probabilities as exactly). A probability enters
 // the value product as two terms of the activations' type (its rounding and the rest), so that only the output is
-// rounded to 16 bits. The next tile's keys load while this tile's softmax and value product run, its values after.
+// rounded to 16 bits: to 2^-16 of itself in bfloat16, whose exponents reach down to float32's. Float16's end at 2^-24, so
+// there the maximum moves with every larger score and stands at 2^15: a probability is within 2^-22 of itself, and where
+// its terms run out of bits within 2^-40 of the largest (with the peak at 1 a tail of slots below 2^-25 behind it was
+// missing from the output). The next tile's keys load while this tile's softmax and value product run, its values after.
 // Measured: 8 sequences of 131072 tokens, 16 / 2 heads of 256, 326 to 330 us (6.5 TB/s, what a copy reaches); one of 8192
 // 13 us, of which the bytes are 2.6: the launch, one or two tiles a warp, the join. 32 ragged sequences to 9001, 32 / 8
 // heads of 128: 116 us (5.5 TB/s), with the weights gathered 131 (the scores' write and the join's read of them).
@@ -39,7 +42,9 @@ constexpr int HEADS = 8;       // query heads of a block: the products' N
 constexpr int warps_of(int dp) { return dp == 256 ? 8 : 4; }
 constexpr int blocks_per_sm(int dp) { return dp == 256 ? 1 : 3; }
 constexpr int SMS = 148;
-constexpr float SLACK = 8.f;   // log2 by which a score may pass the running maximum
+// log2 by which a score may pass the running maximum, and of what a probability at the maximum is taken as
+template <typename T> constexpr float SLACK = std::is_same_v<T, __half> ? 0.f : 8.f;
+template <typename T> constexpr float TOP = std::is_same_v<T, __half> ? 15.f : 0.f;
 constexpr int JOIN_THREADS = 256;
 
 struct Args {
@@ -320,7 +325,7 @@ __global__ void __launch_bounds__(warps_of(DP) * 32, blocks_per_sm(DP)) attend_k
             }
           }
       }
-      if (__any_sync(0xffffffffu, x0 > m0 + SLACK || x1 > m1 + SLACK)) {
+      if (__any_sync(0xffffffffu, x0 > m0 + SLACK<T> || x1 > m1 + SLACK<T>)) {
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) {
           x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, w));
@@ -329,6 +334,7 @@ __global__ void __launch_bounds__(warps_of(DP) * 32, blocks_per_sm(DP)) attend_k
         x0 = fmaxf(x0, m0), x1 = fmaxf(x1, m1);
         b0 = finite_or_0(x0), b1 = finite_or_0(x1);
         const float c0 = ex2(m0 - b0), c1 = ex2(m1 - b1);
+        b0 -= TOP<T>, b1 -= TOP<T>;
         m0 = x0, m1 = x1;
         l0 *= c0, l1 *= c1;
 #pragma unroll
@@ -366,18 +372,20 @@ __global__ void __launch_bounds__(warps_of(DP) * 32, blocks_per_sm(DP)) attend_k
       load_v(base + UNIT, next);
       load_ids(base + 2 * UNIT, next);
     }
-    // ---- the warps' results joined
+    // ---- the warps' results joined, from here on with a probability at the maximum as 1
 #pragma unroll
     for (int w = 4; w < 32; w <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, w);
       l1 += __shfl_xor_sync(0xffffffffu, l1, w);
     }
+    constexpr float DOWN = 1.f / float(1 << int(TOP<T>));
+    l0 *= DOWN, l1 *= DOWN;
     if (g == 0) s_m[warp][2 * t] = m0, s_m[warp][2 * t + 1] = m1, s_l[warp][2 * t] = l0, s_l[warp][2 * t + 1] = l1;
     __syncthreads();
     float M0 = -INFINITY, M1 = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) M0 = fmaxf(M0, s_m[w][2 * t]), M1 = fmaxf(M1, s_m[w][2 * t + 1]);
-    const float c0 = ex2(m0 - finite_or_0(M0)), c1 = ex2(m1 - finite_or_0(M1));
+    const float c0 = DOWN * ex2(m0 - finite_or_0(M0)), c1 = DOWN * ex2(m1 - finite_or_0(M1));
 #pragma unroll
     for (int i = 0; i < VC; ++i) {
       float4* to = reinterpret_cast<float4*>(&s_o[warp][2 * t][64 * i + 8 * g]);
