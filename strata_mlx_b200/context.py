@@ -94,13 +94,13 @@ class KVPages:
 
     def _workspace(self, what: str, size: int, s: int) -> tuple:
         """The workspace of a kind of call on stream s: its address and bytes (fresh in a capture, whose memory is
-        the graph's). Zeroed: kernels count in it, and leave the counts at zero."""
+        the graph's). It may hold anything: the kernels read what they wrote in the same call."""
         if size == 0:
             raise ValueError(f"{what}: this cache or these arguments are not taken (head_dim a multiple of 8 up to 256, "
                              "a power-of-two page, 16-byte rows, query heads a multiple of the cache's)")
         ws = self._ws.get((what, s))
         if ws is None or ws[1] < size or _capturing():
-            t = torch.zeros(size, dtype=torch.uint8, device=self.device)
+            t = torch.empty(size, dtype=torch.uint8, device=self.device)
             ws = (t.data_ptr(), size, t)
             if not _capturing():
                 self._ws[what, s] = ws
