@@ -322,7 +322,7 @@ typedef struct sc_kv_pages {
  * the same bits on every run. head_dim a multiple of 8, at most 256; q_heads a multiple of kv_heads. Slots past a
  * length are never read. A page id outside the pool or a length outside the table records SC_ERR_PAGE in err; such
  * slots are left out. workspace: sc_decode_attention_workspace bytes, 16-byte aligned, not shared by calls that may
- * overlap. */
+ * overlap or whose launches (two a call) may come between each other's on one stream. */
 SC_API int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t q_row, int64_t q_head, int q_heads,
                                float scale, void* out, void* workspace, size_t workspace_bytes, int* err, void* stream);
 SC_API size_t sc_decode_attention_workspace(const sc_kv_pages* kv, int q_heads);

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+import threading
 
 import torch
 
@@ -53,8 +54,8 @@ class KVPages:
     (batch,) int32, the slots in use. weight (batch, >= max_pages * page) float32 gathers each slot's attention
     weight; position, the same shape int32, holds the position of each slot's token (evict needs both). The tensors
     stay the caller's: the object keeps references and reads lengths and table on the device at every call, so that
-    steps replay from a CUDA graph. Calls on one stream may follow each other freely; each stream has a workspace of
-    its own."""
+    steps replay from a CUDA graph. Calls on one stream may follow each other freely, from several threads too (a
+    lock keeps a call's launches together); each stream has a workspace of its own."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
                  weight: torch.Tensor | None = None, position: torch.Tensor | None = None):
@@ -87,6 +88,7 @@ class KVPages:
         P.pool_pages, P.max_pages, P.dtype = k.shape[0], self.max_pages, _TYPES[k.dtype]
         self._pages, self._ref = P, ctypes.addressof(P)
         self._lib, self._err = _lib.lib(), ptr(_lib.error_word(self.device))
+        self._lock = threading.Lock()  # held over a call's launches: they share a workspace
         self._ws: dict = {}
         self._sizes: dict = {}  # of attend's workspace, by the query heads
         self._evict_sizes: dict = {}  # of evict's, by the budget
@@ -128,10 +130,11 @@ class KVPages:
         size = self._sizes.get(heads)
         if size is None:
             size = self._sizes[heads] = self._lib.sc_decode_attention_workspace(self._ref, heads)
-        ws = self._workspace("attend", size, s)
-        rc = self._lib.sc_decode_attention(self._ref, q.data_ptr(), st[0], st[1], heads,
-                                           self._scale if scale is None else scale, out.data_ptr(), ws[0], ws[1],
-                                           self._err, s)
+        with self._lock:
+            ws = self._workspace("attend", size, s)
+            rc = self._lib.sc_decode_attention(self._ref, q.data_ptr(), st[0], st[1], heads,
+                                               self._scale if scale is None else scale, out.data_ptr(), ws[0], ws[1],
+                                               self._err, s)
         if rc:
             check(rc, "decode_attention")
         return out
@@ -165,9 +168,11 @@ class KVPages:
         size = self._evict_sizes.get(keep)
         if size is None:
             size = self._evict_sizes[keep] = self._lib.sc_evict_workspace(self._ref, keep)
-        ws = self._workspace("evict", size, s)
-        rc = self._lib.sc_evict(self._ref, seen.data_ptr(), keep, sinks, recent, weight.data_ptr(), weight.stride(0),
-                                position.data_ptr(), position.stride(0), lengths.data_ptr(), ws[0], ws[1], self._err, s)
+        with self._lock:
+            ws = self._workspace("evict", size, s)
+            rc = self._lib.sc_evict(self._ref, seen.data_ptr(), keep, sinks, recent, weight.data_ptr(),
+                                    weight.stride(0), position.data_ptr(), position.stride(0), lengths.data_ptr(),
+                                    ws[0], ws[1], self._err, s)
         if rc:
             check(rc, "evict")
 

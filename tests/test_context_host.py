@@ -1,0 +1,87 @@
+"""KVPages without a GPU, against a library that only records: what its calls do on the host."""
+
+import threading
+import time
+
+import pytest
+import torch
+
+from strata_mlx_b200 import context
+
+
+class Recorder:
+    """Stands for the library: notes the arguments, and whether a call came while another was under way."""
+
+    def __init__(self):
+        self.busy, self.overlaps, self.calls = 0, 0, []
+
+    def _call(self, name, args):
+        self.busy += 1
+        self.overlaps += self.busy > 1
+        time.sleep(0.002)
+        self.calls.append((name, args))
+        self.busy -= 1
+        return 0
+
+    def sc_decode_attention(self, *args):
+        return self._call("attend", args)
+
+    def sc_evict(self, *args):
+        return self._call("evict", args)
+
+    def sc_error_string(self, code):
+        return b"refused"
+
+    def sc_decode_attention_workspace(self, *args):
+        return 64
+
+    def sc_evict_workspace(self, *args):
+        return 64
+
+
+@pytest.fixture
+def cache(monkeypatch):
+    """A cache on the CPU whose calls reach the recorder."""
+    monkeypatch.setattr(context, "_here", lambda *ts: torch.device("cpu"))
+    monkeypatch.setattr(context, "_stream", lambda index: 0)
+    monkeypatch.setattr(context, "_capturing", lambda: False)
+    monkeypatch.setattr(context._lib, "error_word", lambda device=None: torch.zeros(4, dtype=torch.int32))
+    lib = Recorder()
+    monkeypatch.setattr(context._lib, "lib", lambda: lib)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    k = torch.zeros((4, 16, 1, 64), dtype=torch.bfloat16)
+    table = torch.arange(4, dtype=torch.int32).reshape(2, 2)
+    lengths = torch.tensor([20, 9], dtype=torch.int32)
+    c = context.KVPages(k, k.clone(), table, lengths, torch.zeros((2, 32)), torch.zeros((2, 32), dtype=torch.int32))
+    c._index = -1  # the index of a tensor on the CPU
+    return c, lib
+
+
+def test_two_threads_calls_follow_each_other(cache):
+    """A call is two launches over one workspace: another's launch must not come between them."""
+    c, lib = cache
+    q = torch.zeros((2, 4, 64), dtype=torch.bfloat16)
+    seen = c.lengths.clone()
+
+    def work():
+        for _ in range(5):
+            c.attend(q)
+            c.evict(seen, 12, sinks=0)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(lib.calls) == 40 and lib.overlaps == 0
+
+
+def test_a_call_that_fails_does_not_hold_the_others_up(cache):
+    c, lib = cache
+    lib.sc_decode_attention = lambda *args: -2
+    q = torch.zeros((2, 4, 64), dtype=torch.bfloat16)
+    for _ in range(2):
+        with pytest.raises(ValueError):
+            c.attend(q)
+    c.evict(c.lengths.clone(), 12, sinks=0)
+    assert [name for name, _ in lib.calls] == ["evict"]
