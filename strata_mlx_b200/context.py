@@ -148,8 +148,8 @@ class KVPages:
         theirs until all are done). Slots past the new length keep what they held."""
         if self.weight is None or self.position is None:
             raise ValueError("evict needs the cache's weight and position")
-        if keep < 0 or sinks < 0 or recent < 0 or sinks + recent > keep:
-            raise ValueError(f"sinks {sinks} and recent {recent} have to fit in keep {keep}")
+        if not 0 <= keep < 1 << 31 or sinks < 0 or recent < 0 or sinks + recent > keep:
+            raise ValueError(f"sinks {sinks} and recent {recent} have to fit in keep {keep}, and keep in 31 bits")
         weight, position, lengths = (self.weight, self.position, self.lengths) if out is None else out
         index, n, room = self._index, self.batch, min(keep, self.slots)
         if seen.get_device() != index or torch.cuda.current_device() != index:

@@ -85,3 +85,14 @@ def test_a_call_that_fails_does_not_hold_the_others_up(cache):
             c.attend(q)
     c.evict(c.lengths.clone(), 12, sinks=0)
     assert [name for name, _ in lib.calls] == ["evict"]
+
+
+@pytest.mark.parametrize("keep", [1 << 31, 1 << 32, (1 << 32) + 5, 1 << 40])
+def test_a_budget_past_32_bits_is_refused(cache, keep):
+    """It would reach the library as its low 32 bits: 2^32 as a budget of nothing."""
+    c, lib = cache
+    with pytest.raises(ValueError, match="keep"):
+        c.evict(c.lengths.clone(), keep, sinks=0)
+    assert not lib.calls
+    c.evict(c.lengths.clone(), (1 << 31) - 1, sinks=0)
+    assert lib.calls[0][1][2] == (1 << 31) - 1
