@@ -121,6 +121,7 @@ class HybridDecoder:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)  # slots in use
         self.seen = torch.zeros(batch, dtype=torch.int32, device=device)     # positions so far
         self.most = 0  # no sequence holds more slots
+        self.reached, self.max_pos = 0, max_pos  # no sequence has had more positions; those that rope has angles for
         self.rope = Rope(max_pos, device)
         self.embed = torch.randn((vocab, hidden), generator=g, device=device).to(torch.bfloat16)
         self.head = torch.randn((vocab, hidden), generator=g, device=device) * hidden ** -0.5
@@ -158,6 +159,8 @@ class HybridDecoder:
         n, t = tokens.shape
         if n != self.batch or t > self.capacity:
             raise ValueError(f"prompts ({self.batch}, at most {self.capacity}) expected, got {tuple(tokens.shape)}")
+        if t > self.max_pos:
+            raise ValueError(f"prompts of {t} tokens, but max_pos is {self.max_pos}")
         x = self.embed[tokens]
         for mixer, moe in self.layers:
             x = x + mixer.prompt(rmsnorm(x, self.norm), lengths)
@@ -165,11 +168,15 @@ class HybridDecoder:
                 x = x + moe[0](rmsnorm(x, self.norm).flatten(0, 1)).unflatten(0, (n, t))
         self.lengths.copy_(lengths)
         self.seen.copy_(lengths)
-        self.most = t
+        self.most = self.reached = t
         return self._logits(x[torch.arange(n, device=x.device), lengths.long() - 1])
 
     def step(self, tokens: torch.Tensor) -> torch.Tensor:
-        """One more token a sequence (batch,). A full cache is cut to its budget first."""
+        """One more token a sequence (batch,), up to max_pos positions, the prompt's width among them. A full cache is cut
+        to its budget first."""
+        if self.reached == self.max_pos:
+            raise ValueError(f"all {self.max_pos} positions (max_pos) are taken")
+        self.reached += 1
         if self.most == self.capacity:
             self.evict()
         self.most += 1
