@@ -155,12 +155,14 @@ class HybridDecoder:
         return rmsnorm(x, self.norm).float() @ self.head.T
 
     def prompt(self, tokens: torch.Tensor, lengths: torch.Tensor) -> torch.Tensor:
-        """Prompts (batch, t), sequence b's the first lengths[b] >= 1 tokens: the logits behind each one's last token."""
+        """Prompts (batch, t), sequence b's the first lengths[b] >= 1 tokens: the logits behind each one's last token. Lengths
+        stay on the device; one past t counts as t, one below 0 as 0."""
         n, t = tokens.shape
         if n != self.batch or t > self.capacity:
             raise ValueError(f"prompts ({self.batch}, at most {self.capacity}) expected, got {tuple(tokens.shape)}")
         if t > self.max_pos:
             raise ValueError(f"prompts of {t} tokens, but max_pos is {self.max_pos}")
+        lengths = lengths.clamp(0, t)
         x = self.embed[tokens]
         for mixer, moe in self.layers:
             x = x + mixer.prompt(rmsnorm(x, self.norm), lengths)
@@ -169,7 +171,7 @@ class HybridDecoder:
         self.lengths.copy_(lengths)
         self.seen.copy_(lengths)
         self.most = self.reached = t
-        return self._logits(x[torch.arange(n, device=x.device), lengths.long() - 1])
+        return self._logits(x[torch.arange(n, device=x.device), (lengths.long() - 1).clamp(min=0)])
 
     def step(self, tokens: torch.Tensor) -> torch.Tensor:
         """One more token a sequence (batch,), up to max_pos positions, the prompt's width among them. A full cache is cut

@@ -27,3 +27,14 @@ def test_positions_past_the_rotary_table_are_refused():
     assert dec.seen.tolist() == [40, 7] and dec.lengths.tolist() == [40, 7]
     dec.prompt(torch.zeros((2, 5), dtype=torch.int64), torch.tensor([5, 5], dtype=torch.int32))  # a new prompt starts over
     dec.step(torch.zeros(2, dtype=torch.int64))
+
+
+def test_lengths_past_the_prompts_are_held_to_them():
+    """A length outside the prompt's width would index past the tokens here, and past the cache at the next step."""
+    dec = make()
+    dec.layers = []
+    tokens = torch.arange(16).reshape(2, 8)
+    logits = dec.prompt(tokens, torch.tensor([99, 8], dtype=torch.int32))
+    assert torch.equal(logits, dec.prompt(tokens, torch.tensor([8, 8], dtype=torch.int32)))
+    dec.prompt(tokens, torch.tensor([99, -4], dtype=torch.int32))
+    assert dec.lengths.tolist() == [8, 0] and dec.seen.tolist() == [8, 0]
