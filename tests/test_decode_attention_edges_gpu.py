@@ -104,3 +104,50 @@ def test_long_tails_under_sinks(cuda, dtype, n, d, tail, value):
         ratio = (out[b].double() - o).abs() / tol
         assert (ratio <= 1).all(), (b, ratio.max().item())
     assert got.shape == (4, 2, d)
+
+
+def ragged(n, most, seed):
+    """Lengths of n sequences, empty ones among them and around the ends of runs of 128 and 256."""
+    g = torch.Generator().manual_seed(seed)
+    got = torch.randint(1, most + 1, (n,), generator=g)
+    got[torch.randperm(n, generator=g)[: n // 4]] = 0
+    for at in (0, 126, 127, 128, 129, 254, 255, 256, 257, n - 1):
+        if at < n:
+            got[at] = 0 if at % 3 else most
+    return got.tolist()
+
+
+@pytest.mark.parametrize("tracked", [False, True])
+@pytest.mark.parametrize("d, hq, hkv, dtype", [(64, 6, 2, HF), (128, 4, 4, BF), (256, 8, 1, BF)])
+@pytest.mark.parametrize("n", [127, 128, 129, 256, 257, 300, 600])
+def test_more_sequences_than_a_block_has_threads(cuda, n, d, hq, hkv, dtype, tracked):
+    lengths = ragged(n, 200, n + d)
+    k, v, table, t = pool(lengths, hkv, d, 16, dtype)
+    q = torch.randn((n, hq, d), device="cuda").to(dtype)
+    weight = torch.rand((n, table.shape[1] * 16), device="cuda") if tracked else None
+    check(q, k, v, table, t, weight)
+
+
+@pytest.mark.parametrize("tracked", [False, True])
+@pytest.mark.parametrize("lengths", [[0] * 300, [0] * 299 + [1], [1] + [0] * 299, [0] * 150 + [700] + [0] * 149])
+def test_hardly_a_sequence_with_tokens(cuda, lengths, tracked):
+    k, v, table, t = pool(lengths, 2, 64, 16, BF)
+    q = torch.randn((300, 4, 64), device="cuda").to(BF)
+    check(q, k, v, table, t, torch.rand((300, table.shape[1] * 16), device="cuda") if tracked else None)
+
+
+def test_thousands_of_sequences(cuda):
+    """Some of them against the definition; the whole twice, with the same bits."""
+    n, d = 20000, 64
+    lengths = torch.randint(0, 90, (n,), generator=torch.Generator().manual_seed(3), dtype=torch.int32).cuda()
+    k, v = (torch.randn((500, 16, 2, d), device="cuda").to(BF) for _ in range(2))
+    table = torch.randint(0, 500, (n, 6), device="cuda", dtype=torch.int32)
+    q = torch.randn((n, 4, d), device="cuda").to(BF)
+    weight = torch.zeros((n, 96), device="cuda")
+    out = context.decode_attention(q, k, v, table, lengths, weight=weight)
+    some = torch.cat([torch.arange(0, n, 499), torch.tensor([n - 1])]).cuda()
+    alone = torch.zeros((len(some), 96), device="cuda")
+    want = check(q[some], k, v, table[some].contiguous(), lengths[some], alone)
+    assert torch.equal(out[some], want)  # such short sequences lie in one unit each: the same sums
+    assert torch.equal(weight[some], alone)
+    assert torch.equal(out, context.decode_attention(q, k, v, table, lengths))
