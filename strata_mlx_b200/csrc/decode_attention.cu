@@ -7,6 +7,10 @@
 //                  a long cache spreads over all SMs. A block joins its warps' results in shared memory; a run that
 //                  covers a head's whole length writes the output, the others partial results (at most two a block).
 //   join_kernel    joins the partial results in block order (the same bits on every run), and adds the weights.
+//   starts_kernel  first, for more than two sequences for each thread of an attending block: how many units lie before
+//                  each. (Up to as many, every block counts them itself: 129 of up to 512 tokens 28 us, with this kernel
+//                  32. Past it that took passes in every block of both kernels: 4096 rows of up to 512 tokens, 16 / 2
+//                  heads of 256, 1080 us, with this kernel 783; 65535 of up to 64, heads of 64, 134 ms and 3.8.)
 //
 // A warp's tile goes from memory straight into tensor-core fragments (mma.sync m16n8k16; up to eight query heads share
 // the key/value head, so a product of 16 slots by 8 heads has little padding, and 128-row tcgen05 products would
@@ -62,6 +66,7 @@ struct Args {
   float* part_o;      // (head_tiles, columns, 2, 8, DP) unnormalized outputs of runs that cover part of a head
   float2* part_ml;    // (head_tiles, columns, 2, 8) their maxima and sums
   float2* whole_ml;   // (batch, q_heads) those of heads that one block covered
+  int32_t* starts;    // (batch + 1) units before each sequence, a head's, and in all; NULL where the blocks count
   int* err;
 };
 
@@ -148,21 +153,18 @@ __global__ void __launch_bounds__(warps_of(DP) * 32, blocks_per_sm(DP)) attend_k
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int ht = blockIdx.y;
   const uint32_t x = blockIdx.x;
+  if (A.starts) pdl_wait();
   pdl_launch_dependents();
-  // the units in all, and the sequence that holds this block's first one (a single pass up to THREADS sequences)
-  int U, to;
-  const int first = tid < A.batch ? (length_of(A.pages, tid, A.err) + UNIT - 1) / UNIT : 0;
-  if (A.batch == 1) {
-    U = to = (length_of(A.pages, 0, nullptr) + UNIT - 1) / UNIT;
-  } else {
-    to = block_scan<THREADS>(first, s_sum, U);
-    if (A.batch > THREADS) {
-      int n = first;
-#pragma unroll 1
-      for (int i = tid + THREADS; i < A.batch; i += THREADS) n += (length_of(A.pages, i, A.err) + UNIT - 1) / UNIT;
-      U = block_sum<THREADS>(n, s_sum);
-    }
+  // the units in all, and the sequence that holds this block's first one
+  int U, to = 0;
+  int n0 = 0, n1 = 0;  // of two sequences a thread
+  if (!A.starts && 2 * tid < A.batch) {
+    n0 = (length_of(A.pages, 2 * tid, A.err) + UNIT - 1) / UNIT;
+    if (2 * tid + 1 < A.batch) n1 = (length_of(A.pages, 2 * tid + 1, A.err) + UNIT - 1) / UNIT;
   }
+  if (A.starts) U = A.starts[A.batch];
+  else if (A.batch == 1) U = (length_of(A.pages, 0, nullptr) + UNIT - 1) / UNIT;
+  else to = block_scan<THREADS>(n0 + n1, s_sum, U);
   U *= A.kv_heads;
   const uint32_t X = min(A.columns, U);
   if (x >= X) return;
@@ -170,28 +172,31 @@ __global__ void __launch_bounds__(warps_of(DP) * 32, blocks_per_sm(DP)) attend_k
   int u = split.start(x);
   const int u1 = split.start(x + 1);
   int b = 0, before = 0;
-  if (A.batch > 1) {
+  if (A.starts) {  // the last sequence that begins at or before it: 32 places at a time, every warp for itself
+    const int w = u / A.kv_heads;
+#pragma unroll 1
+    for (int end = A.batch; end - b > 1;) {
+      const int step = (end - b + 31) / 32, at = b + lane * step;
+      const int n = __popc(__ballot_sync(0xffffffffu, at < end && A.starts[at] <= w));
+      b += max(n - 1, 0) * step;
+      end = min(end, b + step);
+    }
+    before = A.starts[b];
+  } else if (A.batch > 1) {
     if (tid == 0) s_b = -1;
     __syncthreads();
-    int mine = first;
-    for (int b0 = 0;;) {
-      if (u >= (to - mine) * A.kv_heads && u < to * A.kv_heads) s_b = b0 + tid, s_before = to - mine;
-      __syncthreads();
-      b0 += THREADS;
-      if (s_b >= 0 || b0 >= A.batch) break;
-      int total;
-      if (tid == THREADS - 1) s_before = to;  // where the next sequences begin
-      __syncthreads();
-      const int from = s_before;
-      mine = b0 + tid < A.batch ? (length_of(A.pages, b0 + tid, nullptr) + UNIT - 1) / UNIT : 0;
-      to = from + block_scan<THREADS>(mine, s_sum, total);
+    if (u >= (to - n1 - n0) * A.kv_heads && u < to * A.kv_heads) {
+      const bool second = u >= (to - n1) * A.kv_heads;
+      s_b = 2 * tid + second, s_before = to - n1 - (second ? 0 : n0);
     }
+    __syncthreads();
     b = s_b, before = s_before;
     if (b < 0) return;  // the lengths changed under the kernel
   }
   int hk, ul;
   {
     const int n = (length_of(A.pages, b, nullptr) + UNIT - 1) / UNIT;
+    if (n == 0) return;  // as above
     const uint32_t in = u - before * A.kv_heads;
     hk = in / n, ul = in % n;
   }
@@ -442,7 +447,9 @@ template <int N>
 __device__ __forceinline__ Share share_of(const Args& A, int unit, int b, int* sh) {
   const int n = (length_of(A.pages, b, nullptr) + unit - 1) / unit;
   int U = n, before = 0;
-  if (A.batch > 1) {
+  if (A.starts) {
+    U = A.starts[A.batch], before = A.starts[b];
+  } else if (A.batch > 1) {
     int all = 0;
 #pragma unroll 1
     for (int i = threadIdx.x; i < A.batch; i += N) {
@@ -454,6 +461,24 @@ __device__ __forceinline__ Share share_of(const Args& A, int unit, int b, int* s
   }
   U = max(1, U * A.kv_heads);  // there may be none
   return {Split(U, min(A.columns, U)), before * A.kv_heads, n};
+}
+
+// One block: each thread a run of sequences.
+constexpr int STARTS_THREADS = 1024;
+__global__ void __launch_bounds__(STARTS_THREADS) starts_kernel(const Args A, int unit) {
+  __shared__ int sh[STARTS_THREADS / 32];
+  pdl_launch_dependents();
+  const int per = (A.batch + STARTS_THREADS - 1) / STARTS_THREADS, b0 = threadIdx.x * per, b1 = min(A.batch, b0 + per);
+  int n = 0, total;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) n += (length_of(A.pages, b, A.err) + unit - 1) / unit;
+  int at = block_scan<STARTS_THREADS>(n, sh, total) - n;
+#pragma unroll 8
+  for (int b = b0; b < b1; ++b) {
+    A.starts[b] = at;
+    at += (length_of(A.pages, b, nullptr) + unit - 1) / unit;
+  }
+  if (threadIdx.x == 0) A.starts[A.batch] = total;
 }
 
 // Blocks 0 .. batch x q_heads - 1: a query head's output from its partial results (zeros for an empty sequence). The
@@ -618,7 +643,8 @@ inline int tile_of(int dp) { return dp == 64 ? 32 : 16; }
 
 struct Layout {
   int dp, unit, head_tiles, columns, pack;
-  size_t part_o, part_ml, whole_ml, scores, bytes;
+  size_t part_o, part_ml, whole_ml, scores, starts, bytes;
+  bool counted;  // by starts_kernel
 };
 
 inline Layout layout(const sc_kv_pages& c, int q_heads) {
@@ -638,6 +664,8 @@ inline Layout layout(const sc_kv_pages& c, int q_heads) {
   };
   l.part_o = take(parts * l.dp * 4);
   l.part_ml = take(parts * 8);
+  l.counted = c.batch > 2 * warps_of(l.dp) * 32;
+  if (l.counted) l.starts = take((size_t(c.batch) + 1) * 4);
   if (c.weight) {
     l.whole_ml = take(size_t(c.batch) * q_heads * 8);
     l.scores = take(size_t(c.batch) * c.kv_heads * l.head_tiles * slots * l.pack * 4);
@@ -683,6 +711,7 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
     A.whole_ml = reinterpret_cast<float2*>(ws + l.whole_ml);
     A.scores = reinterpret_cast<float*>(ws + l.scores);
   }
+  if (l.counted) A.starts = reinterpret_cast<int32_t*>(ws + l.starts);
   A.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int slot_blocks = kv->weight ? int(ceil_div(A.slots, da::JOIN_THREADS)) : 0;
@@ -694,17 +723,24 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
     constexpr int warps = da::warps_of(DP), smem = warps * da::HEADS * DP * 4;
     const auto attend = da::attend_kernel<T, DP, SUB>;
     if (int rc = raise_smem(reinterpret_cast<const void*>(attend), smem, "decode attention smem attribute")) return rc;
-    attend<<<dim3(unsigned(l.columns), unsigned(l.head_tiles)), warps * 32, smem, s>>>(A);
-    // programmatic dependent launch: the joining blocks are placed as the attention's leave
+    // programmatic dependent launches: blocks are placed as those of the kernel before leave
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(join_blocks));
-    cfg.blockDim = dim3(da::JOIN_THREADS);
-    cfg.dynamicSmemBytes = kv->weight ? size_t(kv->kv_heads) * l.head_tiles * l.pack * 8 : 0;
-    cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
+    cfg.stream = s;
+    cfg.gridDim = dim3(unsigned(l.columns), unsigned(l.head_tiles));
+    cfg.blockDim = dim3(warps * 32);
+    cfg.dynamicSmemBytes = smem;
+    if (l.counted) {
+      da::starts_kernel<<<1, da::STARTS_THREADS, 0, s>>>(A, l.unit);
+      cfg.numAttrs = 1;
+    }
+    if (cudaError_t e = cudaLaunchKernelEx(&cfg, attend, A)) return cuda_failed(e, "decode attention launch");
+    cfg.gridDim = dim3(unsigned(join_blocks));
+    cfg.blockDim = dim3(da::JOIN_THREADS);
+    cfg.dynamicSmemBytes = kv->weight ? size_t(kv->kv_heads) * l.head_tiles * l.pack * 8 : 0;
     cfg.numAttrs = 1;
     const auto join = l.pack == 1 ? da::join_kernel<T, DP, 1> : l.pack == 2 ? da::join_kernel<T, DP, 2>
                     : l.pack == 4 ? da::join_kernel<T, DP, 4> : da::join_kernel<T, DP, 8>;
