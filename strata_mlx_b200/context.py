@@ -98,8 +98,9 @@ class KVPages:
         """The workspace of a kind of call on stream s: its address and bytes (fresh in a capture, whose memory is
         the graph's). It may hold anything: the kernels read what they wrote in the same call."""
         if size == 0:
-            raise ValueError(f"{what}: this cache or these arguments are not taken (head_dim a multiple of 8 up to 256, "
-                             "a power-of-two page, 16-byte rows, query heads a multiple of the cache's)")
+            raise ValueError(f"{what}: this cache or these arguments are not taken (at most 65535 sequences, head_dim a "
+                             "multiple of 8 up to 256, a power-of-two page up to 4096, 2^30 slots, 16-byte rows, at most "
+                             "2048 query heads, a multiple of the cache's)")
         ws = self._ws.get((what, s))
         if ws is None or ws[1] < size or _capturing():
             t = torch.empty(size, dtype=torch.uint8, device=self.device)

@@ -61,3 +61,11 @@ def test_a_workspace_may_hold_anything(cuda):
     for other in got[1:]:
         assert all(torch.equal(a, b) for a, b in zip(got[0], other))
     _lib.check_device_errors()
+
+
+def test_a_batch_past_the_limit_is_named(cuda):
+    k = torch.zeros((1, 16, 1, 64), dtype=BF, device="cuda")
+    table = torch.zeros((65536, 1), dtype=torch.int32, device="cuda")
+    cache = context.KVPages(k, k.clone(), table, torch.ones(65536, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="65535"):
+        cache.attend(torch.zeros((65536, 1, 64), dtype=BF, device="cuda"))
