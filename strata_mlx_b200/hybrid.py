@@ -7,7 +7,8 @@ it is full.
     python -m strata_mlx_b200.hybrid [--batch 8] [--prompt 512] [--steps 64]
 
     prompt   linear layers by linear_attention (ragged prompts by their lengths); full layers write their keys and
-             values into the cache and take the prompt's tokens as rows of decode_attention over one row of the table
+             values into the cache and take the prompt's tokens, ROWS at a time, as rows of decode_attention over one
+             row of the table
     step     one token a sequence: linear_attention_step, KVPages.attend with weights, the MoE block's decode kernels
     evict    every full layer's KVPages.evict, then one new length for all of them
 
@@ -25,6 +26,8 @@ from ._lib import check_device_errors
 from .context import KVPages, linear_attention, linear_attention_step
 from .decoder import HEAD_DIM, PAGE, Dense, Rope, rmsnorm
 from .synthetic import blocks_cuda
+
+ROWS = 4096  # a prompt's tokens that one attention call takes: its scores are as many rows of the cache's slots
 
 
 class LinearMixer:
@@ -81,12 +84,20 @@ class CacheMixer:
         q = self._qkv(h.flatten(0, 1), at.repeat(n), rows.flatten())
         self.position[:, :t] = at
         # token i sees slots 0 .. i of its sequence's row; tokens past a length see none
-        seen = torch.where(live, at + 1, 0).to(torch.int32).flatten()
-        weight = torch.zeros((n * t, self.own.capacity), device=h.device)
-        table = self.own.table.repeat_interleave(t, 0)
-        out = KVPages(self.k, self.v, table, seen, weight=weight).attend(q)
-        self.weight[:] = weight.unflatten(0, (n, t)).sum(1)
-        return self.wo(out.flatten(-2)).unflatten(0, (n, t))
+        seen = torch.where(live, at + 1, 0).to(torch.int32)
+        q = q.unflatten(0, (n, t))
+        out = torch.empty_like(q)
+        self.weight.zero_()
+        each = max(1, ROWS // n)
+        for i in range(0, t, each):
+            m = min(each, t - i)
+            weight = torch.zeros((n * m, self.own.capacity), device=h.device)
+            table = self.own.table.repeat_interleave(m, 0)
+            part = KVPages(self.k, self.v, table, seen[:, i : i + m].flatten(), weight=weight).attend(
+                q[:, i : i + m].flatten(0, 1))
+            out[:, i : i + m] = part.unflatten(0, (n, m))
+            self.weight += weight.unflatten(0, (n, m)).sum(1)
+        return self.wo(out.flatten(0, 1).flatten(-2)).unflatten(0, (n, t))
 
     def step(self, h: torch.Tensor) -> torch.Tensor:
         own = self.own
