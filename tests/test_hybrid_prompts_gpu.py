@@ -40,3 +40,45 @@ def test_rows_in_pieces_are_rows_at_once(cuda, monkeypatch):
     wa, wb = a.layers[1][0].weight, b.layers[1][0].weight
     assert torch.allclose(wa, wb, rtol=1e-5, atol=1e-6)
     _lib.check_device_errors()
+
+
+def close(a, b):
+    """Head by head, to bfloat16 roundings of inputs, products and outputs: 8 x 2^-8 of a head's 2-norm."""
+    a, b = a.float(), b.float()
+    ratio = (a - b).norm(dim=-1) / (2.0 ** -5 * b.norm(dim=-1) + 1e-6)
+    assert (ratio <= 1).all(), ratio.max().item()
+
+
+def test_a_cache_layer_s_prompt_is_its_steps(cuda):
+    """One full attention layer on the same inputs: every head of every token, the caches and what slots gathered."""
+    t, lengths = 70, torch.tensor([70, 1, 33], dtype=torch.int32, device="cuda")
+    a, b = make(layers=1, every=1), make(layers=1, every=1)
+    h = torch.randn((3, t, 256), device="cuda").to(torch.bfloat16)
+    x, y = a.layers[0][0], b.layers[0][0]
+    x.wo = y.wo = lambda out: out  # the heads as they are
+    whole = x.prompt(h, lengths).unflatten(-1, (4, -1))
+    for i in range(t):
+        b.lengths += 1
+        close(y.step(h[:, i].contiguous()).unflatten(-1, (4, -1))[lengths > i], whole[:, i][lengths > i])
+        b.seen += 1
+    for n, m in enumerate(lengths.tolist()):
+        rows = [d.rows(torch.arange(m, device="cuda").expand(3, m))[n] for d in (a, b)]
+        for p, q in ((x.k, y.k), (x.v, y.v)):
+            close(p.view(-1, 2, 256)[rows[0]], q.view(-1, 2, 256)[rows[1]])
+        assert torch.equal(x.position[n, :m], y.position[n, :m])
+    assert torch.allclose(x.weight[0, :70], y.weight[0, :70], rtol=2.0 ** -5)
+
+
+def test_a_linear_layer_s_prompt_is_its_steps(cuda):
+    t = 70
+    lengths = torch.tensor([70, 1, 33], dtype=torch.int32, device="cuda")
+    a, b = make(layers=1, linear_heads=4), make(layers=1, linear_heads=4)
+    h = torch.randn((3, t, 256), device="cuda").to(torch.bfloat16)
+    x, y = a.layers[0][0], b.layers[0][0]
+    x.wo = y.wo = lambda out: out
+    whole = x.prompt(h, lengths).unflatten(-1, (4, -1))
+    y.state = torch.zeros_like(x.state)
+    for i in range(t):
+        close(y.step(h[:, i].contiguous()).unflatten(-1, (4, -1))[lengths > i], whole[:, i][lengths > i])
+        for n in (lengths == i + 1).nonzero()[:, 0].tolist():
+            close(y.state[n].flatten(1), x.state[n].flatten(1))
