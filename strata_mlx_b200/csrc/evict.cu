@@ -30,6 +30,8 @@ constexpr int FEW = 256;          // keys that are ranked one against another
 constexpr int MAX_CLUSTER = 8;
 constexpr int STRETCH = 128 * WARPS;  // a block's slots are a multiple
 constexpr int MOST = 50 * 1024;   // slots a block can hold the keys of (200 KB); past 8 such blocks keys are made anew
+constexpr int OWN = 7 * 1024;     // bytes of plan_kernel's other shared arrays, at most
+static_assert(OWN + 4 * MOST <= 227 * 1024, "shared memory of a block");
 constexpr int FETCH = 8;          // weights and positions a thread loads at a time
 constexpr int MOVE_WARPS = 8;
 constexpr uint32_t KEPT = 0xffffffffu;
@@ -73,6 +75,8 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const Args A) {
   __shared__ int s_warp[4][WARPS], s_pick[3], s_n;
   __shared__ uint32_t s_few[2][FEW];  // this block's, and the cluster's
   __shared__ int4 s_mine[3], s_all[2];  // what the other blocks read; sums over the cluster
+  static_assert(sizeof(s_hist) + sizeof(s_warp) + sizeof(s_pick) + sizeof(s_n) + sizeof(s_few) + sizeof(s_mine) +
+                    sizeof(s_all) + 64 <= OWN, "and the places' alignment");
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
   const int b = blockIdx.x / blocks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -423,8 +427,8 @@ extern "C" int sc_evict(const sc_kv_pages* kv, const int32_t* seen, int keep, in
   const bool held = hold <= ev::MOST;
   const int smem = held ? int(hold) * 4 : 0;
   const auto plan = held ? ev::plan_kernel<true> : ev::plan_kernel<false>;
-  // beside the kernel's 17 KB of static shared memory, past 31 KB the dynamic part has to be asked for
-  const int asked = smem > 30 * 1024 ? std::max(smem, 48 * 1024 + 16) : 0;
+  // 48 KB with the kernel's own arrays go without asking; raise_smem asks for more than that only
+  const int asked = smem + ev::OWN > 48 * 1024 ? std::max(smem, 48 * 1024 + 16) : 0;
   if (int rc = raise_smem(reinterpret_cast<const void*>(plan), asked, "evict smem attribute")) return rc;
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = {};

@@ -61,3 +61,21 @@ def test_evict_past_shared_memory(cuda, lengths, keep, sinks, recent, page, plac
         for pool, was in ((k, k0), (v, v0)):
             assert torch.equal(pool.view(-1, 8)[at], was.view(-1, 8)[src])
     _lib.check_device_errors()
+
+
+@pytest.mark.parametrize("slots", [9216, 10240, 11264, 12288, 81920, 98304, 409600])
+def test_evict_at_the_limits_of_shared_memory(cuda, slots):
+    """Around the slots a block gets shared memory for without asking, and up to the most that it holds keys of."""
+    g = np.random.default_rng(slots)
+    keep = slots // 3
+    k, v = (torch.randn((slots // 16, 16, 1, 8), device="cuda").to(torch.bfloat16) for _ in range(2))
+    k0 = k.clone()
+    table = torch.arange(slots // 16, dtype=torch.int32, device="cuda")[None]
+    w, pos = g.random((1, slots)).astype(np.float32), np.arange(slots, dtype=np.int32)[None]
+    cw, cp = torch.from_numpy(w.copy()).cuda(), torch.from_numpy(pos.copy()).cuda()
+    length = torch.tensor([slots], dtype=torch.int32, device="cuda")
+    context.KVPages(k, v, table, length, weight=cw, position=cp).evict(length.clone(), keep, sinks=4, recent=keep // 2)
+    take = kept(w[0], pos[0], slots, keep, 4, keep // 2)
+    assert int(length[0]) == keep and np.array_equal(cp[0, :keep].cpu().numpy(), take)
+    assert torch.equal(k.view(-1, 8)[:keep], k0.view(-1, 8)[torch.from_numpy(take).cuda()])
+    _lib.check_device_errors()
