@@ -79,9 +79,10 @@ struct Decays {
 struct Bars {
   uint64_t qk_full[2][KS], qk_empty[2][KS], v_full[VS], v_empty[VS], dec_full[RING], dec_empty[RING];
   uint64_t a_full, a_empty, p_full, p_empty, o_full, o_empty, kw_full[2], kw_empty[2], d_full, d_empty, s_full, s_empty,
-      done;
+      ends, outs, done;
   uint32_t tmem;
   int bail;
+  int odd[4];  // whether a state at the segment's end is not finite, for each quarter of the value dimensions
 };
 
 struct AddBars {
@@ -332,6 +333,59 @@ __device__ __forceinline__ uint2 take_resets(float2& g) {
   return make_uint2(__ballot_sync(0xffffffffu, x), __ballot_sync(0xffffffffu, y));
 }
 
+// A value that is not finite meets P's zeros (0 times it is NaN) and so reaches the tokens before it in its chunk. It stays
+// in the state, whatever follows; so a segment whose state at its end is finite had none, and the chunks need not look. In
+// another the outputs are mended behind its last chunk: the recurrence from the state before the segment up to the last
+// token whose value is the first that is not finite of its dimension, a lane a dimension, the state in two places of shared
+// memory that the products have done with. What is not finite among the outputs and is in the recurrence is replaced.
+template <int DK>
+__device__ __forceinline__ void mend_outputs(const Args& A, uint8_t* place0, uint8_t* place1, int dv, int t0, int t1) {
+  const sc_linear& a = A.a;
+  const int seg = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / (a.v_heads / a.k_heads);
+  const bool live = dv < a.v_dim;
+  const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v) + b * a.v_row + h * a.v_head + (live ? dv : 0);
+  int last = t0;
+  bool seen = !live;
+#pragma unroll 4
+  for (int t = t0; t < t1; ++t)
+    if (!isfinite(__bfloat162float(v[t * a.v_token])) && !seen) seen = true, last = t;
+  last = __reduce_max_sync(0xffffffffu, last);
+  if (last == t0) return;
+  constexpr int FIRST = QS * DK / 64 * HALF / 512;  // rows of 128 values in place0
+  static_assert((DK - FIRST) * 512 <= 2 * HALF, "the state's places");
+  auto S = [&](int k) -> float& { return reinterpret_cast<float*>(k < FIRST ? place0 + 512 * k : place1 + 512 * (k - FIRST))[dv]; };
+  const int64_t head = int64_t(b) * a.v_heads + h;
+  if (A.segments > 1) pdl_wait();
+#pragma unroll 1
+  for (int k = 0; k < a.k_dim; ++k) {
+    float s = 0.f;
+    if (A.segments > 1) s = A.parts[((head * A.segments + seg) * DK + k) * 128 + dv];
+    else if (a.state_in && live) s = a.state_in[(head * a.k_dim + k) * a.v_dim + dv];
+    S(k) = s;
+  }
+#pragma unroll 1
+  for (int t = t0; t < last; ++t) {
+    const __nv_bfloat16* qt = static_cast<const __nv_bfloat16*>(a.q) + b * a.q_row + hk * a.q_head + t * a.q_token;
+    const __nv_bfloat16* kt = static_cast<const __nv_bfloat16*>(a.k) + b * a.k_row + hk * a.k_head + t * a.k_token;
+    const float x = live ? __bfloat162float(v[t * a.v_token]) : 0.f;
+    const float g = a.decay[b * a.decay_row + h * a.decay_head + t * a.decay_token];
+    const bool near = fabsf(g) < 0.69314718f;
+    const float d = near ? expm1_near(g) : expf(g);
+    float o = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < a.k_dim; k += 2) {
+      const uint32_t k2 = *reinterpret_cast<const uint32_t*>(kt + k), q2 = *reinterpret_cast<const uint32_t*>(qt + k);
+      const float s0 = fmaf(lo_f(k2), x, fmaf(d, S(k), near ? S(k) : 0.f));
+      const float s1 = fmaf(hi_f(k2), x, fmaf(d, S(k + 1), near ? S(k + 1) : 0.f));
+      S(k) = s0, S(k + 1) = s1;
+      o = fmaf(lo_f(q2), s0, fmaf(hi_f(q2), s1, o));
+    }
+    o *= a.scale;
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + ((int64_t(b) * a.tokens + t) * a.v_heads + h) * a.v_dim + dv;
+    if (live && isfinite(o) && !isfinite(__bfloat162float(*out))) *out = __float2bfloat16_rn(o);
+  }
+}
+
 // What a segment adds to the state, and its decay.
 template <int DK>
 __global__ void __launch_bounds__(THREADS, 1) add_kernel(const __grid_constant__ Args A, const __grid_constant__ Maps maps) {
@@ -535,8 +589,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
     mbar_init(&B.o_full, 1), mbar_init(&B.o_empty, 4);
     for (int i = 0; i < 2; ++i) mbar_init(&B.kw_full[i], 4), mbar_init(&B.kw_empty[i], 1);
     mbar_init(&B.d_full, 1), mbar_init(&B.d_empty, 8), mbar_init(&B.s_full, 8), mbar_init(&B.s_empty, 1);
-    mbar_init(&B.done, 2);
-    B.bail = 0;
+    mbar_init(&B.ends, 8), mbar_init(&B.outs, 4), mbar_init(&B.done, 2);
+    B.bail = B.odd[0] = B.odd[1] = B.odd[2] = B.odd[3] = 0;
     fence_mbar_init();
   }
   if (warp == MMA_WARP) tmem_alloc(&B.tmem);
@@ -677,6 +731,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
                                   ((int64_t(b) * a.tokens + t1 + e / pieces) * a.v_heads + h) * a.v_dim + 8 * (e % pieces)) =
             make_uint4(0, 0, 0, 0);
       if (ot == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      out_sync();
+      if (n > 0 && wait(&B.ends, 0) && B.odd[warp & 3] && !*wait.bail)
+        mend_outputs<DK>(A, smem + L::Q, smem + L::P, int(quarter) + lane, c0 * C, min(len, (c0 + n) * C));
+      arrive(&B.outs);
     }
   } else if (warp < KW_WARP) {
     // ---- the state: value dimension `dv`, key dimensions k0 .. k0 + DK / 2 - 1
@@ -741,7 +799,14 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       arrive(&B.d_empty);
       arrive(&B.dec_empty[slot<RING>(i)]);
     }
+    float2 zero = make_float2(0.f, 0.f);  // NaN where a state is not finite
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) zero = __ffma2_rn(S[k], make_float2(0.f, 0.f), zero);
+    if (__any_sync(0xffffffffu, !(zero.x + zero.y == 0.f))) B.odd[warp & 3] = 1;
+    arrive(&B.ends);
     if (seg == A.segments - 1) {
+      // in place: the outputs may go back to the state before
+      if (A.segments == 1 && a.state_in == a.state_out) wait(&B.outs, 0);
       float* to = a.state_out + (head * a.k_dim + k0) * a.v_dim + dv;
       const int kd = dv < a.v_dim ? a.k_dim - k0 : 0;
 #pragma unroll

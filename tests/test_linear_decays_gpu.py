@@ -151,3 +151,62 @@ def test_a_broken_gate_shows(cuda, n, t, hk, hv, dk, dv, dtype, at, resets, stat
     out, state = check(q, k, v, g, S)
     assert out[0, at:, hv - 1].isnan().all() and state[0, hv - 1].isnan().all()
     assert not out[0, :at].isnan().any() and not out[0, :, : hv - 1].isnan().any()
+
+
+@pytest.mark.parametrize("value", [INF, -INF, NAN])
+@pytest.mark.parametrize("at", [0, 1, 40, 63, 64, 100, 149])
+@pytest.mark.parametrize("resets", [False, True])
+@pytest.mark.parametrize("n, t, hk, hv, dk, dv, dtype", LONG)
+def test_a_value_does_not_reach_earlier_tokens(cuda, n, t, hk, hv, dk, dv, dtype, resets, at, value):
+    """A value that is not finite, in a masked place for the tokens before it: their outputs are what they are without it,
+    and so are the other value dimensions and heads; from its token on its dimension is not finite."""
+    at = min(at, t - 1)
+    q, k, v, r, S = make(n, t, hk, hv, dk, dv, dtype)
+    g = -0.05 * r
+    if resets:
+        g[:, max(0, at - 20)] = -INF
+    O, F, OA, A = recurrence(q, k, v, g, S, dk ** -0.5)
+    u, e = U[dtype], (dk + 200 + 128 * 0.05) * E
+    v[0, at, hv - 1, 5] = value
+    v[0, min(t - 1, at + 3), hv - 1, dv - 1] = value
+    out, state = context.linear_attention(q, k, v, g, state=S)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[0, at:, hv - 1, 5] = True
+    bad[0, min(t - 1, at + 3) :, hv - 1, dv - 1] = True
+    assert not out[bad].isfinite().any() and not state[0, hv - 1, :, 5].isfinite().any()
+    ratio = torch.where(bad, 0.0, (out.double() - O).abs() / (u * O.abs() + (u * u + e) * OA + 1e-30 + LEAST[dtype]))
+    assert (ratio <= 1).all(), ratio.max().item()
+    _lib.check_device_errors()
+
+
+@pytest.mark.parametrize("t", [100, 1100])
+def test_in_place_with_a_value_that_is_not_finite(cuda, t):
+    """The library's call with one array for the state before and after: the same bits as with two."""
+    q, k, v, r, S = make(2, t, 2, 2, 128, 128, BF)
+    g = -0.05 * r
+    v[0, 70, 1, 9] = INF
+    v[1, 20, 0, 100] = NAN
+    out, state = context.linear_attention(q, k, v, g, state=S)
+    got, place, lib = torch.empty_like(out), S.clone(), _lib.lib()
+    strides = [x for y in (q, k, v, g) for x in y.stride()[:3]]
+    call = context._LINEAR.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), place.data_ptr(), place.data_ptr(),
+                                0, got.data_ptr(), *strides, 2, t, 2, 2, 128, 128, 2, 128 ** -0.5)
+    size = lib.sc_linear_attention_workspace(call)
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+    assert lib.sc_linear_attention(call, ws.data_ptr(), size, _lib.error_word().data_ptr(), _lib.stream()) == 0
+    assert torch.equal(got.view(torch.int16), out.view(torch.int16))
+    assert torch.equal(place.isnan(), state.isnan()) and torch.equal(place[state.isfinite()], state[state.isfinite()])
+    assert got[0, :70, 1, 9].isfinite().all() and got[1, :20, 0, 100].isfinite().all()
+    _lib.check_device_errors()
+
+
+def test_every_value_is_not_finite(cuda):
+    """The mending over all dimensions and heads of a long prompt, in several segments and in one."""
+    for n, hv in ((1, 2), (8, 16)):
+        q, k, v, r, S = make(n, 4096, 2, hv, 128, 128, BF)
+        v[:, 4000:] = NAN
+        out, state = context.linear_attention(q, k, v, -0.05 * r, state=S)
+        assert out[:, :4000].isfinite().all() and out[:, 4000:].isnan().all() and state.isnan().all()
+        want = context.linear_attention(*(x[:, :4000] for x in (q, k, v, -0.05 * r)), state=S)[0]
+        assert torch.allclose(out[:, :4000].float(), want.float(), rtol=2.0 ** -6, atol=1e-2)
+        _lib.check_device_errors()
