@@ -142,7 +142,20 @@ __device__ __forceinline__ void store_transposed(uint32_t at, uint32_t r0, uint3
                "r"(r3)
                : "memory");
 }
-__device__ __forceinline__ void out_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the output warps
+// the output warps; whether all of them go on: one that gave up its wait would leave the others at the barrier
+__device__ __forceinline__ void out_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool out_all(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(uint32_t(ok))
+      : "memory");
+  return all != 0;
+}
 
 __device__ __forceinline__ uint32_t bits_of(__nv_bfloat162 v) { return *reinterpret_cast<uint32_t*>(&v); }
 __device__ __forceinline__ float lo_f(uint32_t v) { return __uint_as_float(v << 16); }
@@ -674,10 +687,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_kernel(const __grid_constant
       const int token = (lane >> 4) * 8 + (lane & 7), piece = 4 * (warp & 3) + ((lane >> 3) & 1);
 #pragma unroll 1
       for (int i = 0; i < n; ++i) {
-        if (!wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.o_full, i)) break;
+        const bool ok = wait(&B.dec_full[slot<RING>(i)], phase<RING>(i), &B.o_full, i);
         fence_after();
         if (ot == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        out_sync();  // the tile's last store has read it
+        if (!out_all(ok)) break;  // and the tile's last store has read it
         const int t0 = (c0 + i) * C, m = len - t0;
         const float* eg = dec[slot<RING>(i)].eg;
 #pragma unroll 1
