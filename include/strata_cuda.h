@@ -303,7 +303,7 @@ SC_API int sc_rope_cache(void* q, const void* k, const void* v, int tokens, int 
  * slots) are optional to sc_decode_attention, position is not used by it; sc_evict needs both. */
 typedef struct sc_kv_pages {
   void *k, *v;                   /* pools of pool_pages pages, bfloat16 or float16, 16-byte aligned               */
-  int64_t k_page, k_token, k_head; /* strides, multiples of 8                                                     */
+  int64_t k_page, k_token, k_head; /* strides, multiples of 8 on axes of more than one entry                      */
   int64_t v_page, v_token, v_head;
   const int32_t* table;          /* (batch, max_pages) page ids, rows table_row apart                              */
   int64_t table_row;
@@ -315,15 +315,16 @@ typedef struct sc_kv_pages {
   int batch, kv_heads, head_dim, page, pool_pages, max_pages, dtype; /* page a power of two                         */
 } sc_kv_pages;
 
-/* Attention of one new token a sequence over its cache: out[b, h] = sum_s p[s] v[s, h / (q_heads / kv_heads)] with
- * p = softmax over s < lengths[b] of scale q[b, h] . k[s]; zeros where lengths[b] is 0 or every score is -inf. q (batch, q_heads, head_dim)
- * with strides q_row, q_head (multiples of 8, 16-byte aligned); out the same shape, contiguous, of q's type. Where
- * kv->weight is not NULL, weight[b, s] += sum over the query heads of p[s]. Softmax statistics and sums in float32,
- * the same bits on every run. head_dim a multiple of 8, at most 256; q_heads a multiple of kv_heads. Slots past a
- * length are never read. A value in use that is infinite or NaN makes its dimension's outputs infinite or NaN. A
- * page id outside the pool or a length outside the table records SC_ERR_PAGE in err; such slots are left out.
- * workspace: sc_decode_attention_workspace bytes, 16-byte aligned, not shared by calls that may overlap or whose
- * launches (two or three a call) may come between each other's on one stream. */
+/* Attention of one new token a sequence over its cache: out[b, h] = sum_s p[s] v[s, h / (q_heads / kv_heads)]
+ * with p = softmax over s < lengths[b] of scale q[b, h] . k[s]; zeros where lengths[b] is 0 or every score is -inf.
+ * q (batch, q_heads, head_dim) with strides q_row, q_head (multiples of 8 where the axis has more than one entry;
+ * 16-byte aligned); out the same shape, contiguous, of q's type. Where kv->weight is not NULL, weight[b, s] += sum
+ * over the query heads of p[s]. Softmax statistics and sums in float32, the same bits on every run. head_dim a
+ * multiple of 8, at most 256; q_heads a multiple of kv_heads. Slots past a length are never read. A value in use
+ * that is infinite or NaN makes its dimension's outputs infinite or NaN. A page id outside the pool or a length
+ * outside the table records SC_ERR_PAGE in err; such slots are left out. workspace: sc_decode_attention_workspace
+ * bytes, 16-byte aligned, not shared by calls that may overlap or whose launches (two or three a call) may come
+ * between each other's on one stream. */
 SC_API int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t q_row, int64_t q_head, int q_heads,
                                float scale, void* out, void* workspace, size_t workspace_bytes, int* err, void* stream);
 SC_API size_t sc_decode_attention_workspace(const sc_kv_pages* kv, int q_heads);
@@ -351,7 +352,7 @@ SC_API size_t sc_evict_workspace(const sc_kv_pages* kv, int keep);
  * sequence's length are not read and their outputs are zeros. A value that is not finite leaves the outputs of its
  * dimension from its token on and the dimension's state not finite (infinite or NaN), and nothing else. out (batch,
  * tokens, v_heads, v_dim) contiguous, of q's type. k_dim and v_dim multiples of 8, at most 128. Strides of q, k, v
- * multiples of 8, pointers 16-byte aligned. */
+ * multiples of 8 on axes of more than one entry, pointers 16-byte aligned. */
 typedef struct sc_linear {
   const void *q, *k, *v;
   const float* decay;

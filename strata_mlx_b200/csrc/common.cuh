@@ -210,6 +210,8 @@ int cuda_failed(cudaError_t e, const char* where);
 // The record is per kernel: several host paths that launch one kernel with different sizes share it.
 int raise_smem(const void* kern, int bytes, const char* where);
 
+// the stride of an axis of n entries, as far as it is ever taken
+__host__ __device__ constexpr int64_t used(int n, int64_t stride) { return n > 1 ? stride : 0; }
 __host__ __device__ constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 __host__ __device__ constexpr int align16(int v) { return (v + 15) & ~15; }
 

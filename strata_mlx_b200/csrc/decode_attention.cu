@@ -689,7 +689,7 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
   if (int rc = check_pages(kv)) return rc;
   if (kv->batch && (!q || !out || !workspace)) return SC_ERR_ARG;
   if (q_heads < 1 || q_heads % kv->kv_heads || q_heads > 2048) return SC_ERR_SHAPE;
-  if (((q_row | q_head) & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
+  if (((used(kv->batch, q_row) | used(q_heads, q_head)) & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & 15))
     return SC_ERR_ALIGN;
   const da::Layout l = da::layout(*kv, q_heads);

@@ -158,8 +158,8 @@ inline int check(const sc_linear* a) {
   if (a->k_heads < 1 || a->v_heads < 1 || a->v_heads % a->k_heads || a->k_dim < 8 || a->k_dim % 8 || a->k_dim > MAXK ||
       a->v_dim < 8 || a->v_dim % 8 || a->v_dim > 128 || a->batch > 65535 || a->v_heads > 65535)
     return SC_ERR_SHAPE;
-  const int64_t strides = a->q_row | a->q_token | a->q_head | a->k_row | a->k_token | a->k_head | a->v_row | a->v_token |
-                          a->v_head;
+  const int64_t strides = used(a->batch, a->q_row | a->k_row | a->v_row) | used(a->tokens, a->q_token | a->k_token | a->v_token) |
+                          used(a->k_heads, a->q_head | a->k_head) | used(a->v_heads, a->v_head);
   const uintptr_t p = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) |
                       reinterpret_cast<uintptr_t>(a->v) | reinterpret_cast<uintptr_t>(a->out) |
                       reinterpret_cast<uintptr_t>(a->state_in) | reinterpret_cast<uintptr_t>(a->state_out);

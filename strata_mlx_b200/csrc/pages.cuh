@@ -50,7 +50,8 @@ inline int check_pages(const sc_kv_pages* c) {
       c->max_pages < 1 || c->page < 1 || c->page > 4096 || (c->page & (c->page - 1)) ||
       int64_t(c->max_pages) * c->page > (int64_t(1) << 30) || c->batch > 65535)
     return SC_ERR_SHAPE;
-  const int64_t strides = c->k_page | c->k_token | c->k_head | c->v_page | c->v_token | c->v_head;
+  const int64_t strides = used(c->pool_pages, c->k_page | c->v_page) | used(c->page, c->k_token | c->v_token) |
+                          used(c->kv_heads, c->k_head | c->v_head);
   if ((strides & 7) || ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15))
     return SC_ERR_ALIGN;
   return SC_OK;
