@@ -74,6 +74,8 @@ class KVPages:
             if t is not None and (t.dtype != dtype or t.dim() != 2 or t.shape[0] != self.batch or t.stride(1) != 1
                                   or t.shape[1] < self.slots):
                 raise ValueError(f"{name}: {dtype} ({self.batch}, at least {self.slots}) expected")
+            if t is not None and self.batch > 1 and t.stride(0) < self.slots:
+                raise ValueError(f"{name}: the sequences' rows overlap")
         self.k, self.v, self.table, self.lengths, self.weight, self.position = k, v, table, lengths, weight, position
         self.dtype, self.kv_heads, self.head_dim = k.dtype, k.shape[2], k.shape[3]
         P = _lib.SCPages()
@@ -162,6 +164,8 @@ class KVPages:
                 if (t.get_device() != index or t.dtype != dtype or len(shape) != 2 or shape[0] != n or shape[1] < room
                         or t.stride(1) != 1):
                     raise ValueError(f"out {name}: {dtype} ({n}, at least {room}) on {self.device} expected")
+                if n > 1 and t.stride(0) < room:
+                    raise ValueError(f"out {name}: the sequences' rows overlap")
             if lengths.get_device() != index:
                 raise ValueError(f"out lengths: on {self.device} expected")
             _ints("out lengths", lengths, (n,))

@@ -96,3 +96,21 @@ def test_a_budget_past_32_bits_is_refused(cache, keep):
     assert not lib.calls
     c.evict(c.lengths.clone(), (1 << 31) - 1, sinks=0)
     assert lib.calls[0][1][2] == (1 << 31) - 1
+
+
+def test_rows_that_are_written_may_not_overlap(cache):
+    """Sequences are worked on side by side: one row of weights for several would be a race."""
+    c, lib = cache
+    kv = c.k, c.v, c.table, c.lengths
+    one, pos = torch.zeros((1, 32)), torch.zeros((2, 32), dtype=torch.int32)
+    for bad in (dict(weight=one.expand(2, -1)), dict(weight=torch.zeros(48).as_strided((2, 32), (16, 1))),
+                dict(weight=c.weight, position=pos[:1].expand(2, -1))):
+        with pytest.raises(ValueError, match="overlap"):
+            context.KVPages(*kv, **bad)
+    for out in ((one.expand(2, -1), pos, c.lengths), (torch.zeros((2, 32)), pos[:1].expand(2, -1), c.lengths)):
+        with pytest.raises(ValueError, match="overlap"):
+            c.evict(c.lengths.clone(), 12, sinks=0, out=out)
+    alone = context.KVPages(c.k, c.v, c.table[:1], c.lengths[:1], weight=one.as_strided((1, 32), (0, 1)))
+    alone._index = -1
+    alone.attend(torch.zeros((1, 4, 64), dtype=torch.bfloat16))
+    assert [name for name, _ in lib.calls] == ["attend"]
