@@ -25,7 +25,7 @@
 // segment's chunks from the last to the first, the weights w running on from chunk to chunk, so that D of eight chunks
 // adds up in tensor memory and no state is carried between them.
 // What bounds it at 128 dimensions, a chunk: 64 KB of loads and stores (1.5 us of an SM's share of the measured copy),
-// 1,792 tensor cycles (A, of 64 rows, runs at half rate), 9,600 warp instructions (2,400 cycles of issue), and the chain
+// 1,792 tensor cycles (A, of 64 rows, runs at half rate), 9,800 warp instructions (2,450 cycles of issue), and the chain
 // state -> its terms -> X -> state, which sets the pace: 3,500 cycles where a block is alone, 3,900 with all SMs at work.
 // A loop's code counts twice: 24 warps in eight roles share the instruction cache, and what does not fit is fetched
 // again every chunk (kernel of 116 KB: 282 us for 32768 tokens of 16 heads, 70 KB: 195, 61 KB: 184). So loops are rolled, an
@@ -347,25 +347,28 @@ __device__ __forceinline__ uint2 take_resets(float2& g) {
 }
 
 // A value that is not finite meets P's zeros (0 times it is NaN) and so reaches the tokens before it in its chunk. It stays
-// in the state, whatever follows; so a segment whose state at its end is finite had none, and the chunks need not look. In
-// another the outputs are mended behind its last chunk: the recurrence from the state before the segment up to the last
-// token whose value is the first that is not finite of its dimension, a lane a dimension, the state in two places of shared
-// memory that the products have done with. What is not finite among the outputs and is in the recurrence is replaced.
+// in the state, whatever follows; so a segment whose state at its end is finite had none, and the chunks need not look (in
+// the output warps a look through a chunk's values took 2.3 of 54 us, in others more). In another segment the outputs are
+// mended behind its last chunk: the recurrence from the state before the segment up to the last token whose value is the
+// first that is not finite of its dimension, a lane a dimension, the state in two places of shared memory that the products
+// have done with. What is not finite among the outputs and is in the recurrence is replaced. Measured: 3 us a token
+// (one prompt of 32768 tokens, 16 heads, with a NaN near its end 11.8 ms, without 0.22).
 template <int DK>
 __device__ __forceinline__ void mend_outputs(const Args& A, uint8_t* place0, uint8_t* place1, int dv, int t0, int t1) {
   const sc_linear& a = A.a;
   const int seg = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / (a.v_heads / a.k_heads);
   const bool live = dv < a.v_dim;
   const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v) + b * a.v_row + h * a.v_head + (live ? dv : 0);
-  int last = t0;
-  bool seen = !live;
-#pragma unroll 4
+  int odd = INT32_MAX;  // the dimension's first token with such a value
+#pragma unroll 8
   for (int t = t0; t < t1; ++t)
-    if (!isfinite(__bfloat162float(v[t * a.v_token])) && !seen) seen = true, last = t;
-  last = __reduce_max_sync(0xffffffffu, last);
+    if (!isfinite(__bfloat162float(v[t * a.v_token]))) odd = min(odd, t);
+  if (!live) odd = INT32_MAX;
+  const int first = __reduce_min_sync(0xffffffffu, odd) / C * C;
+  const int last = __reduce_max_sync(0xffffffffu, odd == INT32_MAX ? t0 : odd);
   if (last == t0) return;
   constexpr int FIRST = QS * DK / 64 * HALF / 512;  // rows of 128 values in place0
-  static_assert((DK - FIRST) * 512 <= 2 * HALF, "the state's places");
+  static_assert((DK - FIRST) * 512 <= 2 * HALF && FIRST % 8 == 0, "the state's places");
   auto S = [&](int k) -> float& { return reinterpret_cast<float*>(k < FIRST ? place0 + 512 * k : place1 + 512 * (k - FIRST))[dv]; };
   const int64_t head = int64_t(b) * a.v_heads + h;
   if (A.segments > 1) pdl_wait();
@@ -378,20 +381,31 @@ __device__ __forceinline__ void mend_outputs(const Args& A, uint8_t* place0, uin
   }
 #pragma unroll 1
   for (int t = t0; t < last; ++t) {
-    const __nv_bfloat16* qt = static_cast<const __nv_bfloat16*>(a.q) + b * a.q_row + hk * a.q_head + t * a.q_token;
     const __nv_bfloat16* kt = static_cast<const __nv_bfloat16*>(a.k) + b * a.k_row + hk * a.k_head + t * a.k_token;
     const float x = live ? __bfloat162float(v[t * a.v_token]) : 0.f;
     const float g = a.decay[b * a.decay_row + h * a.decay_head + t * a.decay_token];
     const bool near = fabsf(g) < 0.69314718f;
-    const float d = near ? expm1_near(g) : expf(g);
+    const float d = near ? expm1_near(g) : expf(g), one = near ? 1.f : 0.f;
+#pragma unroll 1
+    for (int k = 0; k < a.k_dim; k += 8) {  // loads before stores: they would wait for one another
+      const uint4 k8 = *reinterpret_cast<const uint4*>(kt + k);
+      const uint32_t w[4] = {k8.x, k8.y, k8.z, k8.w};
+      float* at = &S(k);
+      float r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = at[128 * e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = fmaf(d, r[e], fmaf(one, r[e], (e & 1 ? hi_f(w[e / 2]) : lo_f(w[e / 2])) * x));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) at[128 * e] = r[e];
+    }
+    if (t < first) continue;
+    const __nv_bfloat16* qt = static_cast<const __nv_bfloat16*>(a.q) + b * a.q_row + hk * a.q_head + t * a.q_token;
     float o = 0.f;
-#pragma unroll 4
+#pragma unroll 1
     for (int k = 0; k < a.k_dim; k += 2) {
-      const uint32_t k2 = *reinterpret_cast<const uint32_t*>(kt + k), q2 = *reinterpret_cast<const uint32_t*>(qt + k);
-      const float s0 = fmaf(lo_f(k2), x, fmaf(d, S(k), near ? S(k) : 0.f));
-      const float s1 = fmaf(hi_f(k2), x, fmaf(d, S(k + 1), near ? S(k + 1) : 0.f));
-      S(k) = s0, S(k + 1) = s1;
-      o = fmaf(lo_f(q2), s0, fmaf(hi_f(q2), s1, o));
+      const uint32_t q2 = *reinterpret_cast<const uint32_t*>(qt + k);
+      o = fmaf(lo_f(q2), S(k), fmaf(hi_f(q2), S(k + 1), o));
     }
     o *= a.scale;
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + ((int64_t(b) * a.tokens + t) * a.v_heads + h) * a.v_dim + dv;
