@@ -1,7 +1,6 @@
 """What a decoder keeps of its context, for a batch of sequences: a paged key/value cache that can be held to a budget,
-and linear attention, whose state has one size at any length. The reference's engine keeps both kinds
-(strata_mlx/engine.py:276-279 runs a trunk of linear and of full attention layers around the MoE blocks); these are
-the operators for such a trunk on the B200.
+and linear attention, whose state has one size at any length. Additions for a serving decoder around the MoE blocks (the
+reference keeps one conversation, and its trunk's recurrent layers follow a delta rule, which this is not):
 
     KVPages                 a batch's cache: pools of pages, a table and a length a sequence
       .attend(q)            attention of one new token a sequence; the weights each slot gathers, on request

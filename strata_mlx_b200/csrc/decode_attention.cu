@@ -10,7 +10,7 @@
 //   starts_kernel  first, for more than two sequences for each thread of an attending block: how many units lie before
 //                  each. (Up to as many, every block counts them itself: 129 of up to 512 tokens 28 us, with this kernel
 //                  32. Past it that took passes in every block of both kernels: 4096 rows of up to 512 tokens, 16 / 2
-//                  heads of 256, 1080 us, with this kernel 783; 65535 of up to 64, heads of 64, 134 ms and 3.8.)
+//                  heads of 256, 1080 us, with this kernel 778; 65535 of up to 64, heads of 64, 134 ms and 3.8.)
 //
 // A warp's tile goes from memory straight into tensor-core fragments (mma.sync m16n8k16; up to eight query heads share
 // the key/value head, so a product of 16 slots by 8 heads has little padding, and 128-row tcgen05 products would
@@ -26,9 +26,10 @@
 // there the maximum moves with every larger score and stands at 2^15: a probability is within 2^-22 of itself, and where
 // its terms run out of bits within 2^-40 of the largest (with the peak at 1 a tail of slots below 2^-25 behind it was
 // missing from the output). The next tile's keys load while this tile's softmax and value product run, its values after.
-// Measured: 8 sequences of 131072 tokens, 16 / 2 heads of 256, 326 to 330 us (6.5 TB/s, what a copy reaches); one of 8192
-// 13 us, of which the bytes are 2.6: the launch, one or two tiles a warp, the join. 32 ragged sequences to 9001, 32 / 8
-// heads of 128: 116 us (5.5 TB/s), with the weights gathered 131 (the scores' write and the join's read of them).
+// Measured: 8 sequences of 131072 tokens, 16 / 2 heads of 256, 325 to 330 us (6.5 TB/s, what a copy reaches); one of 8192
+// 11.8 us, of which the bytes are 2.6: the launch, one or two tiles a warp, the join. 32 ragged sequences to 9001, 32 / 8
+// heads of 128: 115 us (5.6 TB/s), with the weights gathered 125 (the scores' write and the join's read of them). Heads of
+// 256 take all 255 registers and spill 84 bytes of stores and 124 of loads a thread.
 #include <algorithm>
 #include <type_traits>
 
@@ -689,8 +690,8 @@ extern "C" int sc_decode_attention(const sc_kv_pages* kv, const void* q, int64_t
   if (int rc = check_pages(kv)) return rc;
   if (kv->batch && (!q || !out || !workspace)) return SC_ERR_ARG;
   if (q_heads < 1 || q_heads % kv->kv_heads || q_heads > 2048) return SC_ERR_SHAPE;
-  if (((used(kv->batch, q_row) | used(q_heads, q_head)) & 7) || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
-      (reinterpret_cast<uintptr_t>(out) & 15))
+  if (((used(kv->batch, q_row) | used(q_heads, q_head)) & 7) ||
+      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(out)) & 15))
     return SC_ERR_ALIGN;
   const da::Layout l = da::layout(*kv, q_heads);
   if (workspace_bytes < l.bytes) return SC_ERR_WORKSPACE;

@@ -158,7 +158,8 @@ inline int check(const sc_linear* a) {
   if (a->k_heads < 1 || a->v_heads < 1 || a->v_heads % a->k_heads || a->k_dim < 8 || a->k_dim % 8 || a->k_dim > MAXK ||
       a->v_dim < 8 || a->v_dim % 8 || a->v_dim > 128 || a->batch > 65535 || a->v_heads > 65535)
     return SC_ERR_SHAPE;
-  const int64_t strides = used(a->batch, a->q_row | a->k_row | a->v_row) | used(a->tokens, a->q_token | a->k_token | a->v_token) |
+  const int64_t strides = used(a->batch, a->q_row | a->k_row | a->v_row) |
+                          used(a->tokens, a->q_token | a->k_token | a->v_token) |
                           used(a->k_heads, a->q_head | a->k_head) | used(a->v_heads, a->v_head);
   const uintptr_t p = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) |
                       reinterpret_cast<uintptr_t>(a->v) | reinterpret_cast<uintptr_t>(a->out) |
@@ -182,9 +183,11 @@ int launch(const sc_linear& a, void* stream) {
 
 using namespace sc;
 
-// Prompts of bfloat16 go to the tensor cores; float16 ones, whose states can pass what float16 terms hold, broadcast
-// axes, and a few tokens, which a chunk's products would mostly pad, to the recurrence (16 heads of 128 x 128, one
-// sequence of 8 tokens: 5.4 us, in a chunk 7.7; 32 heads, 16 sequences: 29.0 and 29.8 at 8 tokens, 35.5 and 29.9 at 12).
+// Prompts of bfloat16 go to the tensor cores. To the recurrence go a few tokens, which a chunk's products would mostly pad
+// (16 heads of 128 x 128, one sequence of 8 tokens: 5.4 us, in a chunk 7.7; 32 heads, 16 sequences: 29.0 and 29.8 at 8
+// tokens, 35.5 and 29.9 at 12), and what the chunks are not built for: broadcast axes (a map takes no stride of zero) and
+// float16 (the states need bfloat16's exponents; queries, keys and values would enter as two bfloat16 terms each). That
+// is slow for long ones: 0.31 us a token.
 static bool chunked(const sc_linear& a) { return a.tokens > la::FEW && lc::takes(a); }
 
 extern "C" size_t sc_linear_attention_workspace(const sc_linear* a) {

@@ -1,8 +1,7 @@
 """A small synthetic decoder on the context operators (context.py): a batch of sequences through a trunk of linear and
-of full attention layers around the MoE blocks, the shape of trunk the reference's engine runs
-(strata_mlx/engine.py:276-279). What a sequence keeps is bounded at any length: a state a linear layer, and a cache
-of `capacity` slots a full attention layer, cut to the `keep` tokens that gathered the most attention weight whenever
-it is full.
+of full attention layers around the MoE blocks. What a sequence keeps is bounded at any length: a state a linear layer,
+and a cache of `capacity` slots a full attention layer, cut to the `keep` tokens that gathered the most attention weight
+whenever it is full.
 
     python -m strata_mlx_b200.hybrid [--batch 8] [--prompt 512] [--steps 64]
 
